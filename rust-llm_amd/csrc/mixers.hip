@@ -39,6 +39,15 @@ struct rl_kv_cache {
 struct rl_attention {
     int device = 0;
     uint32_t max_rows = 0, q_heads = 0, kv_heads = 0, dim = 0, max_len = 0;
+    uint64_t slots = 0; // partial results of a row and head
+    float *part_out = nullptr;
+    float2 *part_sum = nullptr;
+    uint32_t *part_count = nullptr;
+    ~rl_attention() {
+        (void)hipFree(part_out);
+        (void)hipFree(part_sum);
+        (void)hipFree(part_count);
+    }
 };
 
 struct rl_delta {
@@ -141,6 +150,19 @@ int check_cache_rows(const rl_kv_cache *c, const rl_heads *k, const rl_heads *v,
     if (!slots) return fail(RL_ERR_ARGUMENT, "slots must be a device pointer");
     if (rows > MAX_ROWS) return fail(RL_ERR_CAPACITY, "more than 2^23 rows in a call");
     return RL_OK;
+}
+
+// Parts of a row's length are at most ATTEND_LONG tokens, so that a batch of very
+// different lengths is shared out evenly, and otherwise as many as give each CU
+// the workgroups it holds at a time, each a tile of 32 tokens a wave or more.
+constexpr uint32_t ATTEND_LONG = 1536, CUS = 256;
+
+uint32_t attend_tiles(uint64_t tokens) { return (uint32_t)((tokens + ATTEND_TILE - 1) / ATTEND_TILE) + 1; }
+
+// Parts that lengths up to `tiles` need at the least.
+uint32_t attend_least_parts(uint32_t tiles) {
+    const uint32_t n = (tiles + ATTEND_LONG / ATTEND_TILE - 1) / (ATTEND_LONG / ATTEND_TILE);
+    return std::min(n, ATTEND_MAX_PARTS);
 }
 
 int launched(const char *what) {
@@ -394,6 +416,18 @@ int rl_attention_create(int device, uint32_t max_rows, uint32_t q_heads, uint32_
     if (!a) return fail(RL_ERR_CAPACITY, "out of host memory");
     a->device = device;
     a->max_rows = max_rows, a->q_heads = q_heads, a->kv_heads = kv_heads, a->dim = dim, a->max_len = max_len;
+    // Room for the least parts of every row, and for as many workgroups of 32 rows as the device holds.
+    const uint64_t heads = (uint64_t)max_rows * q_heads;
+    a->slots = std::max<uint64_t>(heads * attend_least_parts(attend_tiles(max_len)), CUS * 3 * 32);
+    hipError_t e = hipMalloc(&a->part_out, a->slots * attend_dim(dim) * sizeof(float));
+    if (e == hipSuccess) e = hipMalloc(&a->part_sum, a->slots * sizeof(float2));
+    if (e == hipSuccess) e = hipMalloc(&a->part_count, heads * sizeof(uint32_t));
+    if (e == hipSuccess) e = hipMemset(a->part_count, 0, heads * sizeof(uint32_t));
+    if (e == hipSuccess) e = hipDeviceSynchronize();
+    if (e != hipSuccess) {
+        delete a;
+        return hip_fail(e, "rl_attention_create");
+    }
     *out = a;
     return RL_OK;
 }
@@ -425,6 +459,7 @@ int rl_attention_rows(rl_attention *h, const rl_kv_cache *cache, const rl_heads 
     if (rows == 0) return RL_OK;
     if (!lens || !pages || table_width == 0) return fail(RL_ERR_ARGUMENT, "lens and pages must be device pointers");
     if (seqs == 0 || (!starts && seqs != rows)) return fail(RL_ERR_ARGUMENT, "without starts there is one row a sequence");
+    if (window > 0x7FFFFFFFu) window = 0; // no length is above it
     DeviceGuard guard(h->device);
     if (!guard.ok) return fail(RL_ERR_DEVICE, "cannot select the handle's device");
     AttendArgs a{};
@@ -437,11 +472,29 @@ int rl_attention_rows(rl_attention *h, const rl_kv_cache *cache, const rl_heads 
     a.most_rows = most_rows ? std::min(most_rows, rows) : rows;
     a.max_len = max_len ? max_len : h->max_len;
     a.scale = scale;
+    a.group = h->q_heads / h->kv_heads;
+    a.page_inv = (uint32_t)std::min<uint64_t>((1ull << 32) / cache->args.page, 0xFFFFFFFFu);
+    a.wide = wide(q) && wide(out);
+    a.part_out = h->part_out, a.part_sum = h->part_sum, a.part_count = h->part_count;
+    // Two row tiles a workgroup where a sequence has more than one: the keys and values are read once for both.
+    const uint64_t expanded = (uint64_t)a.most_rows * a.group;
+    const bool two = expanded > 16 && attend_two(type_bytes(q->dtype), cache->format, h->dim);
+    a.blocks = (uint32_t)((expanded + (two ? 31 : 15)) / (two ? 32 : 16));
+    const uint64_t columns = (uint64_t)seqs * h->kv_heads * a.blocks;
+    const uint64_t seen = window ? std::min<uint64_t>(a.max_len, (uint64_t)window + a.most_rows - 1) : a.max_len;
+    const uint32_t tiles = attend_tiles(seen);
+    const uint64_t room = std::min<uint64_t>(h->slots / ((uint64_t)rows * h->q_heads), ATTEND_MAX_PARTS);
+    const uint64_t held = CUS * attend_resident(type_bytes(q->dtype), cache->format, h->dim, two ? 2 : 1);
+    uint64_t parts = std::max<uint64_t>(held / columns, attend_least_parts(tiles));
+    parts = std::max<uint64_t>(std::min(parts, room), 1);
+    a.part_tiles = (uint32_t)((tiles + parts - 1) / parts);
+    a.part_tiles = (a.part_tiles + ATTEND_WAVES - 1) / ATTEND_WAVES * ATTEND_WAVES;
+    a.parts = (tiles + a.part_tiles - 1) / a.part_tiles;
+    // Jobs (sequence, head and part) in eights, the row blocks of each eight together.
+    const uint64_t groups = ((uint64_t)seqs * h->kv_heads * a.parts + 7) / 8 * 8 * a.blocks;
+    if (groups > 2 * MAX_ROWS - 1) return fail(RL_ERR_CAPACITY, "too many sequences times row blocks in a call");
     with_type(q->dtype, [&](auto t) {
-        with_format(cache->format, [&](auto f) {
-            hipLaunchKernelGGL((k_attend_rows<decltype(t), decltype(f)::value>), dim3(rows * h->q_heads),
-                               dim3(ATTEND_THREADS), 0, static_cast<hipStream_t>(stream), a);
-        });
+        launch_attend<decltype(t)>(a, cache->format, two, (uint32_t)groups, static_cast<hipStream_t>(stream));
     });
     return launched("rl_attention_rows launch");
 }
