@@ -60,7 +60,6 @@ constexpr int attend_resident(uint32_t query_bytes, uint32_t format, uint32_t di
     }
 }
 
-typedef vec<float, 4> f32x4;
 typedef vec<uint32_t, 4> u32x4;
 
 __device__ inline f32x4 mfma(vec<half_t, 8> a, vec<half_t, 8> b, f32x4 c) {

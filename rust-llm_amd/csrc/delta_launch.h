@@ -1,0 +1,38 @@
+// Launches of the delta rule's kernels for one element type (delta_*.hip, one unit
+// a type).
+#pragma once
+#include "delta_chunks.h"
+
+namespace rl {
+
+template <typename T>
+void launch_delta_steps(const DeltaArgs &a, hipStream_t s);
+template <typename T>
+void launch_delta_chunks(const DeltaArgs &a, const DeltaWork &w, hipStream_t s);
+
+#ifdef RL_DELTA_UNIT
+template <typename T>
+void launch_delta_steps(const DeltaArgs &a, hipStream_t s) {
+    constexpr uint32_t PER = DELTA_COLS * DELTA_WAVES;
+    auto kern = a.key_dim <= 64 ? k_delta_steps<T, 4> : a.key_dim <= 128 ? k_delta_steps<T, 8> : k_delta_steps<T, 16>;
+    hipLaunchKernelGGL(kern, dim3(a.seqs * a.value_heads, (a.value_dim + PER - 1) / PER), dim3(64 * DELTA_WAVES), 0, s, a);
+}
+
+template <typename T, int DK>
+void launch_delta_chunks_dim(const DeltaArgs &a, const DeltaWork &w, hipStream_t s) {
+    hipLaunchKernelGGL((k_delta_prepare<T, DK>), dim3((a.rows / CHUNK + a.seqs) * a.value_heads), dim3(256), 0, s, a, w);
+    const uint32_t jobs = (a.seqs * a.value_heads + 7) / 8 * 8;
+    hipLaunchKernelGGL((k_delta_chunks<T, DK>), dim3(jobs * (a.value_dim / 16)), dim3(256), 0, s, a, w);
+}
+
+template <typename T>
+void launch_delta_chunks(const DeltaArgs &a, const DeltaWork &w, hipStream_t s) {
+    switch (delta_dim(a.key_dim)) {
+    case 64: return launch_delta_chunks_dim<T, 64>(a, w, s);
+    case 128: return launch_delta_chunks_dim<T, 128>(a, w, s);
+    default: return launch_delta_chunks_dim<T, 256>(a, w, s);
+    }
+}
+#endif
+
+}  // namespace rl

@@ -15,6 +15,7 @@ typedef __bf16 bhalf_t;
 
 template <typename T, int N>
 using vec = T __attribute__((ext_vector_type(N)));
+typedef vec<float, 4> f32x4;
 
 // N values at p as f32. `wide`: p is a multiple of 16 bytes (of the vector's size, if that is less).
 template <int N, typename T>

@@ -9,7 +9,7 @@
 #include <vector>
 
 #include "attend.h"
-#include "delta.h"
+#include "delta_launch.h"
 #include "rl_runtime.h"
 
 using namespace rl;
@@ -53,6 +53,14 @@ struct rl_attention {
 struct rl_delta {
     int device = 0;
     uint32_t max_rows = 0, max_seqs = 0, key_heads = 0, value_heads = 0, key_dim = 0, value_dim = 0;
+    uint32_t chunks = 0; // that the workspace has room for
+    DeltaWork work{};
+    ~rl_delta() {
+        (void)hipFree(work.kt);
+        (void)hipFree(work.tm);
+        (void)hipFree(work.pm);
+        (void)hipFree(work.rows);
+    }
 };
 
 namespace {
@@ -164,6 +172,9 @@ uint32_t attend_least_parts(uint32_t tiles) {
     const uint32_t n = (tiles + ATTEND_LONG / ATTEND_TILE - 1) / (ATTEND_LONG / ATTEND_TILE);
     return std::min(n, ATTEND_MAX_PARTS);
 }
+
+// Rows of a sequence from which chunks are faster than one token after the other.
+constexpr uint32_t DELTA_CHUNKED = 32;
 
 int launched(const char *what) {
     const hipError_t e = hipGetLastError();
@@ -517,6 +528,23 @@ int rl_delta_create(int device, uint32_t max_rows, uint32_t max_seqs, uint32_t k
     d->device = device;
     d->max_rows = max_rows, d->max_seqs = max_seqs, d->key_heads = key_heads, d->value_heads = value_heads;
     d->key_dim = key_dim, d->value_dim = value_dim;
+    if (max_rows >= DELTA_CHUNKED) {
+        // Room for a prompt of every row, and for as many sequences as have 16 rows each on average, in f32.
+        d->chunks = max_rows / CHUNK + std::min(max_seqs, max_rows / 16 + 1);
+        const uint64_t heads = (uint64_t)d->chunks * value_heads;
+        if (heads > MAX_ROWS) {
+            delete d;
+            return fail(RL_ERR_CAPACITY, "chunks of max_rows times value_heads above 2^23");
+        }
+        hipError_t e = hipMalloc(&d->work.kt, d->chunks * (uint64_t)key_heads * kt_size(delta_dim(key_dim)) * sizeof(float));
+        if (e == hipSuccess) e = hipMalloc(&d->work.tm, heads * SQUARE * sizeof(float));
+        if (e == hipSuccess) e = hipMalloc(&d->work.pm, heads * SQUARE * sizeof(float));
+        if (e == hipSuccess) e = hipMalloc(&d->work.rows, heads * 4 * CHUNK * sizeof(float));
+        if (e != hipSuccess) {
+            delete d;
+            return hip_fail(e, "rl_delta_create");
+        }
+    }
     *out = d;
     return RL_OK;
 }
@@ -563,13 +591,12 @@ int rl_delta_rows(rl_delta *h, const rl_heads *q, const rl_heads *k, const rl_he
     a.key_dim = h->key_dim, a.value_dim = h->value_dim;
     a.scale = scale, a.eps = norm_eps;
     a.wide = wide(q) && wide(k) && wide(v) && wide(out);
-    (void)most_rows;
-    const uint32_t per = DELTA_COLS * DELTA_WAVES;
+    // Chunks where some sequence has the rows for them and the workspace holds all.
+    const uint32_t most = most_rows ? std::min(most_rows, rows) : rows;
+    const bool chunked = most >= DELTA_CHUNKED && rows / CHUNK + seqs <= h->chunks;
     with_type(q->dtype, [&](auto t) {
-        using T = decltype(t);
-        auto kern = h->key_dim <= 64 ? k_delta_steps<T, 4> : h->key_dim <= 128 ? k_delta_steps<T, 8> : k_delta_steps<T, 16>;
-        hipLaunchKernelGGL(kern, dim3(seqs * h->value_heads, (h->value_dim + per - 1) / per), dim3(64 * DELTA_WAVES), 0,
-                           static_cast<hipStream_t>(stream), a);
+        if (chunked) launch_delta_chunks<decltype(t)>(a, h->work, static_cast<hipStream_t>(stream));
+        else launch_delta_steps<decltype(t)>(a, static_cast<hipStream_t>(stream));
     });
     return launched("rl_delta_rows launch");
 }
