@@ -28,11 +28,15 @@ namespace rl {
 
 constexpr uint32_t CHUNK = 64;
 
-// Operands of the chunks, as fragments: for each of 64 lanes eight values, row
-// lane % 16 of a 16-row tile, columns 8 (lane / 16) on of a step of 32.
+// Operands of the chunks, zeros where a chunk or a head ends early, as fragments: for each of 64 lanes eight values, row
+// lane % 16 of a 16-row tile, columns 8 (lane / 16) on of a step of 32. K and
+// Q too: read where they are, a token's 4 KB or so from the next, all rows of a
+// head come from one channel of the L2 (3.1 us a chunk; 8192 tokens took 464 us).
 struct DeltaWork {
     void *kt;    // [chunk][key head][DK/16 tiles][2 steps]: K^T in the call's type
-    float *tm;   // [chunk][value head][4 tiles][2 steps]: T
+    void *kf;    // [chunk][key head][4 tiles][DK/32 steps]: K in the call's type
+    void *qf;    // the same of Q
+    bhalf_t *tm; // [chunk][value head][4 tiles][2 steps][3 parts]: T
     void *pm;    // [chunk][value head][4 tiles][2 steps]: P, bf16 for bf16 calls, else f32
     float *rows; // [chunk][value head][4][64]: factors of the rows of K S, of Q S and of U in the state; [3][0] e^c_n
 };
@@ -48,7 +52,7 @@ using p_type = std::conditional_t<std::is_same_v<T, bhalf_t>, bhalf_t, float>;
 constexpr int delta_dim(uint32_t key_dim) { return key_dim <= 64 ? 64 : key_dim <= 128 ? 128 : 256; }
 
 constexpr uint32_t FRAGMENT = 512, SQUARE = 4 * 2 * FRAGMENT; // values of a fragment, of a 64 x 64 operand
-constexpr uint32_t kt_size(uint32_t dk) { return dk / 16 * 2 * FRAGMENT; }
+constexpr uint32_t key_size(uint32_t dk) { return CHUNK * dk; } // of a chunk's K, Q or K^T
 
 // Chunks of sequence s start here: no two sequences share one.
 __device__ inline uint32_t first_chunk(const DeltaArgs &a, uint32_t s) { return first_row(a, s) / CHUNK + s; }
@@ -72,10 +76,10 @@ __device__ inline void mma_parts(const bf16x8 (&x)[NX], const bf16x8 (&y)[NY], f
 __device__ inline float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Eight consecutive values of a row as they are.
-template <typename T>
-__device__ inline vec<T, 8> load8(const T *p, bool wide) {
+template <bool WIDE, typename T>
+__device__ inline vec<T, 8> load8(const T *p) {
     vec<T, 8> x;
-    if (wide) {
+    if constexpr (WIDE) {
         constexpr int PER = 16 / sizeof(T);
 #pragma unroll
         for (int i = 0; i < 8; i += PER) {
@@ -119,11 +123,17 @@ __device__ inline void split_store(bhalf_t *to, uint32_t apart, f32x4 x) {
     }
 }
 
-// Values 8 (lane / 16) on of a step of q or k, of a row of the chunk; whatever stands there where there is none.
-template <typename T>
-__device__ inline vec<T, 8> row_fragment(const T *base, uint64_t stride, uint32_t row, uint32_t rows, uint32_t d, uint32_t dim,
-                                         bool wide) {
-    return load8(base + (uint64_t)(row < rows ? row : rows - 1) * stride + (d < dim ? d : 0), wide);
+// Values d on of a row of q or k of the chunk; whatever stands there where there is none.
+template <bool WIDE, typename T>
+__device__ inline vec<T, 8> row_fragment(const T *base, uint64_t stride, uint32_t row, uint32_t rows, uint32_t d, uint32_t dim) {
+    return load8<WIDE>(base + (uint64_t)(row < rows ? row : rows - 1) * stride + (d < dim ? d : 0));
+}
+
+// Calls f with true or false, known to the compiler: no load stands behind a branch of its own.
+template <typename F>
+__device__ inline void with_flag(bool x, F f) {
+    if (x) f(std::true_type{});
+    else f(std::false_type{});
 }
 
 // One workgroup a chunk and value head. The two Gram matrices are a row tile a
@@ -136,8 +146,8 @@ template <typename T, int DK>
 __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_delta_prepare(DeltaArgs a, DeltaWork w) {
     using TP = p_type<T>;
     constexpr int NP = parts_of<T>(), STEPS = DK / 32, LS = 68, KS = DK + 16 / (int)sizeof(T);
-    constexpr size_t K_BYTES = (size_t)CHUNK * KS * sizeof(T), L_BYTES = CHUNK * LS * 4, D_BYTES = 4 * 16 * 20 * 4;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[L_BYTES + D_BYTES > K_BYTES ? L_BYTES + D_BYTES : K_BYTES];
+    constexpr size_t K_BYTES = (size_t)CHUNK * KS * sizeof(T), L_BYTES = CHUNK * LS * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * L_BYTES > K_BYTES ? 2 * L_BYTES : K_BYTES];
     __shared__ double sums[CHUNK];
     __shared__ float betas[CHUNK], knorm[CHUNK], qnorm[CHUNK];
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
@@ -154,11 +164,20 @@ __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_de
     const uint32_t begin = first_row(a, s), end = first_row(a, s + 1), skip = (chunk - first_chunk(a, s)) * CHUNK;
     if (end <= begin || skip >= end - begin) return;
     const uint32_t row0 = begin + skip, rows = min(end - row0, CHUNK);
-    const bool clean = rows == CHUNK && a.key_dim == DK;
-    const T *q = (const T *)a.q + (uint64_t)row0 * a.q_row + key_head * a.q_head;
-    const T *k = (const T *)a.k + (uint64_t)row0 * a.k_row + key_head * a.k_head;
     const uint64_t at = (uint64_t)chunk * a.value_heads + head;
 
+    // The wave's 16 rows of Q and K, all on their way before the first is used.
+    vec<T, 8> xk[STEPS], xq[STEPS];
+    with_flag(a.wide, [&](auto wide) {
+        const T *q = (const T *)a.q + (uint64_t)row0 * a.q_row + key_head * a.q_head;
+        const T *k = (const T *)a.k + (uint64_t)row0 * a.k_row + key_head * a.k_head;
+#pragma unroll
+        for (int st = 0; st < STEPS; st++) {
+            const uint32_t row = wave * 16 + col, d = st * 32 + quad * 8;
+            xk[st] = row_fragment<decltype(wide)::value>(k, a.k_row, row, rows, d, a.key_dim);
+            xq[st] = row_fragment<decltype(wide)::value>(q, a.q_row, row, rows, d, a.key_dim);
+        }
+    });
     if (wave == 0) {
         // Sums of the decays, in powers of two. Below e^-200 every f32 is 0, and the sums stay finite.
         double c = 0.0;
@@ -176,37 +195,26 @@ __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_de
         sums[lane] = c;
         betas[lane] = b;
     }
-    // Gram matrices, the wave's 16 rows by the tiles up to its own.
-    auto fragment = [&](const T *base, uint64_t stride, int tile, int st) {
-        const uint32_t row = tile * 16 + col, d = st * 32 + quad * 8;
-        vec<T, 8> x = row_fragment(base, stride, row, rows, d, a.key_dim, a.wide);
-        if (!clean && (row >= rows || d >= a.key_dim)) x = vec<T, 8>{};
-        return x;
-    };
-    f32x4 kk[4], qk[4];
+    if (rows != CHUNK || a.key_dim != DK) {
 #pragma unroll
-    for (int t = 0; t < 4; t++) kk[t] = qk[t] = f32x4{0, 0, 0, 0};
+        for (int st = 0; st < STEPS; st++)
+            if (wave * 16 + col >= rows || st * 32 + quad * 8 >= a.key_dim) xk[st] = xq[st] = vec<T, 8>{};
+    }
+    const uint64_t keys = ((uint64_t)chunk * a.key_heads + key_head) * key_size(DK);
+    const bool first = head % share == 0; // of the key head's workgroups: writes what all share
     float kn = 0.0f, qn = 0.0f;
 #pragma unroll
     for (int st = 0; st < STEPS; st++) {
-        const vec<T, 8> xk = fragment(k, a.k_row, wave, st), xq = fragment(q, a.q_row, wave, st);
-        *(vec<T, 8> *)((T *)lds + (wave * 16 + col) * KS + st * 32 + quad * 8) = xk;
-        bf16x8 mine_k[NP], mine_q[NP];
-        split8(xk, mine_k);
-        split8(xq, mine_q);
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            kn = fmaf((float)xk[j], (float)xk[j], kn);
-            qn = fmaf((float)xq[j], (float)xq[j], qn);
+        *(vec<T, 8> *)((T *)lds + (wave * 16 + col) * KS + st * 32 + quad * 8) = xk[st];
+        if (first) {
+            const uint64_t f = keys + (wave * STEPS + st) * FRAGMENT + lane * 8;
+            *(vec<T, 8> *)((T *)w.kf + f) = xk[st];
+            *(vec<T, 8> *)((T *)w.qf + f) = xq[st];
         }
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            if (t > (int)wave) continue;
-            bf16x8 other[NP];
-            split8(fragment(k, a.k_row, t, st), other);
-            f32x4(&ka)[1] = *(f32x4(*)[1])&kk[t], (&qa)[1] = *(f32x4(*)[1])&qk[t];
-            mma_parts(mine_k, other, ka);
-            mma_parts(mine_q, other, qa);
+        for (int j = 0; j < 8; j++) {
+            kn = fmaf((float)xk[st][j], (float)xk[st][j], kn);
+            qn = fmaf((float)xq[st][j], (float)xq[st][j], qn);
         }
     }
     kn += __shfl_xor(kn, 16), qn += __shfl_xor(qn, 16);
@@ -216,17 +224,33 @@ __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_de
         qnorm[wave * 16 + col] = a.scale * (a.eps >= 0.0f ? 1.0f / sqrtf(qn + a.eps) : 1.0f);
     }
     __syncthreads();
-    // K^T, turned in LDS, by the first of the key head's workgroups.
-    if (head % share == 0) {
-        T *kt = (T *)w.kt + ((uint64_t)chunk * a.key_heads + key_head) * kt_size(DK);
+    // Gram matrices: these rows by the tiles of K up to their own.
+    f32x4 kk[4], qk[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) kk[t] = qk[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int st = 0; st < STEPS; st++) {
+        bf16x8 mine_k[NP], mine_q[NP];
+        split8(xk[st], mine_k);
+        split8(xq[st], mine_q);
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            if (t > (int)wave) continue;
+            bf16x8 other[NP];
+            split8(*(const vec<T, 8> *)((const T *)lds + (t * 16 + col) * KS + st * 32 + quad * 8), other);
+            f32x4(&ka)[1] = *(f32x4(*)[1])&kk[t], (&qa)[1] = *(f32x4(*)[1])&qk[t];
+            mma_parts(mine_k, other, ka);
+            mma_parts(mine_q, other, qa);
+        }
+    }
+    if (first) // K^T, turned in LDS
         for (uint32_t f = wave; f < DK / 16 * 2; f += 4) {
             vec<T, 8> x;
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = ((const T *)lds)[(f % 2 * 32 + quad * 8 + j) * KS + f / 2 * 16 + col];
-            *(vec<T, 8> *)(kt + f * FRAGMENT + lane * 8) = x;
+            *(vec<T, 8> *)((T *)w.kt + keys + f * FRAGMENT + lane * 8) = x;
         }
-    }
-    if (wave == 1) {
+    if (wave == 3) {
         const double c = sums[lane], whole = sums[CHUNK - 1];
         float *to = w.rows + at * 4 * CHUNK;
         const bool here = lane < rows;
@@ -235,65 +259,66 @@ __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_de
         to[2 * CHUNK + lane] = here ? fast_exp2((float)(whole - c)) * knorm[lane] : 0.0f;
         if (lane == 0) to[3 * CHUNK] = fast_exp2((float)whole);
     }
-    __syncthreads();
-    // P goes out through LDS, then L takes its place.
-    float *L = (float *)lds, *D = (float *)(lds + L_BYTES); // [64][LS]; [4][16][20]
-    f32x4 l[4];
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
+    for (int t = 0; t < 4; t++) { // L in place of kk, P of qk; rows and columns past the chunk's are zeros of both
         const uint32_t j = t * 16 + col;
         const double cj = sums[j];
         const float nj = knorm[j];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const uint32_t i = wave * 16 + quad * 4 + e;
-            float p = 0.0f;
-            l[t][e] = 0.0f;
-            if (j <= i) { // rows and columns past the chunk's are zeros of kk and qk
-                const float f = fast_exp2((float)(sums[i] - cj)) * nj;
-                p = qnorm[i] * (qk[t][e] * f);
-                if (j < i) l[t][e] = betas[i] * (knorm[i] * (kk[t][e] * f));
-            }
-            L[i * LS + j] = p;
+            const float f = fast_exp2((float)(sums[i] - cj)) * nj;
+            qk[t][e] = j <= i ? qnorm[i] * (qk[t][e] * f) : 0.0f;
+            kk[t][e] = j < i ? betas[i] * (knorm[i] * (kk[t][e] * f)) : 0.0f;
         }
     }
-    __syncthreads();
-    auto write_out = [&](auto *to) { // a wave a row tile, from its own rows of LDS
-        using V = std::remove_reference_t<decltype(*to)>;
-#pragma unroll
-        for (uint32_t st = 0; st < 2; st++) {
-            if (st * 32 > wave * 16) continue; // all zeros, not read
-            const float *x = L + (wave * 16 + col) * LS + st * 32 + quad * 8;
-            vec<V, 8> y;
-#pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = (V)x[j];
-            *(vec<V, 8> *)(to + (wave * 2 + st) * FRAGMENT + lane * 8) = y;
-        }
-    };
-    write_out((TP *)w.pm + at * SQUARE);
-    __syncthreads();
+    __syncthreads(); // the keys are used
+    float *L = (float *)lds, *P = L + CHUNK * LS; // [64][LS] each
 #pragma unroll
     for (int t = 0; t < 4; t++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) L[(wave * 16 + quad * 4 + e) * LS + t * 16 + col] = l[t][e];
+        for (int e = 0; e < 4; e++) {
+            const uint32_t f = (wave * 16 + quad * 4 + e) * LS + t * 16 + col;
+            L[f] = kk[t][e], P[f] = qk[t][e];
+        }
     __syncthreads();
-    if (wave == 0) { // D = (1 + L)^-1 of the diagonal blocks: lane 16 b + j has column j of block b
+    // A fragment's eight values out of P or what follows it there.
+    auto eight = [&](int tile, int st) {
+        vec<float, 8> y;
+        const f32x4 *x = (const f32x4 *)(P + (tile * 16 + col) * LS + st * 32 + quad * 8);
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] = x[j / 4][j % 4];
+        return y;
+    };
+    if (wave == 0) { // the diagonal blocks of (1 + L)^-1 in the place of L's: lane 16 b + j has column j of block b
         float x[16];
-        const float *Lb = L + quad * 16 * LS + quad * 16;
+        float *Lb = L + quad * 16 * LS + quad * 16;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            float y = i == (int)col ? 1.0f : 0.0f;
+            f32x4 y = {i == (int)col ? 1.0f : 0.0f, 0.0f, 0.0f, 0.0f}; // four sums: the chain is a quarter as long
 #pragma unroll
             for (int m = 0; m < i; m += 4) {
                 const f32x4 row = *(const f32x4 *)(Lb + i * LS + m); // zeros from the diagonal on
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    if (m + e < i) y = fmaf(-row[e], x[m + e], y);
+                    if (m + e < i) y[e] = fmaf(-row[e], x[m + e], y[e]);
             }
-            x[i] = y;
+            x[i] = (y[0] + y[1]) + (y[2] + y[3]);
         }
 #pragma unroll
-        for (int i = 0; i < 16; i++) D[(quad * 16 + i) * 20 + col] = x[i];
+        for (int i = 0; i < 16; i++) Lb[i * LS + col] = x[i];
+    } else { // meanwhile P goes out
+#pragma unroll
+        for (int tile = 0; tile < 4; tile++)
+#pragma unroll
+            for (int st = 0; st < 2; st++) {
+                if (st * 32 > tile * 16 || (tile ? tile : 1) != (int)wave) continue; // tiles 0 and 1 are the first wave's
+                const vec<float, 8> y = eight(tile, st);
+                vec<TP, 8> z;
+#pragma unroll
+                for (int j = 0; j < 8; j++) z[j] = (TP)y[j];
+                *(vec<TP, 8> *)((TP *)w.pm + at * SQUARE + (tile * 2 + st) * FRAGMENT + lane * 8) = z;
+            }
     }
     __syncthreads();
     f32x4 X[4];
@@ -303,7 +328,7 @@ __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_de
         if (i < (int)wave) continue;
         if (i == (int)wave) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) X[i][e] = D[(i * 16 + quad * 4 + e) * 20 + col];
+            for (int e = 0; e < 4; e++) X[i][e] = L[(i * 16 + quad * 4 + e) * LS + i * 16 + col];
             continue;
         }
         f32x4 sum = {0, 0, 0, 0};
@@ -314,39 +339,45 @@ __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_de
 #pragma unroll
             for (int e = 0; e < 4; e++) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], X[m][e], sum, 0, 0, 0);
         }
-        const f32x4 d = *(const f32x4 *)(D + (i * 16 + col) * 20 + quad * 4);
+        const f32x4 d = *(const f32x4 *)(L + (i * 16 + col) * LS + i * 16 + quad * 4);
 #pragma unroll
         for (int e = 0; e < 4; e++) X[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(-d[e], sum[e], X[i], 0, 0, 0);
     }
-    __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; i++) // block (i, wave) of the inverse, times beta of its columns
 #pragma unroll
-        for (int e = 0; e < 4; e++) L[(i * 16 + quad * 4 + e) * LS + wave * 16 + col] = X[i][e] * betas[wave * 16 + col];
+        for (int e = 0; e < 4; e++) P[(i * 16 + quad * 4 + e) * LS + wave * 16 + col] = X[i][e] * betas[wave * 16 + col];
     __syncthreads();
-    write_out(w.tm + at * SQUARE);
+#pragma unroll
+    for (int st = 0; st < 2; st++) {
+        if (st * 32 > (int)wave * 16) continue; // all zeros, not read
+        bf16x8 part[3];
+        split8(eight(wave, st), part);
+#pragma unroll
+        for (int p = 0; p < 3; p++)
+            *(bf16x8 *)(w.tm + (at * 8 + wave * 2 + st) * 3 * FRAGMENT + p * FRAGMENT + lane * 8) = part[p];
+    }
 }
 
 // What one chunk's step reads.
 template <typename T, int DK>
 struct DeltaChunk {
     vec<T, 8> k[DK / 32], q[DK / 32], kt[DK / 64][2];
-    vec<float, 8> t[2];
+    bf16x8 t[2][3];
     vec<p_type<T>, 8> p[2];
     f32x4 of_k, of_q, of_u;
     float keep;
-    T v[4];
+    uint32_t v[4]; // a value a register
 };
 
 // A workgroup has 16 columns of one head's state, wave w the rows DK/4 w on, and
 // of a chunk's tokens the 16 w on. State, right-hand sides and corrected values
 // pass between the waves through LDS as operands in parts (three barriers a chunk);
-// everything else comes from memory, loaded while the chunk two before is computed.
+// everything else comes from memory, loaded while the chunk before is computed.
 // Bound by the chain of a chunk: the products of a wave, and the three exchanges.
 template <typename T, int DK>
-__global__ void __launch_bounds__(256) k_delta_chunks(DeltaArgs a, DeltaWork w) {
+__global__ void __launch_bounds__(256, DK * sizeof(T) <= 256 ? 2 : 1) k_delta_chunks(DeltaArgs a, DeltaWork w) {
     constexpr int NP = parts_of<T>(), NO = out_parts<T>(), STEPS = DK / 32, TILES = DK / 64, SS = DK + 8, TS = 72;
-    constexpr bool AHEAD = DK * sizeof(T) <= 512; // two chunks' operands fit the registers
     __shared__ __attribute__((aligned(16))) bhalf_t state[3][16 * SS], right[3][16 * TS], values[NO][16 * TS], update[3][16 * TS];
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const uint32_t col = lane % 16, quad = lane / 16;
@@ -379,49 +410,60 @@ __global__ void __launch_bounds__(256) k_delta_chunks(DeltaArgs a, DeltaWork w) 
         }
     };
 
-    const T *q = (const T *)a.q + key_head * a.q_head, *k = (const T *)a.k + key_head * a.k_head;
     const T *v = (const T *)a.v + head * a.v_head + dv;
-    auto load = [&](uint32_t c, DeltaChunk<T, DK> &x) {
-        const uint64_t row0 = begin + c * CHUNK;
-        const uint32_t rows = min(n - c * CHUNK, CHUNK);
+    // Addresses are the wave's plus the lane's share.
+    auto fragment = [&](const auto *p) {
+        using V = std::remove_cv_t<std::remove_reference_t<decltype(*p)>>;
+        return ((const vec<V, 8> *)p)[lane];
+    };
+    // A chunk's operands, each loaded as soon as the chunk before has used its registers: a whole step ahead. No load is
+    // conditional (past the end the last chunk is loaded again), so that a wait is a count that leaves later loads on
+    // their way.
+    DeltaChunk<T, DK> x;
+    auto load_keys = [&](uint32_t c) {
+        const uint64_t keys = ((uint64_t)(chunk0 + c) * a.key_heads + key_head) * key_size(DK);
 #pragma unroll
         for (int st = 0; st < STEPS; st++) {
-            const uint32_t d = st * 32 + quad * 8;
-            x.k[st] = row_fragment(k + row0 * a.k_row, a.k_row, wave * 16 + col, rows, d, a.key_dim, a.wide);
-            x.q[st] = row_fragment(q + row0 * a.q_row, a.q_row, wave * 16 + col, rows, d, a.key_dim, a.wide);
+            x.k[st] = fragment((const T *)w.kf + keys + (wave * STEPS + st) * FRAGMENT);
+            x.q[st] = fragment((const T *)w.qf + keys + (wave * STEPS + st) * FRAGMENT);
         }
+    };
+    auto load_values = [&](uint32_t c) {
+        const uint32_t rows = min(n - c * CHUNK, CHUNK);
+        const T *vc = v + (uint64_t)(begin + c * CHUNK) * a.v_row;
 #pragma unroll
-        for (int i = 0; i < 4; i++) x.v[i] = v[(row0 + min(wave * 16 + quad * 4 + i, rows - 1)) * a.v_row];
+        for (int i = 0; i < 4; i++) {
+            using U = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+            x.v[i] = *(const U *)(vc + (uint64_t)min(wave * 16 + quad * 4 + i, rows - 1) * a.v_row);
+        }
+        x.of_k = ((const f32x4 *)(w.rows + ((uint64_t)(chunk0 + c) * a.value_heads + head) * 4 * CHUNK) + wave * 4)[quad];
+    };
+    auto load_system = [&](uint32_t c) {
         const uint64_t at = (uint64_t)(chunk0 + c) * a.value_heads + head;
-        const float *f = w.rows + at * 4 * CHUNK + wave * 16 + quad * 4;
-        x.of_k = *(const f32x4 *)f, x.of_q = *(const f32x4 *)(f + CHUNK), x.of_u = *(const f32x4 *)(f + 2 * CHUNK);
-        x.keep = w.rows[at * 4 * CHUNK + 3 * CHUNK];
 #pragma unroll
-        for (int st = 0; st < 2; st++) {
-            if (st * 32 > (int)wave * 16) continue; // all zeros: not written, not used
-            const uint64_t f = at * SQUARE + (wave * 2 + st) * FRAGMENT + lane * 8;
-            x.t[st] = *(const vec<float, 8> *)(w.tm + f);
-            x.p[st] = *(const vec<p_type<T>, 8> *)((const p_type<T> *)w.pm + f);
-        }
-        const T *kt = (const T *)w.kt + ((uint64_t)(chunk0 + c) * a.key_heads + key_head) * kt_size(DK);
+        for (int st = 0; st < 2; st++)
+            if (st * 32 <= (int)wave * 16) // else all zeros: not written, not used
+#pragma unroll
+                for (int p = 0; p < 3; p++) x.t[st][p] = fragment(w.tm + (at * 8 + wave * 2 + st) * 3 * FRAGMENT + p * FRAGMENT);
+        x.of_u = ((const f32x4 *)(w.rows + at * 4 * CHUNK) + CHUNK / 2 + wave * 4)[quad];
+    };
+    auto load_rest = [&](uint32_t c) {
+        const uint64_t keys = ((uint64_t)(chunk0 + c) * a.key_heads + key_head) * key_size(DK);
+        const uint64_t at = (uint64_t)(chunk0 + c) * a.value_heads + head;
+        x.keep = w.rows[at * 4 * CHUNK + 3 * CHUNK];
 #pragma unroll
         for (int m = 0; m < TILES; m++)
 #pragma unroll
-            for (int st = 0; st < 2; st++)
-                x.kt[m][st] = *(const vec<T, 8> *)(kt + ((wave * TILES + m) * 2 + st) * FRAGMENT + lane * 8);
+            for (int st = 0; st < 2; st++) x.kt[m][st] = fragment((const T *)w.kt + keys + ((wave * TILES + m) * 2 + st) * FRAGMENT);
+        x.of_q = ((const f32x4 *)(w.rows + at * 4 * CHUNK) + CHUNK / 4 + wave * 4)[quad];
+#pragma unroll
+        for (int st = 0; st < 2; st++)
+            if (st * 32 <= (int)wave * 16) x.p[st] = fragment((const p_type<T> *)w.pm + at * SQUARE + (wave * 2 + st) * FRAGMENT);
     };
 
-    auto step = [&](uint32_t c, DeltaChunk<T, DK> &x) {
+    auto step = [&](uint32_t c, uint32_t next) {
         const uint32_t rows = min(n - c * CHUNK, CHUNK);
-        const bool clean = rows == CHUNK && a.key_dim == DK;
-        if (!clean) { // what stands outside the chunk or the head may be anything
-#pragma unroll
-            for (int st = 0; st < STEPS; st++)
-                if (wave * 16 + col >= rows || st * 32 + quad * 8 >= a.key_dim) x.k[st] = x.q[st] = vec<T, 8>{};
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (wave * 16 + quad * 4 + i >= rows) x.v[i] = (T)0.0f;
-        }
+        const bool whole = rows == CHUNK;
         // K S and Q S for the wave's tokens.
         f32x4 ks[3], qs[3];
 #pragma unroll
@@ -442,13 +484,16 @@ __global__ void __launch_bounds__(256) k_delta_chunks(DeltaArgs a, DeltaWork w) 
         }
         f32x4 r;
 #pragma unroll
-        for (int i = 0; i < 4; i++) r[i] = (float)x.v[i] - x.of_k[i] * (ks[0][i] + (ks[1][i] + ks[2][i]));
+        for (int i = 0; i < 4; i++) {
+            using U = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+            r[i] = (float)__builtin_bit_cast(T, (U)x.v[i]);
+            if (!whole && wave * 16 + quad * 4 + i >= rows) r[i] = 0.0f;
+            r[i] -= x.of_k[i] * (ks[0][i] + (ks[1][i] + ks[2][i]));
+        }
         const uint32_t mine = col * TS + wave * 16 + quad * 4;
         split_store<3>(right[0] + mine, 16 * TS, r);
-        bf16x8 t[2][3];
-#pragma unroll
-        for (int st = 0; st < 2; st++)
-            if (st * 32 <= (int)wave * 16) split8(x.t[st], t[st]);
+        load_keys(next);
+        load_values(next);
         __syncthreads();
         // U = T R.
         f32x4 u[3];
@@ -459,11 +504,12 @@ __global__ void __launch_bounds__(256) k_delta_chunks(DeltaArgs a, DeltaWork w) 
             bf16x8 b[3];
 #pragma unroll
             for (int p = 0; p < 3; p++) b[p] = *(const bf16x8 *)(right[p] + col * TS + st * 32 + quad * 8);
-            mma_parts(t[st], b, u);
+            mma_parts(x.t[st], b, u);
         }
         u[0] += u[1] + u[2];
         split_store<3>(update[0] + mine, 16 * TS, u[0] * x.of_u);
         split_store<NO>(values[0] + mine, 16 * TS, u[0]);
+        load_system(next);
         __syncthreads();
         // The state, and out = Q S + P U.
         f32x4 add[TILES][3];
@@ -499,36 +545,28 @@ __global__ void __launch_bounds__(256) k_delta_chunks(DeltaArgs a, DeltaWork w) 
             split8(x.p[st], p);
             mma_parts(p, b, o);
         }
-        T *out = (T *)a.out + head * a.out_head + dv;
+        load_rest(next);
+        T *out = (T *)a.out + (uint64_t)(begin + c * CHUNK) * a.out_row + head * a.out_head + dv;
+        auto write = [&](int i) { out[(uint64_t)(wave * 16 + quad * 4 + i) * a.out_row] = (T)(o[0][i] + (o[1][i] + o[2][i])); };
+        if (whole) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t row = c * CHUNK + wave * 16 + quad * 4 + i;
-            if (row < n) out[(uint64_t)(begin + row) * a.out_row] = (T)(o[0][i] + (o[1][i] + o[2][i]));
-        }
+            for (int i = 0; i < 4; i++) write(i);
+        } else
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (wave * 16 + quad * 4 + i < rows) write(i);
         __syncthreads();
     };
 
     publish();
-    DeltaChunk<T, DK> x;
-    if (chunks > 0) load(0, x);
-    if constexpr (AHEAD) {
-        DeltaChunk<T, DK> y;
-        if (chunks > 1) load(1, y);
-        __syncthreads();
-        for (uint32_t c = 0; c < chunks; c += 2) {
-            step(c, x);
-            if (c + 2 < chunks) load(c + 2, x);
-            if (c + 1 >= chunks) break;
-            step(c + 1, y);
-            if (c + 3 < chunks) load(c + 3, y);
-        }
-    } else {
-        __syncthreads();
-        for (uint32_t c = 0; c < chunks; c++) {
-            step(c, x);
-            if (c + 1 < chunks) load(c + 1, x);
-        }
+    __syncthreads();
+    if (chunks > 0) {
+        load_keys(0);
+        load_values(0);
+        load_system(0);
+        load_rest(0);
     }
+    for (uint32_t c = 0; c < chunks; c++) step(c, min(c + 1, chunks - 1));
     if (to < 0 || (uint64_t)to >= a.state_slots) return;
     float *dst = a.states + ((uint64_t)to * a.value_heads + head) * size + dv;
 #pragma unroll

@@ -57,6 +57,8 @@ struct rl_delta {
     DeltaWork work{};
     ~rl_delta() {
         (void)hipFree(work.kt);
+        (void)hipFree(work.kf);
+        (void)hipFree(work.qf);
         (void)hipFree(work.tm);
         (void)hipFree(work.pm);
         (void)hipFree(work.rows);
@@ -536,8 +538,11 @@ int rl_delta_create(int device, uint32_t max_rows, uint32_t max_seqs, uint32_t k
             delete d;
             return fail(RL_ERR_CAPACITY, "chunks of max_rows times value_heads above 2^23");
         }
-        hipError_t e = hipMalloc(&d->work.kt, d->chunks * (uint64_t)key_heads * kt_size(delta_dim(key_dim)) * sizeof(float));
-        if (e == hipSuccess) e = hipMalloc(&d->work.tm, heads * SQUARE * sizeof(float));
+        const uint64_t keys = (uint64_t)d->chunks * key_heads * key_size(delta_dim(key_dim)) * sizeof(float);
+        hipError_t e = hipMalloc(&d->work.kt, keys);
+        if (e == hipSuccess) e = hipMalloc(&d->work.kf, keys);
+        if (e == hipSuccess) e = hipMalloc(&d->work.qf, keys);
+        if (e == hipSuccess) e = hipMalloc(&d->work.tm, heads * 3 * SQUARE * sizeof(bhalf_t));
         if (e == hipSuccess) e = hipMalloc(&d->work.pm, heads * SQUARE * sizeof(float));
         if (e == hipSuccess) e = hipMalloc(&d->work.rows, heads * 4 * CHUNK * sizeof(float));
         if (e != hipSuccess) {
