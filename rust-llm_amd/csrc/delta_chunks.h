@@ -108,18 +108,27 @@ __device__ inline void split8(const vec<T, 8> &x, bf16x8 (&part)[NP]) {
         }
 }
 
-// Four consecutive f32 values into the rows of their parts, `apart` values from part to part.
+// Four consecutive f32 values into the rows of their parts, `apart` values from part to part. All parts but the last are
+// cut off, not rounded (a bit mask instead of a conversion each way): three hold 24 bits either way, two 16.
 template <int NP>
 __device__ inline void split_store(bhalf_t *to, uint32_t apart, f32x4 x) {
 #pragma unroll
     for (int p = 0; p < NP; p++) {
-        bf16x4 h;
+        if (p + 1 < NP) {
+            uint32_t u[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            h[i] = (bhalf_t)x[i];
-            x[i] -= (float)h[i];
+            for (int i = 0; i < 4; i++) {
+                u[i] = __float_as_uint(x[i]);
+                x[i] -= __uint_as_float(u[i] & 0xFFFF0000u);
+            }
+            *(uint2 *)(to + p * apart) = make_uint2(__builtin_amdgcn_perm(u[1], u[0], 0x07060302u),
+                                                    __builtin_amdgcn_perm(u[3], u[2], 0x07060302u));
+        } else {
+            bf16x4 h;
+#pragma unroll
+            for (int i = 0; i < 4; i++) h[i] = (bhalf_t)x[i];
+            *(bf16x4 *)(to + p * apart) = h;
         }
-        *(bf16x4 *)(to + p * apart) = h;
     }
 }
 
@@ -362,7 +371,7 @@ __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_de
 // What one chunk's step reads.
 template <typename T, int DK>
 struct DeltaChunk {
-    vec<T, 8> k[DK / 32], q[DK / 32], kt[DK / 64][2];
+    vec<T, 8> k[DK / 32], kt[DK / 64][2]; // k: Q for the output's waves
     bf16x8 t[2][3];
     vec<p_type<T>, 8> p[2];
     f32x4 of_k, of_q, of_u;
@@ -370,16 +379,20 @@ struct DeltaChunk {
     uint32_t v[4]; // a value a register
 };
 
-// A workgroup has 16 columns of one head's state, wave w the rows DK/4 w on, and
-// of a chunk's tokens the 16 w on. State, right-hand sides and corrected values
-// pass between the waves through LDS as operands in parts (three barriers a chunk);
-// everything else comes from memory, loaded while the chunk before is computed.
-// Bound by the chain of a chunk: the products of a wave, and the three exchanges.
+// A workgroup has 16 columns of one head's state. Four waves carry the state, wave
+// w the rows DK/4 w on, and of a chunk's tokens the 16 w on: K S, the corrected
+// values and the new state, which pass between them through LDS as operands in
+// parts (three barriers a chunk). Four more waves follow with the output, Q S and
+// P U of the chunk before, in the gaps. Everything else comes from memory, loaded
+// while the chunk before is computed. Bound by the first four's chain: LDS, the
+// products (36 of 16 cycles) and the barriers.
+constexpr uint32_t DELTA_CHUNK_THREADS = 512;
 template <typename T, int DK>
-__global__ void __launch_bounds__(256, DK * sizeof(T) <= 256 ? 2 : 1) k_delta_chunks(DeltaArgs a, DeltaWork w) {
+__global__ void __launch_bounds__(DELTA_CHUNK_THREADS) k_delta_chunks(DeltaArgs a, DeltaWork w) {
     constexpr int NP = parts_of<T>(), NO = out_parts<T>(), STEPS = DK / 32, TILES = DK / 64, SS = DK + 8, TS = 72;
     __shared__ __attribute__((aligned(16))) bhalf_t state[3][16 * SS], right[3][16 * TS], values[NO][16 * TS], update[3][16 * TS];
-    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const uint32_t tid = threadIdx.x, lane = tid % 64, all = __builtin_amdgcn_readfirstlane(tid / 64), wave = all % 4;
+    const bool follows = all >= 4; // with the output
     const uint32_t col = lane % 16, quad = lane / 16;
     // The column groups of one head are eight workgroups apart: on one XCD, whose L2 then has what they share.
     const uint32_t slices = a.value_dim / 16, job = blockIdx.x / (8 * slices) * 8 + blockIdx.x % 8;
@@ -392,16 +405,6 @@ __global__ void __launch_bounds__(256, DK * sizeof(T) <= 256 ? 2 : 1) k_delta_ch
     const uint64_t size = (uint64_t)a.key_dim * a.value_dim;
 
     f32x4 S[TILES]; // rows (wave * TILES + tile) * 16 + 4 quad + i, column dv
-#pragma unroll
-    for (int m = 0; m < TILES; m++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t r = (wave * TILES + m) * 16 + quad * 4 + i;
-            float x = in >= 0 && r < a.key_dim ? NAN : 0.0f;
-            if (in >= 0 && (uint64_t)in < a.state_slots && r < a.key_dim)
-                x = a.states[((uint64_t)in * a.value_heads + head) * size + (uint64_t)r * a.value_dim + dv];
-            S[m][i] = x;
-        }
     auto publish = [&] {
 #pragma unroll
         for (int m = 0; m < TILES; m++) {
@@ -409,115 +412,137 @@ __global__ void __launch_bounds__(256, DK * sizeof(T) <= 256 ? 2 : 1) k_delta_ch
             split_store<3>(state[0] + col * SS + r, 16 * SS, S[m]);
         }
     };
+    if (!follows) {
+#pragma unroll
+        for (int m = 0; m < TILES; m++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t r = (wave * TILES + m) * 16 + quad * 4 + i;
+                float x = in >= 0 && r < a.key_dim ? NAN : 0.0f;
+                if (in >= 0 && (uint64_t)in < a.state_slots && r < a.key_dim)
+                    x = a.states[((uint64_t)in * a.value_heads + head) * size + (uint64_t)r * a.value_dim + dv];
+                S[m][i] = x;
+            }
+        publish();
+    }
 
-    const T *v = (const T *)a.v + head * a.v_head + dv;
     // Addresses are the wave's plus the lane's share.
     auto fragment = [&](const auto *p) {
         using V = std::remove_cv_t<std::remove_reference_t<decltype(*p)>>;
         return ((const vec<V, 8> *)p)[lane];
     };
-    // A chunk's operands, each loaded as soon as the chunk before has used its registers: a whole step ahead. No load is
-    // conditional (past the end the last chunk is loaded again), so that a wait is a count that leaves later loads on
-    // their way.
+    // A chunk's operands, each loaded as soon as the chunk before has used its registers: a whole step ahead, and spread
+    // over the step (a burst of them fills the path to the L1 and holds the wave up). No load is conditional (past the
+    // end the last chunk is loaded again), so that a wait is a count that leaves later loads on their way.
     DeltaChunk<T, DK> x;
-    auto load_keys = [&](uint32_t c) {
-        const uint64_t keys = ((uint64_t)(chunk0 + c) * a.key_heads + key_head) * key_size(DK);
-#pragma unroll
-        for (int st = 0; st < STEPS; st++) {
-            x.k[st] = fragment((const T *)w.kf + keys + (wave * STEPS + st) * FRAGMENT);
-            x.q[st] = fragment((const T *)w.qf + keys + (wave * STEPS + st) * FRAGMENT);
-        }
+    auto key_at = [&](uint32_t c) { return ((uint64_t)(chunk0 + c) * a.key_heads + key_head) * key_size(DK); };
+    auto head_at = [&](uint32_t c) { return (uint64_t)(chunk0 + c) * a.value_heads + head; };
+    auto factors = [&](uint32_t c, uint32_t which) {
+        return ((const f32x4 *)(w.rows + head_at(c) * 4 * CHUNK) + which * (CHUNK / 4) + wave * 4)[quad];
     };
-    auto load_values = [&](uint32_t c) {
+    const T *rows_of = (const T *)(follows ? w.qf : w.kf);
+    auto load_k = [&](uint32_t c, int st) { x.k[st] = fragment(rows_of + key_at(c) + (wave * STEPS + st) * FRAGMENT); };
+    // The lane's four tokens of a chunk: their rows' offsets, past the chunk's end its last row again (T has zeros there).
+    const uint32_t token = wave * 16 + quad * 4;
+    const T *v = (const T *)a.v + (uint64_t)begin * a.v_row + head * a.v_head + dv;
+    uint64_t v_off[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) v_off[i] = (uint64_t)(token + i) * a.v_row;
+    auto load_v = [&](uint32_t c) {
         const uint32_t rows = min(n - c * CHUNK, CHUNK);
-        const T *vc = v + (uint64_t)(begin + c * CHUNK) * a.v_row;
+        const T *vc = v + (uint64_t)(c * CHUNK) * a.v_row;
+        uint64_t off[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) off[i] = v_off[i];
+        if (rows != CHUNK) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) off[i] = (uint64_t)min(token + i, rows - 1) * a.v_row;
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             using U = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
-            x.v[i] = *(const U *)(vc + (uint64_t)min(wave * 16 + quad * 4 + i, rows - 1) * a.v_row);
+            x.v[i] = *(const U *)(vc + off[i]);
         }
-        x.of_k = ((const f32x4 *)(w.rows + ((uint64_t)(chunk0 + c) * a.value_heads + head) * 4 * CHUNK) + wave * 4)[quad];
+        x.of_k = factors(c, 0);
     };
-    auto load_system = [&](uint32_t c) {
-        const uint64_t at = (uint64_t)(chunk0 + c) * a.value_heads + head;
+    // Waves 0 and 1 have only zeros in the second step of T and P, which are not written: they load the first again and
+    // leave it out.
+    const uint32_t second = wave < 2 ? 0 : 1;
+    auto load_t = [&](uint32_t c, int st) {
 #pragma unroll
-        for (int st = 0; st < 2; st++)
-            if (st * 32 <= (int)wave * 16) // else all zeros: not written, not used
-#pragma unroll
-                for (int p = 0; p < 3; p++) x.t[st][p] = fragment(w.tm + (at * 8 + wave * 2 + st) * 3 * FRAGMENT + p * FRAGMENT);
-        x.of_u = ((const f32x4 *)(w.rows + at * 4 * CHUNK) + CHUNK / 2 + wave * 4)[quad];
+        for (int p = 0; p < 3; p++)
+            x.t[st][p] = fragment(w.tm + (head_at(c) * 8 + wave * 2 + (st ? second : 0)) * 3 * FRAGMENT + p * FRAGMENT);
     };
-    auto load_rest = [&](uint32_t c) {
-        const uint64_t keys = ((uint64_t)(chunk0 + c) * a.key_heads + key_head) * key_size(DK);
-        const uint64_t at = (uint64_t)(chunk0 + c) * a.value_heads + head;
-        x.keep = w.rows[at * 4 * CHUNK + 3 * CHUNK];
-#pragma unroll
-        for (int m = 0; m < TILES; m++)
-#pragma unroll
-            for (int st = 0; st < 2; st++) x.kt[m][st] = fragment((const T *)w.kt + keys + ((wave * TILES + m) * 2 + st) * FRAGMENT);
-        x.of_q = ((const f32x4 *)(w.rows + at * 4 * CHUNK) + CHUNK / 4 + wave * 4)[quad];
-#pragma unroll
-        for (int st = 0; st < 2; st++)
-            if (st * 32 <= (int)wave * 16) x.p[st] = fragment((const p_type<T> *)w.pm + at * SQUARE + (wave * 2 + st) * FRAGMENT);
+    auto load_p = [&](uint32_t c, int st) {
+        x.p[st] = fragment((const p_type<T> *)w.pm + head_at(c) * SQUARE + (wave * 2 + (st ? second : 0)) * FRAGMENT);
+    };
+    auto load_kt = [&](uint32_t c, int m, int st) {
+        x.kt[m][st] = fragment((const T *)w.kt + key_at(c) + ((wave * TILES + m) * 2 + st) * FRAGMENT);
+    };
+    auto load_keep = [&](uint32_t c) { x.keep = w.rows[head_at(c) * 4 * CHUNK + 3 * CHUNK]; };
+    const uint32_t mine = col * TS + token;
+    // What waits for a later load stays behind the barrier it is written behind.
+    auto barrier = [] {
+        __builtin_amdgcn_sched_barrier(0);
+        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
     };
 
-    auto step = [&](uint32_t c, uint32_t next) {
-        const uint32_t rows = min(n - c * CHUNK, CHUNK);
-        const bool whole = rows == CHUNK;
-        // K S and Q S for the wave's tokens.
-        f32x4 ks[3], qs[3];
+    // (K or Q) S for the wave's 16 tokens, from the first N parts of the state.
+    auto times_state = [&](auto parts, uint32_t next, f32x4(&acc)[3]) {
+        constexpr int N = decltype(parts)::value;
+        bf16x8 b[STEPS][N];
 #pragma unroll
-        for (int i = 0; i < 3; i++) ks[i] = qs[i] = f32x4{0, 0, 0, 0};
+        for (int st = 0; st < STEPS; st++)
+#pragma unroll
+            for (int p = 0; p < N; p++) b[st][p] = *(const bf16x8 *)(state[p] + col * SS + st * 32 + quad * 8);
+#pragma unroll
+        for (int i = 0; i < 3; i++) acc[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int st = 0; st < STEPS; st++) {
-            bf16x8 b[3], kp[NP], qp[NP];
-#pragma unroll
-            for (int p = 0; p < 3; p++) b[p] = *(const bf16x8 *)(state[p] + col * SS + st * 32 + quad * 8);
+            bf16x8 kp[NP];
             split8(x.k[st], kp);
-            split8(x.q[st], qp);
-            mma_parts(kp, b, ks);
-            if constexpr (NO == 3) mma_parts(qp, b, qs);
-            else {
-                bf16x8(&two)[2] = *(bf16x8(*)[2])b;
-                mma_parts(qp, two, qs);
-            }
+            mma_parts(kp, b[st], acc);
+            load_k(next, st);
         }
-        f32x4 r;
+    };
+    auto right_side = [&](uint32_t next) { // R = V - K S
+        f32x4 ks[3], r;
+        times_state(std::integral_constant<int, 3>{}, next, ks);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             using U = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
-            r[i] = (float)__builtin_bit_cast(T, (U)x.v[i]);
-            if (!whole && wave * 16 + quad * 4 + i >= rows) r[i] = 0.0f;
-            r[i] -= x.of_k[i] * (ks[0][i] + (ks[1][i] + ks[2][i]));
+            r[i] = (float)__builtin_bit_cast(T, (U)x.v[i]) - x.of_k[i] * (ks[0][i] + (ks[1][i] + ks[2][i]));
         }
-        const uint32_t mine = col * TS + wave * 16 + quad * 4;
         split_store<3>(right[0] + mine, 16 * TS, r);
-        load_keys(next);
-        load_values(next);
-        __syncthreads();
-        // U = T R.
+        load_v(next);
+    };
+    auto correct = [&](uint32_t next) { // U = T R
         f32x4 u[3];
         u[0] = u[1] = u[2] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int st = 0; st < 2; st++) {
-            if (st * 32 > (int)wave * 16) continue;
-            bf16x8 b[3];
+            if (st <= (int)second) {
+                bf16x8 b[3];
 #pragma unroll
-            for (int p = 0; p < 3; p++) b[p] = *(const bf16x8 *)(right[p] + col * TS + st * 32 + quad * 8);
-            mma_parts(x.t[st], b, u);
+                for (int p = 0; p < 3; p++) b[p] = *(const bf16x8 *)(right[p] + col * TS + st * 32 + quad * 8);
+                mma_parts(x.t[st], b, u);
+            }
+            load_t(next, st);
         }
         u[0] += u[1] + u[2];
         split_store<3>(update[0] + mine, 16 * TS, u[0] * x.of_u);
         split_store<NO>(values[0] + mine, 16 * TS, u[0]);
-        load_system(next);
-        __syncthreads();
-        // The state, and out = Q S + P U.
+        x.of_u = factors(next, 2);
+    };
+    auto renew = [&](uint32_t next) { // the state
         f32x4 add[TILES][3];
 #pragma unroll
         for (int m = 0; m < TILES; m++) {
             add[m][0] = S[m] * x.keep;
             add[m][1] = add[m][2] = f32x4{0, 0, 0, 0};
         }
+        load_keep(next);
 #pragma unroll
         for (int st = 0; st < 2; st++) {
             bf16x8 b[3];
@@ -528,45 +553,87 @@ __global__ void __launch_bounds__(256, DK * sizeof(T) <= 256 ? 2 : 1) k_delta_ch
                 bf16x8 kp[NP];
                 split8(x.kt[m][st], kp);
                 mma_parts(kp, b, add[m]);
+                load_kt(next, m, st);
             }
         }
 #pragma unroll
         for (int m = 0; m < TILES; m++) S[m] = add[m][0] + (add[m][1] + add[m][2]);
         publish();
+    };
+    f32x4 qs[3];
+    uint64_t out_off[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) out_off[i] = (uint64_t)(token + i) * a.out_row;
+    auto output = [&](uint32_t c, uint32_t next) { // out = Q S + P U of a chunk whose Q S stands in qs
         f32x4 o[3];
         o[0] = (qs[0] + (qs[1] + qs[2])) * x.of_q, o[1] = o[2] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int st = 0; st < 2; st++) {
-            if (st * 32 > (int)wave * 16) continue;
-            constexpr int PP = std::is_same_v<T, bhalf_t> ? 1 : 3;
-            bf16x8 b[NO], p[PP];
+            if (st <= (int)second) {
+                constexpr int PP = std::is_same_v<T, bhalf_t> ? 1 : 3;
+                bf16x8 b[NO], p[PP];
 #pragma unroll
-            for (int i = 0; i < NO; i++) b[i] = *(const bf16x8 *)(values[i] + col * TS + st * 32 + quad * 8);
-            split8(x.p[st], p);
-            mma_parts(p, b, o);
+                for (int i = 0; i < NO; i++) b[i] = *(const bf16x8 *)(values[i] + col * TS + st * 32 + quad * 8);
+                split8(x.p[st], p);
+                mma_parts(p, b, o);
+            }
+            load_p(next, st);
         }
-        load_rest(next);
+        x.of_q = factors(next, 1);
+        const uint32_t rows = min(n - c * CHUNK, CHUNK);
         T *out = (T *)a.out + (uint64_t)(begin + c * CHUNK) * a.out_row + head * a.out_head + dv;
-        auto write = [&](int i) { out[(uint64_t)(wave * 16 + quad * 4 + i) * a.out_row] = (T)(o[0][i] + (o[1][i] + o[2][i])); };
-        if (whole) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) write(i);
-        } else
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (wave * 16 + quad * 4 + i < rows) write(i);
-        __syncthreads();
+        for (int i = 0; i < 4; i++)
+            if (token + i < rows) out[out_off[i]] = (T)(o[0][i] + (o[1][i] + o[2][i]));
     };
 
-    publish();
-    __syncthreads();
-    if (chunks > 0) {
-        load_keys(0);
-        load_values(0);
-        load_system(0);
-        load_rest(0);
+    // Each kind of wave has a loop of its own, of the same three barriers a chunk (a barrier counts the workgroup's waves,
+    // whichever instruction they wait at): in a common one a wait for one kind's loads would be held to the other's too.
+    // First loads go in the order of the steps' own: a wait in the loop has to hold for the first step too.
+    if (follows) {
+        if (chunks > 0) {
+            load_p(0, 0), load_p(0, 1);
+            x.of_q = factors(0, 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int st = 0; st < STEPS; st++) load_k(0, st);
+        }
+        barrier();
+        for (uint32_t c = 0; c < chunks; c++) {
+            if (c) output(c - 1, c); // its U stands until the next barrier
+            barrier();
+            times_state(std::integral_constant<int, NO>{}, min(c + 1, chunks - 1), qs); // before this chunk, until the next
+            barrier();
+            barrier();
+        }
+        if (chunks > 0) output(chunks - 1, chunks - 1);
+        return;
     }
-    for (uint32_t c = 0; c < chunks; c++) step(c, min(c + 1, chunks - 1));
+    if (chunks > 0) {
+#pragma unroll
+        for (int st = 0; st < STEPS; st++) load_k(0, st);
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(0);
+        __builtin_amdgcn_sched_barrier(0);
+        load_t(0, 0), load_t(0, 1);
+        x.of_u = factors(0, 2);
+        __builtin_amdgcn_sched_barrier(0);
+        load_keep(0);
+#pragma unroll
+        for (int st = 0; st < 2; st++)
+#pragma unroll
+            for (int m = 0; m < TILES; m++) load_kt(0, m, st);
+    }
+    barrier();
+    for (uint32_t c = 0; c < chunks; c++) {
+        const uint32_t next = min(c + 1, chunks - 1);
+        right_side(next);
+        barrier();
+        correct(next);
+        barrier();
+        renew(next);
+        barrier();
+    }
     if (to < 0 || (uint64_t)to >= a.state_slots) return;
     float *dst = a.states + ((uint64_t)to * a.value_heads + head) * size + dv;
 #pragma unroll

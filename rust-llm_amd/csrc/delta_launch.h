@@ -22,7 +22,7 @@ template <typename T, int DK>
 void launch_delta_chunks_dim(const DeltaArgs &a, const DeltaWork &w, hipStream_t s) {
     hipLaunchKernelGGL((k_delta_prepare<T, DK>), dim3((a.rows / CHUNK + a.seqs) * a.value_heads), dim3(256), 0, s, a, w);
     const uint32_t jobs = (a.seqs * a.value_heads + 7) / 8 * 8;
-    hipLaunchKernelGGL((k_delta_chunks<T, DK>), dim3(jobs * (a.value_dim / 16)), dim3(256), 0, s, a, w);
+    hipLaunchKernelGGL((k_delta_chunks<T, DK>), dim3(jobs * (a.value_dim / 16)), dim3(DELTA_CHUNK_THREADS), 0, s, a, w);
 }
 
 template <typename T>
