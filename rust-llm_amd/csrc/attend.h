@@ -71,16 +71,6 @@ __device__ inline f32x4 mfma(vec<bhalf_t, 8> a, vec<bhalf_t, 8> b, f32x4 c) {
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Over the four lanes 16 apart.
-__device__ inline float rows_max(float x) {
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
-}
-__device__ inline float rows_sum(float x) {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
-}
-
 // The sequence's rows, and what a row sees: [begin, end).
 struct AttendSpan {
     int32_t len, n, window;

@@ -28,18 +28,17 @@ __device__ inline uint32_t first_row(const DeltaArgs &a, uint32_t s) {
 
 // Sum over the 16 lanes that hold one column quad (lanes 4 apart).
 __device__ inline float quad_sum(float x) {
-#pragma unroll
-    for (int d = 4; d < 64; d *= 2) x += __shfl_xor(x, d);
-    return x;
+    x += rotate16<8>(x);
+    return rows_sum(x + rotate16<4>(x));
 }
 
 // A wave holds 16 columns of one head's state in registers: a column does not
 // depend on the others, so a state splits over as many waves as it has column
 // groups and no wave waits for another. Lane l has the columns 4 (l % 4) .. + 4 of
 // the rows R (l / 4) .. + R; the two products with the state are summed over the
-// 16 lanes of a column. A step's inputs are loaded while the one before is
-// computed. For single tokens bound by HBM (the state is read and written once);
-// for several by the chain of a step.
+// 16 lanes of a column, in registers. A step's inputs are loaded, and made ready,
+// while the one before is computed. For single tokens bound by HBM (the state is
+// read and written once); for several by the chain of a step.
 template <typename T, int R>
 __global__ void __launch_bounds__(64 * DELTA_WAVES) k_delta_steps(DeltaArgs a) {
     const uint32_t lane = threadIdx.x % 64, col0 = (blockIdx.y * DELTA_WAVES + threadIdx.x / 64) * DELTA_COLS;
@@ -50,58 +49,52 @@ __global__ void __launch_bounds__(64 * DELTA_WAVES) k_delta_steps(DeltaArgs a) {
     const uint32_t begin = first_row(a, s), end = first_row(a, s + 1);
     const int32_t in = a.slots_in[s], to = a.slots_out[s];
     const uint64_t size = (uint64_t)a.key_dim * a.value_dim;
-    vec<float, 4> S[R];
-    const float fill = in >= 0 ? NAN : 0.0f;
-#pragma unroll
-    for (int j = 0; j < R; j++) {
-        S[j] = fill;
-        if (row0 + j >= a.key_dim) S[j] = 0.0f;
-        else if (in >= 0 && (uint64_t)in < a.state_slots)
-            S[j] = *(const vec<float, 4> *)(a.states + ((uint64_t)in * a.value_heads + head) * size +
-                                            (uint64_t)(row0 + j) * a.value_dim + col);
-    }
+    const bool here = row0 + R <= a.key_dim; // else none of the lane's rows: key_dim is a multiple of 16, so of R
     float k[R], q[R], v[4], g = 0.0f, beta = 0.0f;
     auto fetch = [&](uint32_t t) {
-        const T *kp = (const T *)a.k + t * a.k_row + key_head * a.k_head;
-        const T *qp = (const T *)a.q + t * a.q_row + key_head * a.q_head;
 #pragma unroll
         for (int j = 0; j < R; j++) k[j] = q[j] = 0.0f;
-        if (row0 + R <= a.key_dim) {
-            load_f32(kp + row0, a.wide, k);
-            load_f32(qp + row0, a.wide, q);
-        } // else none of them: key_dim is a multiple of 16, so of R
+        if (here) {
+            load_f32((const T *)a.k + t * a.k_row + key_head * a.k_head + row0, a.wide, k);
+            load_f32((const T *)a.q + t * a.q_row + key_head * a.q_head + row0, a.wide, q);
+        }
         load_f32((const T *)a.v + t * a.v_row + head * a.v_head + col, a.wide, v);
         g = a.g[t * a.g_row + head];
         beta = a.beta[t * a.beta_row + head];
     };
     if (begin < end) fetch(begin);
+    vec<float, 4> S[R];
+    const float fill = in >= 0 && here ? NAN : 0.0f;
+#pragma unroll
+    for (int j = 0; j < R; j++) S[j] = fill;
+    if (in >= 0 && (uint64_t)in < a.state_slots && here) {
+        const float *src = a.states + ((uint64_t)in * a.value_heads + head) * size + (uint64_t)row0 * a.value_dim + col;
+#pragma unroll
+        for (int j = 0; j < R; j++) S[j] = *(const vec<float, 4> *)(src + (uint64_t)j * a.value_dim);
+    }
     for (uint32_t t = begin; t < end; t++) {
-        float kc[R], qc[R], vc[4];
-        float kk = 0.0f, qq = 0.0f;
-#pragma unroll
-        for (int j = 0; j < R; j++) {
-            kc[j] = k[j], qc[j] = q[j];
-            kk += k[j] * k[j], qq += q[j] * q[j];
-        }
-#pragma unroll
-        for (int c = 0; c < 4; c++) vc[c] = v[c];
+        float kc[R], qc[R], vc[4], kn = 1.0f, qn = a.scale;
         const float keep = expf(g), b = beta;
-        if (t + 1 < end) fetch(t + 1);
-        float kn = 1.0f, qn = a.scale;
         if (a.eps >= 0.0f) {
+            float kk = 0.0f, qq = 0.0f;
+#pragma unroll
+            for (int j = 0; j < R; j++) kk = fmaf(k[j], k[j], kk), qq = fmaf(q[j], q[j], qq);
             kn = 1.0f / sqrtf(quad_sum(kk) + a.eps);
             qn = a.scale / sqrtf(quad_sum(qq) + a.eps);
         }
+#pragma unroll
+        for (int j = 0; j < R; j++) kc[j] = k[j] * kn, qc[j] = q[j] * qn;
+#pragma unroll
+        for (int c = 0; c < 4; c++) vc[c] = v[c];
+        if (t + 1 < end) fetch(t + 1);
         float p[4] = {}, o[4] = {};
 #pragma unroll
-        for (int j = 0; j < R; j++) {
-            kc[j] *= kn;
+        for (int j = 0; j < R; j++)
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 S[j][c] *= keep;
                 p[c] = fmaf(S[j][c], kc[j], p[c]);
             }
-        }
 #pragma unroll
         for (int c = 0; c < 4; c++) p[c] = b * (vc[c] - quad_sum(p[c]));
 #pragma unroll
@@ -112,14 +105,13 @@ __global__ void __launch_bounds__(64 * DELTA_WAVES) k_delta_steps(DeltaArgs a) {
                 o[c] = fmaf(S[j][c], qc[j], o[c]);
             }
 #pragma unroll
-        for (int c = 0; c < 4; c++) o[c] = qn * quad_sum(o[c]);
+        for (int c = 0; c < 4; c++) o[c] = quad_sum(o[c]);
         if (lane < 4) store_f32((T *)a.out + t * a.out_row + head * a.out_head + col, a.wide, o);
     }
-    if (to < 0 || (uint64_t)to >= a.state_slots) return;
-    float *dst = a.states + ((uint64_t)to * a.value_heads + head) * size + col;
+    if (to < 0 || (uint64_t)to >= a.state_slots || !here) return;
+    float *dst = a.states + ((uint64_t)to * a.value_heads + head) * size + (uint64_t)row0 * a.value_dim + col;
 #pragma unroll
-    for (int j = 0; j < R; j++)
-        if (row0 + j < a.key_dim) *(vec<float, 4> *)(dst + (uint64_t)(row0 + j) * a.value_dim) = S[j];
+    for (int j = 0; j < R; j++) *(vec<float, 4> *)(dst + (uint64_t)j * a.value_dim) = S[j];
 }
 
 }  // namespace rl

@@ -85,6 +85,34 @@ __device__ inline uint2 encode8(const float (&x)[8]) {
     return make_uint2(u[0], u[1]);
 }
 
+// The other half of a swap: lanes 16 apart (of 32) and 32 apart, without LDS.
+__device__ inline float2 swap16(float x) { // each lane's own row of 16 and its neighbour's, in some order
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float2 swap32(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// Over the four lanes 16 apart.
+__device__ inline float rows_max(float x) {
+    float2 y = swap16(x);
+    y = swap32(fmaxf(y.x, y.y));
+    return fmaxf(y.x, y.y);
+}
+__device__ inline float rows_sum(float x) {
+    float2 y = swap16(x);
+    y = swap32(y.x + y.y);
+    return y.x + y.y;
+}
+
+// Of the lane N further on in its row of 16, cyclically.
+template <int N>
+__device__ inline float rotate16(float x) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x120 + N, 0xf, 0xf, false));
+}
+
 // Sum and maximum over the aligned group of N lanes that holds the caller, N a power of two.
 template <int N>
 __device__ inline float group_sum(float x) {

@@ -169,14 +169,18 @@ constexpr uint32_t ATTEND_LONG = 1536, CUS = 256;
 
 uint32_t attend_tiles(uint64_t tokens) { return (uint32_t)((tokens + ATTEND_TILE - 1) / ATTEND_TILE) + 1; }
 
-// Parts that lengths up to `tiles` need at the least.
-uint32_t attend_least_parts(uint32_t tiles) {
+// Parts that lengths up to `tiles` need at the least; one sequence has no others to wait for.
+uint32_t attend_least_parts(uint32_t tiles, uint32_t seqs) {
+    if (seqs == 1) return 1;
     const uint32_t n = (tiles + ATTEND_LONG / ATTEND_TILE - 1) / (ATTEND_LONG / ATTEND_TILE);
     return std::min(n, ATTEND_MAX_PARTS);
 }
 
-// Rows of a sequence from which chunks are faster than one token after the other.
-constexpr uint32_t DELTA_CHUNKED = 32;
+// Rows of a sequence from which chunks are faster than one token after the other (us, steps / chunks; 32 heads of 128 x
+// 128). While every workgroup of the chunks has a CU to itself they cost the same for any rows up to 64: one bf16
+// sequence of 9 rows 13.7 / 16, of 16 21.6 / 16; f32, more products, 16 rows 18.2 / 22.7, 24 rows 25.7 / 22.7. Beyond
+// that they wait for each other: 16 sequences of 16 rows 54 / 75, of 24 75 / 75.
+constexpr uint32_t DELTA_CHUNKED = 13, DELTA_CHUNKED_WIDE = 20, DELTA_CHUNKED_MANY = 24;
 
 int launched(const char *what) {
     const hipError_t e = hipGetLastError();
@@ -431,7 +435,7 @@ int rl_attention_create(int device, uint32_t max_rows, uint32_t q_heads, uint32_
     a->max_rows = max_rows, a->q_heads = q_heads, a->kv_heads = kv_heads, a->dim = dim, a->max_len = max_len;
     // Room for the least parts of every row, and for as many workgroups of 32 rows as the device holds.
     const uint64_t heads = (uint64_t)max_rows * q_heads;
-    a->slots = std::max<uint64_t>(heads * attend_least_parts(attend_tiles(max_len)), CUS * 3 * 32);
+    a->slots = std::max<uint64_t>(heads * attend_least_parts(attend_tiles(max_len), 2), CUS * 3 * 32);
     hipError_t e = hipMalloc(&a->part_out, a->slots * attend_dim(dim) * sizeof(float));
     if (e == hipSuccess) e = hipMalloc(&a->part_sum, a->slots * sizeof(float2));
     if (e == hipSuccess) e = hipMalloc(&a->part_count, heads * sizeof(uint32_t));
@@ -498,7 +502,7 @@ int rl_attention_rows(rl_attention *h, const rl_kv_cache *cache, const rl_heads 
     const uint32_t tiles = attend_tiles(seen);
     const uint64_t room = std::min<uint64_t>(h->slots / ((uint64_t)rows * h->q_heads), ATTEND_MAX_PARTS);
     const uint64_t held = CUS * attend_resident(type_bytes(q->dtype), cache->format, h->dim, two ? 2 : 1);
-    uint64_t parts = std::max<uint64_t>(held / columns, attend_least_parts(tiles));
+    uint64_t parts = std::max<uint64_t>(held / columns, attend_least_parts(tiles, seqs));
     parts = std::max<uint64_t>(std::min(parts, room), 1);
     a.part_tiles = (uint32_t)((tiles + parts - 1) / parts);
     a.part_tiles = (a.part_tiles + ATTEND_WAVES - 1) / ATTEND_WAVES * ATTEND_WAVES;
@@ -598,7 +602,9 @@ int rl_delta_rows(rl_delta *h, const rl_heads *q, const rl_heads *k, const rl_he
     a.wide = wide(q) && wide(k) && wide(v) && wide(out);
     // Chunks where some sequence has the rows for them and the workspace holds all.
     const uint32_t most = most_rows ? std::min(most_rows, rows) : rows;
-    const bool chunked = most >= DELTA_CHUNKED && rows / CHUNK + seqs <= h->chunks;
+    const bool alone = (uint64_t)seqs * h->value_heads * (h->value_dim / 16) <= CUS;
+    const uint32_t least = !alone ? DELTA_CHUNKED_MANY : q->dtype == RL_BF16 ? DELTA_CHUNKED : DELTA_CHUNKED_WIDE;
+    const bool chunked = most >= least && rows / CHUNK + seqs <= h->chunks;
     with_type(q->dtype, [&](auto t) {
         if (chunked) launch_delta_chunks<decltype(t)>(a, h->work, static_cast<hipStream_t>(stream));
         else launch_delta_steps<decltype(t)>(a, static_cast<hipStream_t>(stream));

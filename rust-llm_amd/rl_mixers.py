@@ -10,8 +10,10 @@ the library raises rl_sampler.SamplerError.
 import ctypes
 import struct
 
+import torch
+
 import rl_sampler
-from rl_sampler import _check, _u32, _u64, _vp, current_stream
+from rl_sampler import _check, _u32, _u64, _vp
 
 TYPES = {"f32": 0, "f16": 1, "bf16": 2, "i8": 3, "f8": 4}
 LAYOUTS = {"half": 0, "interleaved": 1}
@@ -58,14 +60,17 @@ def lib():
     return _bound
 
 
-_codes = {}
+_codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _stream(t, stream):
+    """The stream given, or the current one of the tensor's device (without the
+    Stream object of torch.cuda.current_stream, which costs 3 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device()) if stream is None else stream
 
 
 def _heads(t):
     """A tensor [rows][heads][dim] as a packed rl_heads."""
-    if not _codes:
-        import torch
-        _codes.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
     _, heads, dim = t.shape
     rows, per, one = t.stride()
     if one != 1 or t.dtype not in _codes:
@@ -118,7 +123,6 @@ class DeviceRotary(_Handle):
     def apply(self, x, positions, out=None, second=None, second_out=None, inverse=False, stream=None):
         """Turns x [rows][heads][dim] by positions [rows] (int64) into `out` (x
         itself if None), and `second` likewise in the same launch."""
-        import torch
         rows = x.shape[0]
         out = x if out is None else out
         ins, outs, tensors = _heads(x), _heads(out), 1
@@ -130,7 +134,7 @@ class DeviceRotary(_Handle):
                 raise ValueError("the second tensor has other rows, or its output another shape")
             ins, outs, tensors = ins + _heads(second), outs + _heads(second_out), 2
         _check(lib().rl_rotary_rows(self.h, _index(positions, torch.int64, rows), rows, ins, outs, tensors,
-                                    int(inverse), current_stream() if stream is None else stream))
+                                    int(inverse), _stream(x, stream)))
 
 
 class DeviceCache(_Handle):
@@ -151,23 +155,20 @@ class DeviceCache(_Handle):
     def write(self, keys, values, slots, rotary=None, positions=None, stream=None):
         """Rows keys[i], values[i] to slots[i] (int64; negative: left out), the keys
         turned by positions[i] first if a DeviceRotary is given."""
-        import torch
         rows = keys.shape[0]
         if values.shape[0] != rows:
             raise ValueError("keys and values have one row a slot")
         at = None if rotary is None else _index(positions, torch.int64, rows)
         _check(lib().rl_kv_cache_write(self.h, _heads(keys), _heads(values), _index(slots, torch.int64, rows), rows,
-                                       None if rotary is None else rotary.h, at,
-                                       current_stream() if stream is None else stream))
+                                       None if rotary is None else rotary.h, at, _stream(keys, stream)))
 
     def read(self, slots, keys, values, stream=None):
         """Into keys[i], values[i] what slots[i] holds (NaN outside the cache)."""
-        import torch
         rows = keys.shape[0]
         if values.shape[0] != rows:
             raise ValueError("keys and values have one row a slot")
         _check(lib().rl_kv_cache_read(self.h, _index(slots, torch.int64, rows), rows, _heads(keys), _heads(values),
-                                      current_stream() if stream is None else stream))
+                                      _stream(keys, stream)))
 
 
 class DeviceAttention(_Handle):
@@ -186,7 +187,6 @@ class DeviceAttention(_Handle):
         """q, out [rows][q_heads][dim]; lens int32 [seqs]; pages int32
         [seqs][width]; starts int32 [seqs + 1] (None: one row a sequence); lse f32
         [rows][q_heads] if wanted; scale: dim^-1/2 if None."""
-        import torch
         rows, seqs, width = q.shape[0], pages.shape[0], pages.shape[1]
         if out.shape != q.shape:
             raise ValueError("out has another shape than q")
@@ -195,7 +195,7 @@ class DeviceAttention(_Handle):
             None if lse is None else _index(lse, torch.float32, rows * self.q_heads), rows,
             None if starts is None else _index(starts, torch.int32, seqs + 1), _index(lens, torch.int32, seqs), seqs,
             _index(pages, torch.int32, seqs * width), width, self.scale if scale is None else scale, window, most_rows,
-            max_len, current_stream() if stream is None else stream))
+            max_len, _stream(q, stream)))
 
 
 class DeviceDelta(_Handle):
@@ -217,7 +217,6 @@ class DeviceDelta(_Handle):
         g, beta f32 [rows][value_heads]; states f32 [slots][value_heads][key_dim]
         [value_dim], contiguous; slots_in, slots_out int32 [seqs]; starts int32
         [seqs + 1] (None: one row a sequence); scale: key_dim^-1/2 if None."""
-        import torch
         rows, seqs = q.shape[0], slots_in.shape[0]
         if k.shape[0] != rows or v.shape[0] != rows or out.shape[0] != rows:
             raise ValueError("q, k, v and out have one row a token")
@@ -231,4 +230,4 @@ class DeviceDelta(_Handle):
             beta.stride(0), states.data_ptr(), states.shape[0], _index(slots_in, torch.int32, seqs),
             _index(slots_out, torch.int32, seqs), None if starts is None else _index(starts, torch.int32, seqs + 1),
             rows, seqs, self.scale if scale is None else scale, eps if normalise else -1.0, most_rows,
-            current_stream() if stream is None else stream))
+            _stream(q, stream)))
