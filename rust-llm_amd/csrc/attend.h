@@ -84,16 +84,13 @@ __device__ inline uint2 split_by(uint32_t t, uint32_t d, uint32_t inv) { // (t /
     return make_uint2(q, r);
 }
 
-// The eight bytes 16-bit pairs (lo, hi) of two 8-bit codes: the low or high half of u.
+// Two 8-bit codes, the low or high half of u, as two 16-bit values. Keys: int8 codes lie in the cache with their sign
+// bit flipped, and 0x6400 | b is 1024 + b in f16, so each reads as the code and 1152, exactly.
+constexpr float KEY_BIAS = 1152.0f;
 template <int FMT, bool HIGH>
 __device__ inline uint32_t pair_f16(uint32_t u) {
-    if constexpr (FMT == RL_F8) {
-        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(u, 1.0f, HIGH));
-    } else { // 0x6400 | b is 1024 + b in f16: the code with its sign bit flipped, and 1152 taken off, exactly
-        const uint32_t w = __builtin_amdgcn_perm(0x64646464u, u ^ 0x80808080u, HIGH ? 0x04030402u : 0x04010400u);
-        const vec<half_t, 2> bias = {(half_t)1152.0f, (half_t)1152.0f};
-        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(vec<half_t, 2>, w) - bias);
-    }
+    if constexpr (FMT == RL_F8) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(u, 1.0f, HIGH));
+    else return __builtin_amdgcn_perm(0x64646464u, u, HIGH ? 0x04030402u : 0x04010400u);
 }
 template <int FMT, bool HIGH>
 __device__ inline uint32_t pair_bf16(uint32_t u) {
@@ -138,11 +135,14 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     constexpr int VW = VD * SIZE / 4;         // dwords of a value that a lane holds
     constexpr int STEPS = HD / 32;            // products a score tile
     constexpr float LIFT = FMT == RL_F16 ? ATTEND_LIFT : 0.0f; // weights up to 2^8: their second f16 parts stay normal
+    // int8 keys with their bias: q (c + 1152) - 1152 sum q, where f32's 24 bits leave 16-bit queries' scores exact enough
+    // (4e-6 off at most); f32 queries take the bias off every key.
+    constexpr bool BIASED = FMT == RL_I8 && !F32Q;
     constexpr bool Q_REGS = RT * QP * STEPS <= 4;
     constexpr int QS = HD + 8;
-    constexpr size_t Q_BYTES = (size_t)QP * ROWS * QS * 2, O_BYTES = (size_t)ROWS * (HD + 4) * 4;
+    constexpr size_t Q_BYTES = (size_t)QP * ROWS * QS * 2, O_BYTES = (size_t)ATTEND_WAVES * 16 * (HD + 4) * 4;
     __shared__ __attribute__((aligned(16))) uint8_t lds[Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES];
-    __shared__ float mults[ROWS], maxima[ATTEND_WAVES][ROWS], sums[ATTEND_WAVES][ROWS];
+    __shared__ float mults[ROWS], biases[ROWS], maxima[ATTEND_WAVES][ROWS], sums[ATTEND_WAVES][ROWS];
 
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     // The row blocks of one sequence, head and part are eight workgroups apart: on one XCD, so that its L2 has the keys
@@ -151,8 +151,11 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     const uint32_t columns = a.seqs * a.cache.heads, part = job / columns, sh = job - part * columns;
     if (part >= a.parts) return;
     const uint32_t s = sh / a.cache.heads, head = sh - s * a.cache.heads, G = a.group;
-    const int32_t first = a.starts ? a.starts[s] : (int32_t)s;
-    AttendSpan span{a.lens[s], a.starts ? a.starts[s + 1] - first : 1, (int32_t)a.window};
+    // Not written while the kernel runs: read through the scalar cache where the index is the wave's.
+    typedef const __attribute__((address_space(4))) int32_t constant_i32;
+    const constant_i32 *starts = (constant_i32 *)(uintptr_t)a.starts, *lens = (constant_i32 *)(uintptr_t)a.lens;
+    const int32_t first = starts ? starts[s] : (int32_t)s;
+    AttendSpan span{lens[s], starts ? starts[s + 1] - first : 1, (int32_t)a.window};
     if (span.n <= 0 || first < 0 || (uint32_t)first + span.n > a.rows) return; // no rows, or `starts` is not what it should be
     const uint32_t expanded = (uint32_t)span.n * G;
     const int32_t longest = span.end(span.n - 1);
@@ -210,8 +213,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
 
     const uint32_t dim_bytes = a.cache.dim * SIZE;
     const uint8_t *keys = (const uint8_t *)a.cache.keys, *values = (const uint8_t *)a.cache.values;
-    // Not written while the kernel runs: read through the scalar cache where the index is the wave's.
-    const auto *table = (const __attribute__((address_space(4))) int32_t *)(uintptr_t)(a.pages + (uint64_t)s * a.table_width);
+    const auto *table = (constant_i32 *)(uintptr_t)(a.pages + (uint64_t)s * a.table_width);
     const uint32_t pool = (uint32_t)(a.cache.slots / page);
     bool poison = false; // a page number that is none
 
@@ -366,14 +368,20 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
 #pragma unroll
             for (uint32_t j = 0; j < EPT; j++) x[j] *= down;
         }
+        float sum = 0.0f;
 #pragma unroll
         for (int p = 0; p < QP; p++)
 #pragma unroll
             for (uint32_t j = 0; j < EPT; j++) {
                 const MK y = (MK)x[j];
                 qs[(p * ROWS + q_row) * QS + q_at + j] = y;
+                if (BIASED) sum += (float)y;
                 x[j] -= (float)y;
             }
+        if (BIASED) {
+            sum = group_sum<TPR>(sum);
+            if (tid % TPR == 0) biases[q_row] = KEY_BIAS * sum;
+        }
         if (tid % TPR == 0) mults[q_row] = a.scale * 1.44269504088896341f * unit;
     }
     __syncthreads();
@@ -393,12 +401,13 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
 #pragma unroll
                 for (int st = 0; st < STEPS; st++) qf[rt][p][st] = q_fragment(rt, p, st);
     }
-    float mult[RT];
+    float mult[RT], bias[RT];
     int32_t row_begin[RT], row_end[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         const uint32_t r = rt * 16 + col;
         mult[rt] = mults[r];
+        bias[rt] = BIASED ? biases[r] : 0.0f;
         const int32_t i = r < count ? (r0 + r) / G : 0;
         row_begin[rt] = r < count ? span.begin(i) : begin_min; // rows past the block's see what any of it sees
         row_end[rt] = r < count ? span.end(i) : end_max;
@@ -420,9 +429,12 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
                     const uint32_t x = kr[u][st / 2][st % 2 * 2], y = kr[u][st / 2][st % 2 * 2 + 1];
                     const u32x4 w = {pair_f16<FMT, false>(x), pair_f16<FMT, true>(x), pair_f16<FMT, false>(y), pair_f16<FMT, true>(y)};
                     k[u] = __builtin_bit_cast(vec<MK, 8>, w);
-                } else
+                    if constexpr (FMT == RL_I8 && !BIASED) k[u] -= (MK)KEY_BIAS;
+                } else {
                     k[u] = __builtin_bit_cast(vec<MK, 8>, kr[u][st]);
-                if (a.cache.dim != HD && (EIGHT ? st / 2 * 64 : st * 64) + quad * 16 >= dim_bytes) k[u] = vec<MK, 8>{};
+                    // Queries are zeros past the head's end; 16-bit keys may hold what a zero does not cancel.
+                    if (a.cache.dim != HD && st * 64 + quad * 16 >= dim_bytes) k[u] = vec<MK, 8>{};
+                }
             }
 #pragma unroll
             for (int rt = 0; rt < RT; rt++)
@@ -451,8 +463,9 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
             float x[8], most = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                x[j] = S[rt][j / 4][j % 4] * mult[rt];
-                if constexpr (EIGHT) x[j] *= step[j / 4][j % 4];
+                if constexpr (BIASED) S[rt][j / 4][j % 4] -= bias[rt];
+                if constexpr (EIGHT) x[j] = S[rt][j / 4][j % 4] * (step[j / 4][j % 4] * mult[rt]);
+                else x[j] = S[rt][j / 4][j % 4] * mult[rt];
                 if (edge) {
                     const int32_t t = t0 + j / 4 * 16 + (int)quad * 4 + j % 4;
                     if (t < row_begin[rt] || t >= row_end[rt]) x[j] = -INFINITY;
@@ -468,6 +481,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
                 top[rt] = most;
             }
             const float base = (most == -INFINITY ? 0.0f : most) - LIFT;
+            float rest[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 float p = exp2_fast(x[j] - base);
@@ -476,13 +490,26 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
                     p *= vs[j / 4][j % 4];
                     if (edge && x[j] == -INFINITY) p = 0.0f; // whatever the step of an unseen token is
                 }
-#pragma unroll
-                for (int i = 0; i < PP; i++) {
-                    const MV y = (MV)p;
-                    w[rt][i][j] = y;
-                    p -= (float)y;
-                }
+                rest[j] = p;
             }
+            if constexpr (std::is_same_v<MV, bhalf_t>) { // the first part cut off, not rounded: a mask, and one v_perm for two
+                u32x4 cut;
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const uint32_t u0 = __float_as_uint(rest[j]), u1 = __float_as_uint(rest[j + 1]);
+                    cut[j / 2] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
+                    rest[j] -= __uint_as_float(u0 & 0xFFFF0000u);
+                    rest[j + 1] -= __uint_as_float(u1 & 0xFFFF0000u);
+                }
+                w[rt][0] = __builtin_bit_cast(vec<MV, 8>, cut);
+            } else
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    w[rt][0][j] = (MV)rest[j];
+                    rest[j] -= (float)w[rt][0][j];
+                }
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[rt][1][j] = (MV)rest[j];
         }
         bool stray = false;
         constexpr uint32_t E = std::is_same_v<MV, half_t> ? 0x7C00u : 0x7F80u; // the exponent of what is not finite
@@ -533,63 +560,46 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
         if (more) load_values(next);
     }
 
-    // The four waves' sums.
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         total[rt] = rows_sum(total[rt]);
         if (__any(poison)) total[rt] = NAN;
         if (quad == 0) maxima[wave][rt * 16 + col] = top[rt], sums[wave][rt * 16 + col] = total[rt];
     }
-    __syncthreads();
-    float *ob = (float *)lds; // [ROWS][HD + 4]
-    float share[RT]; // of this wave's sums in the row's
+    // Every wave's 16 rows side by side in LDS, then each thread adds four columns of a row.
+    float *ob = (float *)lds; // [wave][16][HD + 4]
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        const uint32_t r = rt * 16 + col;
-        float most = maxima[0][r];
-        for (uint32_t i = 1; i < ATTEND_WAVES; i++) most = fmaxf(most, maxima[i][r]);
-        share[rt] = top[rt] == -INFINITY ? 0.0f : exp2_fast(top[rt] - most);
-    }
-    // In four rounds each wave adds another quarter of the columns.
-    constexpr int QUARTER = VD / 4;
-#pragma unroll
-    for (uint32_t round = 0; round < 4; round++) {
-#pragma unroll
-        for (uint32_t g = 0; g < 4; g++)
-            if ((wave + round) % 4 == g) {
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        vec<float, QUARTER> x;
-#pragma unroll
-                        for (int m = 0; m < QUARTER; m++) x[m] = O[rt][g * QUARTER + m][i] * share[rt];
-                        auto *p = (vec<float, QUARTER> *)(ob + (rt * 16 + col) * (HD + 4) + (quad * 4 + i) * VD + g * QUARTER);
-                        *p = round ? *p + x : x;
-                    }
-            }
         __syncthreads();
-    }
-    // A row's maximum and sum over the waves; a wave without tokens adds its sum of 0 (or NaN).
-    auto joined = [&](uint32_t r) {
-        float most = maxima[0][r], sum = 0.0f;
-        for (uint32_t i = 1; i < ATTEND_WAVES; i++) most = fmaxf(most, maxima[i][r]);
-        for (uint32_t i = 0; i < ATTEND_WAVES; i++)
-            sum += maxima[i][r] == -INFINITY ? sums[i][r] : sums[i][r] * exp2_fast(maxima[i][r] - most);
-        return make_float2(most, sum);
-    };
-    for (uint32_t i = tid; i < count * (HD / 4); i += ATTEND_THREADS) {
-        const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4, e = r0 + r;
-        const float2 ms = joined(r);
-        const f32x4 x = *(const f32x4 *)(ob + r * (HD + 4) + d);
-        const uint64_t row = first + e / G, qh = head * G + e % G, at = row * a.q_heads + qh;
-        const bool none = span.end(e / G) <= span.begin(e / G);
-        if (parts == 1) attend_write<T>(a, row, qh, d, none, ms, x, LIFT);
-        else {
-            *(f32x4 *)(a.part_out + (at * a.parts + part) * HD + d) = x;
-            if (d == 0) a.part_sum[at * a.parts + part] = ms;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int m = 0; m < VD; m += 4)
+                *(f32x4 *)(ob + (wave * 16 + col) * (HD + 4) + (quad * 4 + i) * VD + m) =
+                    f32x4{O[rt][m][i], O[rt][m + 1][i], O[rt][m + 2][i], O[rt][m + 3][i]};
+        __syncthreads();
+        for (uint32_t i = tid; i < 16 * (HD / 4); i += ATTEND_THREADS) {
+            const uint32_t r = rt * 16 + i / (HD / 4), d = i % (HD / 4) * 4, e = r0 + r;
+            if (r >= count) break;
+            float2 ms = make_float2(maxima[0][r], 0.0f);
+#pragma unroll
+            for (uint32_t v = 1; v < ATTEND_WAVES; v++) ms.x = fmaxf(ms.x, maxima[v][r]);
+            f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t v = 0; v < ATTEND_WAVES; v++) { // a wave without tokens adds zeros (or NaN)
+                const float f = maxima[v][r] == -INFINITY ? 1.0f : exp2_fast(maxima[v][r] - ms.x);
+                ms.y += sums[v][r] * f;
+                x += *(const f32x4 *)(ob + (v * 16 + i / (HD / 4)) * (HD + 4) + d) * f;
+            }
+            const uint64_t row = first + e / G, qh = head * G + e % G, at = row * a.q_heads + qh;
+            const bool none = span.end(e / G) <= span.begin(e / G);
+            if (parts == 1) attend_write<T>(a, row, qh, d, none, ms, x, LIFT);
+            else {
+                *(f32x4 *)(a.part_out + (at * a.parts + part) * HD + d) = x;
+                if (d == 0) a.part_sum[at * a.parts + part] = ms;
+            }
+            if (d == 0 && part == 0) a.part_count[at] = parts | (none ? ATTEND_NONE : 0);
         }
-        if (d == 0 && part == 0) a.part_count[at] = parts | (none ? ATTEND_NONE : 0);
     }
 }
 

@@ -7,7 +7,9 @@ namespace rl {
 
 // Codes are [page][head][token of the page][dim], steps (8-bit formats) f32
 // [page][head][token]: the tokens of one page and head lie together, as the
-// attention reads them.
+// attention reads them. int8 codes of keys have their sign bit flipped, which
+// saves the attention an instruction a dword.
+constexpr uint32_t KEY_SIGNS = 0x80808080u;
 struct CacheArgs {
     void *keys, *values;
     float *key_steps, *value_steps;
@@ -107,7 +109,9 @@ __global__ void __launch_bounds__(CACHE_THREADS) k_cache_write(CacheArgs c, Cach
 #pragma unroll
             for (int j = 0; j < 8; j++) y[j] = step > 0.0f ? fminf(fmaxf(x[j] / step, -TOP), TOP) : 0.0f;
             if (here) {
-                *reinterpret_cast<uint2 *>((uint8_t *)(is_value ? c.values : c.keys) + v * c.dim + at) = encode8<FMT>(y);
+                uint2 u = encode8<FMT>(y);
+                if (FMT == RL_I8 && !is_value) u.x ^= KEY_SIGNS, u.y ^= KEY_SIGNS;
+                *reinterpret_cast<uint2 *>((uint8_t *)(is_value ? c.values : c.keys) + v * c.dim + at) = u;
                 if (lane == 0) (is_value ? c.value_steps : c.key_steps)[v] = step;
             }
         }
@@ -137,7 +141,9 @@ __global__ void __launch_bounds__(CACHE_THREADS) k_cache_read(CacheArgs c, Cache
             using S = std::conditional_t<FMT == RL_F16, half_t, bhalf_t>;
             load_f32((const S *)codes + v * c.dim + at, true, x);
         } else {
-            decode8<FMT>(*reinterpret_cast<const uint2 *>((const uint8_t *)codes + v * c.dim + at), x);
+            uint2 u = *reinterpret_cast<const uint2 *>((const uint8_t *)codes + v * c.dim + at);
+            if (FMT == RL_I8 && !is_value) u.x ^= KEY_SIGNS, u.y ^= KEY_SIGNS;
+            decode8<FMT>(u, x);
             const float step = (is_value ? c.value_steps : c.key_steps)[v];
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] *= step;
