@@ -31,7 +31,6 @@ struct AttendArgs {
     uint32_t group;       // query heads of a key-value head
     uint32_t blocks;      // row blocks a sequence
     uint32_t part_tiles;  // tiles of 32 tokens a part
-    uint32_t page_inv;    // floor(2^32 / page), at most 2^32 - 1
     uint32_t wide;        // whether q and out are aligned for 16-byte accesses
     float *part_out;      // [row * q_heads + head][part][HD]: sums of the weighted values
     float2 *part_sum;     // [row * q_heads + head][part]: maximum and sum
@@ -78,12 +77,6 @@ struct AttendSpan {
     __device__ int32_t begin(int32_t i) const { return window ? max(end(i) - window, 0) : 0; }
 };
 
-__device__ inline uint2 split_by(uint32_t t, uint32_t d, uint32_t inv) { // (t / d, t % d)
-    uint32_t q = __umulhi(t, inv), r = t - q * d; // the quotient, or one less
-    if (r >= d) q++, r -= d;
-    return make_uint2(q, r);
-}
-
 // Two 8-bit codes, the low or high half of u, as two 16-bit values. Keys: int8 codes lie in the cache with their sign
 // bit flipped, and 0x6400 | b is 1024 + b in f16, so each reads as the code and 1152, exactly.
 constexpr float KEY_BIAS = 1152.0f;
@@ -126,10 +119,11 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     // (below), weights times a value's step need bf16's range.
     using MK = std::conditional_t<FMT == RL_BF16, bhalf_t, half_t>;
     using MV = std::conditional_t<FMT == RL_F16, half_t, bhalf_t>;
-    // f32 queries are split into parts that add up to them (24 bits in three bf16 parts, 22 in two of f16); weights into
-    // two parts for every type (16 or 22 bits): one alone, of 8 bits, cost as much as the output's own rounding (0.0025
-    // off f64 against 0.0017 over 64 int8 sequences), and a second product hides behind the loads.
-    constexpr int QP = !F32Q ? 1 : std::is_same_v<MK, bhalf_t> ? 3 : 2, PP = 2;
+    // f32 queries are split into parts that add up to them (24 bits in three bf16 parts, 22 in two of f16), and so are
+    // the weights of f32 outputs. Those of 16-bit outputs are two parts too (16 or 22 bits): one alone, of 8 bits, cost as
+    // much as the output's own rounding (0.0025 off f64 against 0.0017 over 64 int8 sequences), and a second product
+    // hides behind the loads.
+    constexpr int QP = !F32Q ? 1 : std::is_same_v<MK, bhalf_t> ? 3 : 2, PP = F32Q && std::is_same_v<MV, bhalf_t> ? 3 : 2;
     constexpr int ROWS = 16 * RT, VD = HD / 16, SIZE = EIGHT ? 1 : 2;
     constexpr int KC = HD * SIZE / 64;        // 64-byte chunks of a key
     constexpr int VW = VD * SIZE / 4;         // dwords of a value that a lane holds
@@ -162,7 +156,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     const uint32_t page = a.cache.page;
     // What the call's bounds or the page table do not cover is NaN, written once.
     if ((uint32_t)span.n > a.most_rows || span.len > (int64_t)a.max_len ||
-        (longest > 0 && split_by(longest - 1, page, a.page_inv).x >= a.table_width)) {
+        (longest > 0 && split_by(longest - 1, page, a.cache.page_inv).x >= a.table_width)) {
         if (part || block) return;
         const uint32_t dim = a.cache.dim;
         for (uint64_t i = tid; i < (uint64_t)expanded * dim; i += ATTEND_THREADS) {
@@ -239,7 +233,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
 #pragma unroll
         for (int u = 0; u < (P16 ? 2 : 1); u++) {
             const int32_t t = t0 + (P16 ? 16 * u : (int)(lane % 32));
-            if (in_sight(t)) p.id[u] = (uint32_t)table[split_by(t, page, a.page_inv).x];
+            if (in_sight(t)) p.id[u] = (uint32_t)table[split_by(t, page, a.cache.page_inv).x];
         }
         return p;
     };
@@ -250,7 +244,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
             const int32_t t = t0 + (P16 ? 16 * u : (int)(lane % 32));
             if (!in_sight(t)) continue;
             poison |= p.id[u] >= pool;
-            w.at[u] = ((uint64_t)(p.id[u] < pool ? p.id[u] : 0) * a.cache.heads + head) * page + split_by(t, page, a.page_inv).y;
+            w.at[u] = ((uint64_t)(p.id[u] < pool ? p.id[u] : 0) * a.cache.heads + head) * page + split_by(t, page, a.cache.page_inv).y;
         }
         return w;
     };
@@ -509,7 +503,12 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
                     rest[j] -= (float)w[rt][0][j];
                 }
 #pragma unroll
-            for (int j = 0; j < 8; j++) w[rt][1][j] = (MV)rest[j];
+            for (int i = 1; i < PP; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    w[rt][i][j] = (MV)rest[j];
+                    rest[j] -= (float)w[rt][i][j];
+                }
         }
         bool stray = false;
         constexpr uint32_t E = std::is_same_v<MV, half_t> ? 0x7C00u : 0x7F80u; // the exponent of what is not finite

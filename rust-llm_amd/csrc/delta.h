@@ -18,7 +18,6 @@ struct DeltaArgs {
     uint32_t wide;    // whether q, k, v and out are aligned for 16-byte accesses
 };
 
-constexpr uint32_t DELTA_COLS = 16; // value columns a wave
 constexpr uint32_t DELTA_WAVES = 4;
 
 // Where a sequence's rows begin, within the call's rows whatever `starts` holds.
@@ -26,26 +25,30 @@ __device__ inline uint32_t first_row(const DeltaArgs &a, uint32_t s) {
     return a.starts ? (uint32_t)min(max(a.starts[s], 0), (int)a.rows) : s;
 }
 
-// Sum over the 16 lanes that hold one column quad (lanes 4 apart).
+// Sum over the lanes Q apart, which hold one column quad.
+template <int Q>
 __device__ inline float quad_sum(float x) {
     x += rotate16<8>(x);
-    return rows_sum(x + rotate16<4>(x));
+    x += rotate16<4>(x);
+    if (Q == 2) x += rotate16<2>(x);
+    return rows_sum(x);
 }
 
-// A wave holds 16 columns of one head's state in registers: a column does not
+// A wave holds 4 Q columns of one head's state in registers (16, or 8 where 16
+// leave SIMDs idle and the chain of a step counts): a column does not
 // depend on the others, so a state splits over as many waves as it has column
-// groups and no wave waits for another. Lane l has the columns 4 (l % 4) .. + 4 of
-// the rows R (l / 4) .. + R; the two products with the state are summed over the
-// 16 lanes of a column, in registers. A step's inputs are loaded, and made ready,
+// groups and no wave waits for another. Lane l has the columns 4 (l % Q) .. + 4 of
+// the rows R (l / Q) .. + R; the two products with the state are summed over the
+// 64 / Q lanes of a column, in registers. A step's inputs are loaded, and made ready,
 // while the one before is computed. For single tokens bound by HBM (the state is
 // read and written once); for several by the chain of a step.
-template <typename T, int R>
+template <typename T, int R, int Q>
 __global__ void __launch_bounds__(64 * DELTA_WAVES) k_delta_steps(DeltaArgs a) {
-    const uint32_t lane = threadIdx.x % 64, col0 = (blockIdx.y * DELTA_WAVES + threadIdx.x / 64) * DELTA_COLS;
+    const uint32_t lane = threadIdx.x % 64, col0 = (blockIdx.y * DELTA_WAVES + threadIdx.x / 64) * 4 * Q;
     const uint32_t s = blockIdx.x / a.value_heads, head = blockIdx.x - s * a.value_heads;
     if (col0 >= a.value_dim) return;
     const uint32_t key_head = head / (a.value_heads / a.key_heads);
-    const uint32_t col = col0 + 4 * (lane % 4), row0 = R * (lane / 4);
+    const uint32_t col = col0 + 4 * (lane % Q), row0 = R * (lane / Q);
     const uint32_t begin = first_row(a, s), end = first_row(a, s + 1);
     const int32_t in = a.slots_in[s], to = a.slots_out[s];
     const uint64_t size = (uint64_t)a.key_dim * a.value_dim;
@@ -79,8 +82,8 @@ __global__ void __launch_bounds__(64 * DELTA_WAVES) k_delta_steps(DeltaArgs a) {
             float kk = 0.0f, qq = 0.0f;
 #pragma unroll
             for (int j = 0; j < R; j++) kk = fmaf(k[j], k[j], kk), qq = fmaf(q[j], q[j], qq);
-            kn = 1.0f / sqrtf(quad_sum(kk) + a.eps);
-            qn = a.scale / sqrtf(quad_sum(qq) + a.eps);
+            kn = 1.0f / sqrtf(quad_sum<Q>(kk) + a.eps);
+            qn = a.scale / sqrtf(quad_sum<Q>(qq) + a.eps);
         }
 #pragma unroll
         for (int j = 0; j < R; j++) kc[j] = k[j] * kn, qc[j] = q[j] * qn;
@@ -96,7 +99,7 @@ __global__ void __launch_bounds__(64 * DELTA_WAVES) k_delta_steps(DeltaArgs a) {
                 p[c] = fmaf(S[j][c], kc[j], p[c]);
             }
 #pragma unroll
-        for (int c = 0; c < 4; c++) p[c] = b * (vc[c] - quad_sum(p[c]));
+        for (int c = 0; c < 4; c++) p[c] = b * (vc[c] - quad_sum<Q>(p[c]));
 #pragma unroll
         for (int j = 0; j < R; j++)
 #pragma unroll
@@ -105,8 +108,8 @@ __global__ void __launch_bounds__(64 * DELTA_WAVES) k_delta_steps(DeltaArgs a) {
                 o[c] = fmaf(S[j][c], qc[j], o[c]);
             }
 #pragma unroll
-        for (int c = 0; c < 4; c++) o[c] = quad_sum(o[c]);
-        if (lane < 4) store_f32((T *)a.out + t * a.out_row + head * a.out_head + col, a.wide, o);
+        for (int c = 0; c < 4; c++) o[c] = quad_sum<Q>(o[c]);
+        if (lane < Q) store_f32((T *)a.out + t * a.out_row + head * a.out_head + col, a.wide, o);
     }
     if (to < 0 || (uint64_t)to >= a.state_slots || !here) return;
     float *dst = a.states + ((uint64_t)to * a.value_heads + head) * size + (uint64_t)row0 * a.value_dim + col;

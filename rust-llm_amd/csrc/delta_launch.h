@@ -10,12 +10,21 @@ void launch_delta_steps(const DeltaArgs &a, hipStream_t s);
 template <typename T>
 void launch_delta_chunks(const DeltaArgs &a, const DeltaWork &w, hipStream_t s);
 
+constexpr uint32_t DELTA_FEW = 512;
+
 #ifdef RL_DELTA_UNIT
+template <typename T, int Q>
+void launch_delta_steps_of(const DeltaArgs &a, hipStream_t s) {
+    constexpr uint32_t PER = 4 * Q * DELTA_WAVES;
+    auto kern = a.key_dim <= 64 ? k_delta_steps<T, Q, Q> : a.key_dim <= 128 ? k_delta_steps<T, 2 * Q, Q> : k_delta_steps<T, 4 * Q, Q>;
+    hipLaunchKernelGGL(kern, dim3(a.seqs * a.value_heads, (a.value_dim + PER - 1) / PER), dim3(64 * DELTA_WAVES), 0, s, a);
+}
+
 template <typename T>
 void launch_delta_steps(const DeltaArgs &a, hipStream_t s) {
-    constexpr uint32_t PER = DELTA_COLS * DELTA_WAVES;
-    auto kern = a.key_dim <= 64 ? k_delta_steps<T, 4> : a.key_dim <= 128 ? k_delta_steps<T, 8> : k_delta_steps<T, 16>;
-    hipLaunchKernelGGL(kern, dim3(a.seqs * a.value_heads, (a.value_dim + PER - 1) / PER), dim3(64 * DELTA_WAVES), 0, s, a);
+    // Waves of 16 columns unless they leave half the SIMDs idle.
+    if ((uint64_t)a.seqs * a.value_heads * (a.value_dim / 16) <= DELTA_FEW) launch_delta_steps_of<T, 2>(a, s);
+    else launch_delta_steps_of<T, 4>(a, s);
 }
 
 template <typename T, int DK>

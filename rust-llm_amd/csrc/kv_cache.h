@@ -15,12 +15,17 @@ struct CacheArgs {
     float *key_steps, *value_steps;
     uint64_t slots;
     uint32_t page, heads, dim;
+    uint32_t page_inv, vectors_inv; // inverse_of the page and of the vectors of a row, 2 heads
 };
 
 // The vector of a slot and head, counted in vectors of dim values.
 __device__ inline uint64_t cache_vector(const CacheArgs &c, uint64_t slot, uint32_t head) {
-    const uint64_t p = slot / c.page;
-    return (p * c.heads + head) * c.page + (slot - p * c.page);
+    if (c.slots >> 32) {
+        const uint64_t p = slot / c.page;
+        return (p * c.heads + head) * c.page + (slot - p * c.page);
+    }
+    const uint2 p = split_by((uint32_t)slot, c.page, c.page_inv);
+    return ((uint64_t)p.x * c.heads + head) * c.page + p.y;
 }
 
 struct CacheRows {
@@ -32,22 +37,28 @@ struct CacheRows {
 
 constexpr uint32_t CACHE_THREADS = 256;
 constexpr uint32_t CACHE_MAX_ROWS = 16; // rows a workgroup, LDS holds their angles
+constexpr int CACHE_AHEAD = 2;          // vectors that a group of lanes has on their way
 
-// Eight values of a head's key, turned if they are among the turned ones. A
-// partner that another lane holds is read again (it is in the cache).
+// Turns eight values of a head's key if they are among the turned ones, y their partners where they are eight in a row
+// (half layout of a multiple of 8 pairs; another lane's, read again), else read here.
 template <typename T>
-__device__ inline void turned8(const RotaryArgs &r, const T *in, bool wide, uint32_t at, const float2 *cs,
-                               float (&x)[8]) {
+__device__ inline void turn8(const RotaryArgs &r, const T *in, uint32_t at, const float2 *cs, const vec<T, 8> &y, float (&x)[8]) {
     const uint32_t turned = 2 * r.pairs;
-    load_f32(in + at, wide, x);
     if (at >= turned) return;
     if (!r.interleaved && r.pairs % 8 == 0) {
         const bool second = at >= r.pairs;
         const uint32_t i = second ? at - r.pairs : at;
-        float y[8];
-        load_f32(in + (second ? i : at + r.pairs), wide, y);
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = second ? turn_b(y[j], x[j], cs[i + j]) : turn_a(x[j], y[j], cs[i + j]);
+        for (int j = 0; j < 8; j++)
+            x[j] = second ? turn_b((float)y[j], x[j], cs[i + j]) : turn_a(x[j], (float)y[j], cs[i + j]);
+    } else if (r.interleaved && at + 8 <= turned) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const float2 w = cs[(at + j) / 2];
+            const float p = x[j], q = x[j + 1];
+            x[j] = turn_a(p, q, w);
+            x[j + 1] = turn_b(p, q, w);
+        }
     } else {
         for (int j = 0; j < 8 && at + j < turned; j++) {
             const uint32_t e = at + j;
@@ -64,57 +75,114 @@ __device__ inline void turned8(const RotaryArgs &r, const T *in, bool wide, uint
 
 // G lanes hold a vector of up to 8 G values, eight a lane. Vectors of a workgroup's
 // rows: keys of every head, then values of every head. One pass: the largest
-// magnitude is reduced over the lanes while the values stay in registers.
+// magnitude is reduced over the lanes while the values stay in registers. The
+// first CACHE_AHEAD vectors of a group are loaded before the angles are formed and
+// waited for. Bound by HBM for a prompt, by its chain of loads for a few tokens.
 template <typename T, int FMT, int G>
 __global__ void __launch_bounds__(CACHE_THREADS) k_cache_write(CacheArgs c, CacheRows in, const int64_t *slots,
                                                                uint32_t rows_a_group, RotaryArgs r,
                                                                const int64_t *positions) {
     __shared__ float2 cs[CACHE_MAX_ROWS * ROTARY_MAX_PAIRS / 2];
+    constexpr uint32_t GROUPS = CACHE_THREADS / G;
     const uint32_t row0 = blockIdx.x * rows_a_group, n = min(rows_a_group, in.rows - row0);
+    const uint32_t lane = threadIdx.x % G, at = lane * 8, all = n * 2 * c.heads;
+    const bool here = at < c.dim, wide = in.wide;
+    const uint32_t from = here ? at : 0; // lanes past the head's end load its start
+    // The partners of the lane's values, if they are turned and lie eight in a row.
+    const bool pairs8 = !r.interleaved && r.pairs % 8 == 0 && at < 2 * r.pairs;
+    const uint32_t other = !pairs8 ? from : at >= r.pairs ? at - r.pairs : at + r.pairs;
+    struct Item {
+        const T *p;
+        bool is_value;
+        uint32_t rr, head;
+        int64_t slot;
+        vec<T, 8> x, y;
+    };
+    auto load = [&](uint32_t i, Item &t) { // past the end the last vector again
+        i = min(i, all - 1);
+        const uint2 row_vector = split_by(i, 2 * c.heads, c.vectors_inv);
+        t.rr = row_vector.x;
+        const uint32_t h2 = row_vector.y;
+        t.is_value = h2 >= c.heads;
+        t.head = t.is_value ? h2 - c.heads : h2;
+        const uint64_t row = row0 + t.rr;
+        t.slot = slots[row];
+        t.p = t.is_value ? (const T *)in.values + row * in.value_row + t.head * in.value_head
+                         : (const T *)in.keys + row * in.key_row + t.head * in.key_head;
+        if (wide) {
+            constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+            for (int j = 0; j < 8; j += PER) {
+                const vec<T, PER> x = *(const vec<T, PER> *)(t.p + from + j);
+#pragma unroll
+                for (int e = 0; e < PER; e++) t.x[j + e] = x[e];
+            }
+            if (pairs8 && !t.is_value)
+#pragma unroll
+                for (int j = 0; j < 8; j += PER) {
+                    const vec<T, PER> y = *(const vec<T, PER> *)(t.p + other + j);
+#pragma unroll
+                    for (int e = 0; e < PER; e++) t.y[j + e] = y[e];
+                }
+        } else
+#pragma unroll
+            for (int j = 0; j < 8; j++) t.x[j] = t.p[from + j], t.y[j] = t.p[other + j];
+    };
+    auto store = [&](const Item &t) {
+        if (t.slot < 0 || (uint64_t)t.slot >= c.slots) return;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = here ? (float)t.x[j] : 0.0f;
+        if (here && !t.is_value) turn8(r, t.p, at, cs + t.rr * r.pairs, t.y, x);
+        const uint64_t v = cache_vector(c, (uint64_t)t.slot, t.head);
+        if constexpr (FMT == RL_F16 || FMT == RL_BF16) {
+            using S = std::conditional_t<FMT == RL_F16, half_t, bhalf_t>;
+            if (here) store_f32((S *)(t.is_value ? c.values : c.keys) + v * c.dim + at, true, x);
+        } else {
+            constexpr float TOP = FMT == RL_I8 ? 127.0f : 448.0f;
+            // The largest magnitude by its bits, in which infinities and NaNs are the largest.
+            uint32_t most = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(x[j]) & 0x7FFFFFFFu);
+            const float m = __uint_as_float(group_max_bits<G>(most));
+            const float step = m < INFINITY ? m / TOP : NAN;
+            float y[8];
+            if (step > 0x1p-90f && step < 0x1p90f) {
+                // The IEEE quotient by one reciprocal: x r and its remainder's correction are correctly rounded where r is
+                // the rounded 1 / step and nothing leaves the normal numbers (Markstein); quotients below 2^-9 round to 0
+                // either way.
+                const float r = 1.0f / step;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float z = x[j] * r;
+                    y[j] = __builtin_amdgcn_fmed3f(fmaf(fmaf(-z, step, x[j]), r, z), -TOP, TOP);
+                }
+            } else
+#pragma unroll
+                for (int j = 0; j < 8; j++) y[j] = step > 0.0f ? __builtin_amdgcn_fmed3f(x[j] / step, -TOP, TOP) : 0.0f;
+            if (here) {
+                uint2 u = encode8<FMT>(y);
+                if (FMT == RL_I8 && !t.is_value) u.x ^= KEY_SIGNS, u.y ^= KEY_SIGNS;
+                *reinterpret_cast<uint2 *>((uint8_t *)(t.is_value ? c.values : c.keys) + v * c.dim + at) = u;
+                if (lane == 0) (t.is_value ? c.value_steps : c.key_steps)[v] = step;
+            }
+        }
+    };
+    Item item[CACHE_AHEAD];
+    const uint32_t group = threadIdx.x / G;
+#pragma unroll
+    for (int j = 0; j < CACHE_AHEAD; j++) load(group + j * GROUPS, item[j]);
     for (uint32_t i = threadIdx.x; i < n * r.pairs; i += CACHE_THREADS)
         cs[i] = rotary_angle(r, positions[row0 + i / r.pairs], i % r.pairs);
     if (r.pairs) __syncthreads();
-    const uint32_t lane = threadIdx.x % G, at = lane * 8;
-    const bool here = at < c.dim, wide = in.wide;
-    for (uint32_t i = threadIdx.x / G; i < n * 2 * c.heads; i += CACHE_THREADS / G) {
-        const uint32_t rr = i / (2 * c.heads), h2 = i - rr * 2 * c.heads;
-        const bool is_value = h2 >= c.heads;
-        const uint32_t head = is_value ? h2 - c.heads : h2;
-        const uint64_t row = row0 + rr;
-        const int64_t slot = slots[row];
-        if (slot < 0 || (uint64_t)slot >= c.slots) continue;
-        float x[8] = {};
-        if (here) {
-            if (is_value)
-                load_f32((const T *)in.values + row * in.value_row + head * in.value_head + at, wide, x);
-            else
-                turned8(r, (const T *)in.keys + row * in.key_row + head * in.key_head, wide, at, cs + rr * r.pairs, x);
-        }
-        const uint64_t v = cache_vector(c, (uint64_t)slot, head);
-        if constexpr (FMT == RL_F16 || FMT == RL_BF16) {
-            using S = std::conditional_t<FMT == RL_F16, half_t, bhalf_t>;
-            if (here) store_f32((S *)(is_value ? c.values : c.keys) + v * c.dim + at, true, x);
-        } else {
-            constexpr float TOP = FMT == RL_I8 ? 127.0f : 448.0f;
-            float m = 0.0f;
-            bool bad = false; // an infinity or a NaN
+    for (uint32_t i = group;;) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                m = fmaxf(m, fabsf(x[j]));
-                bad |= !(fabsf(x[j]) < INFINITY);
-            }
-            m = group_max<G>(bad ? INFINITY : m);
-            const float step = m < INFINITY ? m / TOP : NAN;
-            float y[8];
+        for (int j = 0; j < CACHE_AHEAD; j++)
+            if (i + j * GROUPS < all) store(item[j]);
+        i += CACHE_AHEAD * GROUPS;
+        if (i >= all) break;
 #pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = step > 0.0f ? fminf(fmaxf(x[j] / step, -TOP), TOP) : 0.0f;
-            if (here) {
-                uint2 u = encode8<FMT>(y);
-                if (FMT == RL_I8 && !is_value) u.x ^= KEY_SIGNS, u.y ^= KEY_SIGNS;
-                *reinterpret_cast<uint2 *>((uint8_t *)(is_value ? c.values : c.keys) + v * c.dim + at) = u;
-                if (lane == 0) (is_value ? c.value_steps : c.key_steps)[v] = step;
-            }
-        }
+        for (int j = 0; j < CACHE_AHEAD; j++) load(i + j * GROUPS, item[j]);
     }
 }
 
@@ -122,11 +190,11 @@ __global__ void __launch_bounds__(CACHE_THREADS) k_cache_write(CacheArgs c, Cach
 template <typename T, int FMT, int G>
 __global__ void __launch_bounds__(CACHE_THREADS) k_cache_read(CacheArgs c, CacheRows out, const int64_t *slots) {
     const uint32_t lane = threadIdx.x % G, at = lane * 8;
-    const uint64_t i = (uint64_t)blockIdx.x * (CACHE_THREADS / G) + threadIdx.x / G;
-    const uint32_t per = 2 * c.heads;
-    const uint64_t row = i / per;
+    // At most 2^23 workgroups of 32 vectors: below 2^28.
+    const uint2 row_vector = split_by(blockIdx.x * (CACHE_THREADS / G) + threadIdx.x / G, 2 * c.heads, c.vectors_inv);
+    const uint64_t row = row_vector.x;
     if (row >= out.rows || at >= c.dim) return;
-    const uint32_t h2 = (uint32_t)(i - row * per);
+    const uint32_t h2 = row_vector.y;
     const bool is_value = h2 >= c.heads;
     const uint32_t head = is_value ? h2 - c.heads : h2;
     const int64_t slot = slots[row];

@@ -337,6 +337,7 @@ int rl_kv_cache_create(int device, uint32_t pages, uint32_t page, uint32_t kv_he
     c->format = format;
     c->args.slots = slots;
     c->args.page = page, c->args.heads = kv_heads, c->args.dim = dim;
+    c->args.page_inv = inverse_of(page), c->args.vectors_inv = inverse_of(2 * kv_heads);
     const uint64_t codes = slots * kv_heads * dim * type_bytes(format), steps = slots * kv_heads * sizeof(float);
     hipError_t e = hipMalloc(&c->args.keys, codes);
     if (e == hipSuccess) e = hipMalloc(&c->args.values, codes);
@@ -382,8 +383,9 @@ int rl_kv_cache_write(rl_kv_cache *c, const rl_heads *keys, const rl_heads *valu
         with_format(c->format, [&](auto f) {
             with_group(c->args.dim, [&](auto g) {
                 constexpr int G = decltype(g)::value;
-                // As many rows as fill the workgroup's groups of lanes.
-                const uint32_t per = std::min(std::max(CACHE_THREADS / G / (2 * c->args.heads), 1u), CACHE_MAX_ROWS);
+                // As many rows as give each group of lanes the vectors it loads ahead, while that leaves two workgroups a CU.
+                const uint32_t vectors = CACHE_THREADS / G * (rows >= 2 * CUS * 4 ? CACHE_AHEAD : 1);
+                const uint32_t per = std::min(std::max(vectors / (2 * c->args.heads), 1u), CACHE_MAX_ROWS);
                 hipLaunchKernelGGL((k_cache_write<decltype(t), decltype(f)::value, G>), dim3((rows + per - 1) / per),
                                    dim3(CACHE_THREADS), 0, static_cast<hipStream_t>(stream), c->args, in, slots, per, r,
                                    positions);
@@ -486,11 +488,10 @@ int rl_attention_rows(rl_attention *h, const rl_kv_cache *cache, const rl_heads 
     a.out_row = out->row_stride, a.out_head = out->head_stride;
     a.starts = starts, a.lens = lens, a.pages = pages;
     a.rows = rows, a.seqs = seqs, a.q_heads = h->q_heads, a.table_width = table_width, a.window = window;
-    a.most_rows = most_rows ? std::min(most_rows, rows) : rows;
+    a.most_rows = !starts ? 1 : most_rows ? std::min(most_rows, rows) : rows;
     a.max_len = max_len ? max_len : h->max_len;
     a.scale = scale;
     a.group = h->q_heads / h->kv_heads;
-    a.page_inv = (uint32_t)std::min<uint64_t>((1ull << 32) / cache->args.page, 0xFFFFFFFFu);
     a.wide = wide(q) && wide(out);
     a.part_out = h->part_out, a.part_sum = h->part_sum, a.part_count = h->part_count;
     // Two row tiles a workgroup where a sequence has more than one: the keys and values are read once for both.
@@ -601,7 +602,7 @@ int rl_delta_rows(rl_delta *h, const rl_heads *q, const rl_heads *k, const rl_he
     a.scale = scale, a.eps = norm_eps;
     a.wide = wide(q) && wide(k) && wide(v) && wide(out);
     // Chunks where some sequence has the rows for them and the workspace holds all.
-    const uint32_t most = most_rows ? std::min(most_rows, rows) : rows;
+    const uint32_t most = !starts ? 1 : most_rows ? std::min(most_rows, rows) : rows;
     const bool alone = (uint64_t)seqs * h->value_heads * (h->value_dim / 16) <= CUS;
     const uint32_t least = !alone ? DELTA_CHUNKED_MANY : q->dtype == RL_BF16 ? DELTA_CHUNKED : DELTA_CHUNKED_WIDE;
     const bool chunked = most >= least && rows / CHUNK + seqs <= h->chunks;
