@@ -94,8 +94,8 @@ int rl_rotary_rows(rl_rotary *rotary, const int64_t *positions, uint32_t rows, c
  * throughout in these two. */
 typedef struct rl_kv_cache rl_kv_cache;
 
-/* dim: 16 to 256, a multiple of 16. page and pages: any from 1; pages * page
- * below 2^40 tokens. The contents start as zeros. */
+/* dim: 16 to 256, a multiple of 16. page and pages: any from 1; pages * page at
+ * most 2^32 tokens, kv_heads at most 2^16. The contents start as zeros. */
 int rl_kv_cache_create(int device, uint32_t pages, uint32_t page, uint32_t kv_heads, uint32_t dim, uint32_t format,
                        rl_kv_cache **out);
 void rl_kv_cache_destroy(rl_kv_cache *cache);
@@ -124,13 +124,15 @@ int rl_kv_cache_read(rl_kv_cache *cache, const int64_t *slots, uint32_t rows, co
  * tokens up to its own, with window > 0 the last `window` of them:
  *   out = sum_t softmax_t(scale q . k_t) v_t,  lse = ln sum_t exp(scale q . k_t)
  * Query head h reads the key-value head h / (q_heads / kv_heads). A row that sees
- * nothing gives zeros and an lse of -inf. Scores, softmax and sums are f32; with
- * f16 and bf16 queries the weights are rounded to 16 bits before the product
- * with the values, with f32 queries every product is good to f32. */
+ * nothing gives zeros and an lse of -inf. Scores, softmax and sums are f32; the
+ * weights go into the product with the values as sums of 16-bit parts, good to 16
+ * bits or more for 16-bit queries and to 22 or more for f32 ones. An infinity in an
+ * f16 or bf16 value that only some rows of a sequence see may read as NaN there. */
 typedef struct rl_attention rl_attention;
 
 /* Workspace for calls of up to max_rows query rows over caches of kv_heads heads
- * and up to max_len tokens a sequence. q_heads: a multiple of kv_heads. */
+ * and up to max_len tokens a sequence. q_heads: a multiple of kv_heads;
+ * max_rows * q_heads at most 2^23. */
 int rl_attention_create(int device, uint32_t max_rows, uint32_t q_heads, uint32_t kv_heads, uint32_t dim,
                         uint32_t max_len, rl_attention **out);
 void rl_attention_destroy(rl_attention *attention);
@@ -157,8 +159,10 @@ int rl_attention_rows(rl_attention *attention, const rl_kv_cache *cache, const r
  * sums are f32. */
 typedef struct rl_delta rl_delta;
 
-/* Workspace for calls of up to max_rows tokens in up to max_seqs sequences.
- * value_heads: a multiple of key_heads. key_dim, value_dim: 16 to 256, multiples
+/* Workspace for calls of up to max_rows tokens in up to max_seqs sequences (none is
+ * needed below 13 rows; else about 64 KB a value head for every 64 rows, and
+ * for every sequence that has 16 rows or more to itself on average). value_heads:
+ * a multiple of key_heads. key_dim, value_dim: 16 to 256, multiples
  * of 16. */
 int rl_delta_create(int device, uint32_t max_rows, uint32_t max_seqs, uint32_t key_heads, uint32_t value_heads,
                     uint32_t key_dim, uint32_t value_dim, rl_delta **out);

@@ -13,18 +13,14 @@ constexpr uint32_t KEY_SIGNS = 0x80808080u;
 struct CacheArgs {
     void *keys, *values;
     float *key_steps, *value_steps;
-    uint64_t slots;
+    uint64_t slots; // at most 2^32
     uint32_t page, heads, dim;
     uint32_t page_inv, vectors_inv; // inverse_of the page and of the vectors of a row, 2 heads
 };
 
 // The vector of a slot and head, counted in vectors of dim values.
-__device__ inline uint64_t cache_vector(const CacheArgs &c, uint64_t slot, uint32_t head) {
-    if (c.slots >> 32) {
-        const uint64_t p = slot / c.page;
-        return (p * c.heads + head) * c.page + (slot - p * c.page);
-    }
-    const uint2 p = split_by((uint32_t)slot, c.page, c.page_inv);
+__device__ inline uint64_t cache_vector(const CacheArgs &c, uint32_t slot, uint32_t head) {
+    const uint2 p = split_by(slot, c.page, c.page_inv);
     return ((uint64_t)p.x * c.heads + head) * c.page + p.y;
 }
 
@@ -134,7 +130,7 @@ __global__ void __launch_bounds__(CACHE_THREADS) k_cache_write(CacheArgs c, Cach
 #pragma unroll
         for (int j = 0; j < 8; j++) x[j] = here ? (float)t.x[j] : 0.0f;
         if (here && !t.is_value) turn8(r, t.p, at, cs + t.rr * r.pairs, t.y, x);
-        const uint64_t v = cache_vector(c, (uint64_t)t.slot, t.head);
+        const uint64_t v = cache_vector(c, (uint32_t)t.slot, t.head);
         if constexpr (FMT == RL_F16 || FMT == RL_BF16) {
             using S = std::conditional_t<FMT == RL_F16, half_t, bhalf_t>;
             if (here) store_f32((S *)(t.is_value ? c.values : c.keys) + v * c.dim + at, true, x);
@@ -203,7 +199,7 @@ __global__ void __launch_bounds__(CACHE_THREADS) k_cache_read(CacheArgs c, Cache
 #pragma unroll
         for (int j = 0; j < 8; j++) x[j] = NAN;
     } else {
-        const uint64_t v = cache_vector(c, (uint64_t)slot, head);
+        const uint64_t v = cache_vector(c, (uint32_t)slot, head);
         const void *codes = is_value ? c.values : c.keys;
         if constexpr (FMT == RL_F16 || FMT == RL_BF16) {
             using S = std::conditional_t<FMT == RL_F16, half_t, bhalf_t>;

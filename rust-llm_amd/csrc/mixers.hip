@@ -157,7 +157,7 @@ int check_cache_rows(const rl_kv_cache *c, const rl_heads *k, const rl_heads *v,
     for (const rl_heads *h : {k, v})
         if (h->heads != c->args.heads || h->dim != c->args.dim)
             return fail(RL_ERR_ARGUMENT, "keys and values must have the cache's heads and dim");
-    if (!slots) return fail(RL_ERR_ARGUMENT, "slots must be a device pointer");
+    if (rows && !slots) return fail(RL_ERR_ARGUMENT, "slots must be a device pointer");
     if (rows > MAX_ROWS) return fail(RL_ERR_CAPACITY, "more than 2^23 rows in a call");
     return RL_OK;
 }
@@ -328,7 +328,7 @@ int rl_kv_cache_create(int device, uint32_t pages, uint32_t page, uint32_t kv_he
     if (dim < 16 || dim > 256 || dim % 16) return fail(RL_ERR_ARGUMENT, "dim must be a multiple of 16, from 16 to 256");
     if (format < RL_F16 || format > RL_F8) return fail(RL_ERR_ARGUMENT, "unknown cache format");
     const uint64_t slots = (uint64_t)pages * page;
-    if (slots >> 40 || kv_heads > 1u << 16) return fail(RL_ERR_CAPACITY, "the cache is too large");
+    if (slots > 1ull << 32 || kv_heads > 1u << 16) return fail(RL_ERR_CAPACITY, "the cache is too large");
     DeviceGuard guard(device);
     if (!guard.ok) return fail(RL_ERR_DEVICE, "cannot select device " + std::to_string(device));
     auto *c = new (std::nothrow) rl_kv_cache();
@@ -584,7 +584,7 @@ int rl_delta_rows(rl_delta *h, const rl_heads *q, const rl_heads *k, const rl_he
         if (x->dtype != q->dtype) return fail(RL_ERR_ARGUMENT, "q, k, v and out have one type");
     if (rows > h->max_rows || seqs > h->max_seqs) return fail(RL_ERR_CAPACITY, "rows or seqs above the handle's");
     if (seqs == 0) return rows == 0 ? RL_OK : fail(RL_ERR_ARGUMENT, "rows without sequences");
-    if (!g || !beta || !states || !slots_in || !slots_out)
+    if ((rows && (!g || !beta)) || !states || !slots_in || !slots_out)
         return fail(RL_ERR_ARGUMENT, "g, beta, states and slots must be device pointers");
     if ((uintptr_t)states % 16) return fail(RL_ERR_ARGUMENT, "states must be aligned to 16 bytes");
     if (!starts && rows != seqs) return fail(RL_ERR_ARGUMENT, "without starts there is one row a sequence");
