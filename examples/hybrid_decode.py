@@ -84,7 +84,7 @@ class HybridModel:
         lens = torch.tensor(self.lens, dtype=torch.int32, device=DEV)
         own = torch.arange(seqs, dtype=torch.int32, device=DEV)
         most = max(counts)
-        x = norm(self.head.embed(tokens))
+        x = 0.2 * norm(self.head.embed(tokens))
         for kind, (w_in, w_out), cache, states in zip(self.layers, self.weights, self.caches, self.states):
             y = norm(x) @ w_in
             if kind == "a":

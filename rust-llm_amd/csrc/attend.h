@@ -55,7 +55,7 @@ constexpr int attend_resident(uint32_t query_bytes, uint32_t format, uint32_t di
     switch (attend_dim(dim)) {
     case 64: return row_tiles == 1 ? 3 : 2;
     case 128: return row_tiles == 1 ? (eight && query_bytes == 2 ? 3 : 2) : eight ? 2 : 1;
-    default: return row_tiles == 1 && eight && query_bytes == 2 ? 2 : 1;
+    default: return row_tiles == 1 && eight ? 2 : 1;
     }
 }
 
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
 
     // Where a tile's tokens lie. P16 (pages of a multiple of 16 tokens): each half of a tile lies in one page, at[u] is
     // its first vector. Else lane l has the vector of token l % 32. Tokens that no row sees, whose pages are not looked
-    // up, are loaded from the cache's first vectors instead, so no load is conditional; what is loaded there is masked.
+    // up, are the nearest that some row does: what is loaded for them is masked, and no load is conditional.
     // Page numbers are fetched two tiles ahead, before the keys of the next: waiting for them waits for nothing newer.
     struct Place {
         uint64_t at[2];
@@ -226,23 +226,20 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
         uint32_t id[2];
     };
     auto in_sight = [&](int32_t t) {
-        return P16 ? t < end_max && t + 16 > begin_min : t < end_max && t >= begin_min;
+        return (uint32_t)(P16 ? min(max(t, begin_min & ~15), (end_max - 1) & ~15) : min(max(t, begin_min), end_max - 1));
     };
     auto fetch = [&](int32_t t0) {
         Pages p{{0, 0}};
 #pragma unroll
-        for (int u = 0; u < (P16 ? 2 : 1); u++) {
-            const int32_t t = t0 + (P16 ? 16 * u : (int)(lane % 32));
-            if (in_sight(t)) p.id[u] = (uint32_t)table[split_by(t, page, a.cache.page_inv).x];
-        }
+        for (int u = 0; u < (P16 ? 2 : 1); u++)
+            p.id[u] = (uint32_t)table[split_by(in_sight(t0 + (P16 ? 16 * u : (int)(lane % 32))), page, a.cache.page_inv).x];
         return p;
     };
     auto place = [&](int32_t t0, const Pages &p) {
         Place w{{0, 0}};
 #pragma unroll
         for (int u = 0; u < (P16 ? 2 : 1); u++) {
-            const int32_t t = t0 + (P16 ? 16 * u : (int)(lane % 32));
-            if (!in_sight(t)) continue;
+            const uint32_t t = in_sight(t0 + (P16 ? 16 * u : (int)(lane % 32)));
             poison |= p.id[u] >= pool;
             w.at[u] = ((uint64_t)(p.id[u] < pool ? p.id[u] : 0) * a.cache.heads + head) * page + split_by(t, page, a.cache.page_inv).y;
         }
@@ -338,12 +335,16 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     int32_t tile = part_begin + (int32_t)wave;
     Pages ahead{{0, 0}}; // of this wave's next tile
     if (tile < part_end) {
-        const int32_t t0 = tile * (int)ATTEND_TILE, t1 = (tile + (int)ATTEND_WAVES) * (int)ATTEND_TILE;
+        // In the order of the loop's own loads: a wait in the loop has to hold for the first tile too.
+        const int32_t t0 = tile * (int)ATTEND_TILE;
         const Pages now = fetch(t0);
-        if (tile + (int)ATTEND_WAVES < part_end) ahead = fetch(t1);
+        ahead = fetch(t0 + (int)(ATTEND_WAVES * ATTEND_TILE));
         const Place at = place(t0, now);
+        __builtin_amdgcn_sched_barrier(0);
         load_keys(at);
+        __builtin_amdgcn_sched_barrier(0);
         load_values(at);
+        __builtin_amdgcn_sched_barrier(0);
     }
     // Queries into LDS in the type of the product. In f16 a row is scaled by the power of two that brings its largest
     // value to [1, 2), which costs nothing of its values down to 2^-24 of the largest.
@@ -406,9 +407,11 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
         row_begin[rt] = r < count ? span.begin(i) : begin_min; // rows past the block's see what any of it sees
         row_end[rt] = r < count ? span.end(i) : end_max;
     }
-    for (; tile < part_end; tile += ATTEND_WAVES) {
+    // A tile; with `more` the next one's loads go out as their registers become free. That is known to the compiler, so
+    // that a wait for this tile's values leaves the next one's keys on their way.
+    auto step = [&](auto more) {
+        constexpr bool MORE = decltype(more)::value;
         const int32_t t0 = tile * (int)ATTEND_TILE;
-        const bool more = tile + (int)ATTEND_WAVES < part_end;
         f32x4 S[RT][2];
 #pragma unroll
         for (int u = 0; u < 2; u++)
@@ -443,11 +446,13 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
         }
         const f32x4 step[2] = {ks[0], ks[1]};
         Place next{{0, 0}};
-        if (more) {
-            const int32_t t1 = (tile + (int)ATTEND_WAVES) * (int)ATTEND_TILE;
+        if constexpr (MORE) {
+            const int32_t t1 = t0 + (int)(ATTEND_WAVES * ATTEND_TILE);
             next = place(t1, ahead);
-            if (tile + 2 * (int)ATTEND_WAVES < part_end) ahead = fetch(t1 + (int)(ATTEND_WAVES * ATTEND_TILE));
+            ahead = fetch(t1 + (int)(ATTEND_WAVES * ATTEND_TILE));
+            __builtin_amdgcn_sched_barrier(0);
             load_keys(next);
+            __builtin_amdgcn_sched_barrier(0);
         }
         // A tile that some row of the block does not see all of.
         const bool edge = t0 < begin_max || t0 + (int)ATTEND_TILE > end_min;
@@ -556,8 +561,14 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
             });
         } else
             each_column([&](const u32x4 &v, int column) { multiply(v, w, column); });
-        if (more) load_values(next);
-    }
+        if constexpr (MORE) {
+            __builtin_amdgcn_sched_barrier(0);
+            load_values(next);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    for (; tile + (int)ATTEND_WAVES < part_end; tile += ATTEND_WAVES) step(std::true_type{});
+    if (tile < part_end) step(std::false_type{});
 
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {

@@ -1,12 +1,12 @@
 // C ABI of the token mixers (include/rl_mixers.h): handles, checks of arguments
-// and launches. Kernels are in rotary.h, kv_cache.h, attend.h and delta.h.
+// and launches. Kernels are in rotary.h, kv_cache.h, attend.h, delta.h and
+// delta_chunks.h.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cmath>
 #include <new>
 #include <string>
-#include <vector>
 
 #include "attend.h"
 #include "delta_launch.h"
@@ -18,7 +18,7 @@ struct rl_rotary {
     int device = 0;
     rl_rotary_spec spec{};
     double magnitude = 1.0;
-    std::vector<double> radians;
+    double radians[ROTARY_MAX_PAIRS] = {};
     double *turns = nullptr; // device: revolutions a position
     ~rl_rotary() { (void)hipFree(turns); }
 };
@@ -230,8 +230,7 @@ int rl_rotary_create(int device, const rl_rotary_spec *spec, rl_rotary **out) {
         low = std::max(std::floor(place(fast)), 0.0);
         high = std::min(std::ceil(place(slow)), (double)d - 1.0);
     }
-    std::vector<double> turns(d / 2);
-    r->radians.resize(d / 2);
+    double turns[ROTARY_MAX_PAIRS] = {};
     for (uint32_t i = 0; i < d / 2; i++) {
         double f = std::pow(base, -2.0 * i / d);
         if (spec->scaling == RL_ROTARY_LINEAR) f /= spec->factor;
@@ -245,8 +244,8 @@ int rl_rotary_create(int device, const rl_rotary_spec *spec, rl_rotary **out) {
     r->magnitude = spec->magnitude != 0.0 ? spec->magnitude
                    : spec->scaling == RL_ROTARY_YARN ? 0.1 * std::log(spec->factor) + 1.0
                                                      : 1.0;
-    hipError_t e = hipMalloc(&r->turns, turns.size() * sizeof(double));
-    if (e == hipSuccess) e = hipMemcpy(r->turns, turns.data(), turns.size() * sizeof(double), hipMemcpyHostToDevice);
+    hipError_t e = hipMalloc(&r->turns, sizeof turns);
+    if (e == hipSuccess) e = hipMemcpy(r->turns, turns, sizeof turns, hipMemcpyHostToDevice);
     if (e != hipSuccess) {
         delete r;
         return hip_fail(e, "rl_rotary_create");
@@ -263,7 +262,7 @@ void rl_rotary_destroy(rl_rotary *rotary) {
 
 int rl_rotary_frequencies(const rl_rotary *r, double *radians, double *magnitude) {
     if (!r) return fail(RL_ERR_ARGUMENT, "rotary is null");
-    if (radians) std::copy(r->radians.begin(), r->radians.end(), radians);
+    if (radians) std::copy(r->radians, r->radians + r->spec.dims / 2, radians);
     if (magnitude) *magnitude = r->magnitude;
     return RL_OK;
 }

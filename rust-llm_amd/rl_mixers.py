@@ -66,7 +66,10 @@ _codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 def _stream(t, stream):
     """The stream given, or the current one of the tensor's device (without the
     Stream object of torch.cuda.current_stream, which costs 3 us a call)."""
-    return torch._C._cuda_getCurrentRawStream(t.get_device()) if stream is None else stream
+    device = t.get_device()
+    if device < 0:
+        raise ValueError("the tensors of a call are on a device")
+    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream
 
 
 def _heads(t):

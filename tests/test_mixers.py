@@ -88,3 +88,12 @@ def test_the_statements_agree_with_other_forms():
     # Codes: the largest value is the largest code, halves go to even.
     assert np.array_equal(F.encode(np.array([[127.0, 0.5, 1.5, -2.5]]), "i8"), [[127.0, 0.0, 2.0, -2.0]])
     assert np.array_equal(F.encode(np.array([[448.0, 1.0625, -3.0]]), "f8"), [[448.0, 1.0, -3.0]])
+
+
+def test_host_tensors_are_refused():
+    # Before any call: a kernel could not read them.
+    x, at = torch.zeros(2, 1, 8), torch.zeros(2, dtype=torch.int64)
+    r = M.DeviceRotary.__new__(M.DeviceRotary)
+    r.h = ctypes.c_void_p()
+    with pytest.raises(ValueError, match="device"):
+        r.apply(x, at)
