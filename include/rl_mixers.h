@@ -126,8 +126,9 @@ int rl_kv_cache_read(rl_kv_cache *cache, const int64_t *slots, uint32_t rows, co
  * Query head h reads the key-value head h / (q_heads / kv_heads). A row that sees
  * nothing gives zeros and an lse of -inf. Scores, softmax and sums are f32; the
  * weights go into the product with the values as sums of 16-bit parts, good to 16
- * bits or more for 16-bit queries and to 22 or more for f32 ones. An infinity in an
- * f16 or bf16 value that only some rows of a sequence see may read as NaN there. */
+ * bits or more for 16-bit queries and to 22 or more for f32 ones. What a
+ * row does not see does not reach it, whatever it holds; an infinity among the f16
+ * or bf16 values that only some rows of a sequence see may be NaN to those. */
 typedef struct rl_attention rl_attention;
 
 /* Workspace for calls of up to max_rows query rows over caches of kv_heads heads
@@ -179,8 +180,8 @@ void rl_delta_destroy(rl_delta *delta);
  * sequence without rows passes its state on. most_rows bounds the rows of any one
  * sequence (0: as many as the call has); it picks the form that is used (one
  * token after the other, or chunks on the matrix cores) and no result depends on
- * its being exact. An infinity or NaN in a token may reach the outputs of the 63
- * tokens before it in its own sequence where chunks are used. */
+ * its being exact. What is not finite reaches the tokens after it, none before;
+ * where chunks are used an infinity reads as NaN. */
 int rl_delta_rows(rl_delta *delta, const rl_heads *q, const rl_heads *k, const rl_heads *v, const rl_heads *out,
                   const float *g, uint64_t g_stride, const float *beta, uint64_t beta_stride, float *states,
                   uint64_t state_slots, const int32_t *slots_in, const int32_t *slots_out, const int32_t *starts,

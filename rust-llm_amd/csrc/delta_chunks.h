@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_de
     constexpr size_t K_BYTES = (size_t)CHUNK * KS * sizeof(T), L_BYTES = CHUNK * LS * 4;
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * L_BYTES > K_BYTES ? 2 * L_BYTES : K_BYTES];
     __shared__ double sums[CHUNK];
-    __shared__ float betas[CHUNK], knorm[CHUNK], qnorm[CHUNK];
+    __shared__ float betas[CHUNK], knorm[CHUNK], qnorm[CHUNK], spoilt[CHUNK];
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const uint32_t col = lane % 16, quad = lane / 16;
     const uint32_t chunk = blockIdx.x / a.value_heads, head = blockIdx.x - chunk * a.value_heads;
@@ -202,7 +202,10 @@ __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_de
             if ((int)lane >= d) c += y;
         }
         sums[lane] = c;
-        betas[lane] = b;
+        // What is not finite must not meet the zeros above the diagonal: it is left out of T, and its row marked.
+        const bool fine = fabsf(b) < INFINITY;
+        betas[lane] = fine ? b : 0.0f;
+        spoilt[lane] = fine ? 0.0f : NAN;
     }
     if (rows != CHUNK || a.key_dim != DK) {
 #pragma unroll
@@ -259,15 +262,6 @@ __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_de
             for (int j = 0; j < 8; j++) x[j] = ((const T *)lds)[(f % 2 * 32 + quad * 8 + j) * KS + f / 2 * 16 + col];
             *(vec<T, 8> *)((T *)w.kt + keys + f * FRAGMENT + lane * 8) = x;
         }
-    if (wave == 3) {
-        const double c = sums[lane], whole = sums[CHUNK - 1];
-        float *to = w.rows + at * 4 * CHUNK;
-        const bool here = lane < rows;
-        to[lane] = here ? fast_exp2((float)c) * knorm[lane] : 0.0f;
-        to[CHUNK + lane] = here ? fast_exp2((float)c) * qnorm[lane] : 0.0f;
-        to[2 * CHUNK + lane] = here ? fast_exp2((float)(whole - c)) * knorm[lane] : 0.0f;
-        if (lane == 0) to[3 * CHUNK] = fast_exp2((float)whole);
-    }
 #pragma unroll
     for (int t = 0; t < 4; t++) { // L in place of kk, P of qk; rows and columns past the chunk's are zeros of both
         const uint32_t j = t * 16 + col;
@@ -278,7 +272,10 @@ __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_de
             const uint32_t i = wave * 16 + quad * 4 + e;
             const float f = fast_exp2((float)(sums[i] - cj)) * nj;
             qk[t][e] = j <= i ? qnorm[i] * (qk[t][e] * f) : 0.0f;
-            kk[t][e] = j < i ? betas[i] * (knorm[i] * (kk[t][e] * f)) : 0.0f;
+            const float l = j < i ? betas[i] * (knorm[i] * (kk[t][e] * f)) : 0.0f;
+            const bool fine = fabsf(l) < INFINITY;
+            if (!fine) spoilt[i] = NAN;
+            kk[t][e] = fine ? l : 0.0f;
         }
     }
     __syncthreads(); // the keys are used
@@ -328,6 +325,15 @@ __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_de
                 for (int j = 0; j < 8; j++) z[j] = (TP)y[j];
                 *(vec<TP, 8> *)((TP *)w.pm + at * SQUARE + (tile * 2 + st) * FRAGMENT + lane * 8) = z;
             }
+        if (wave == 3) {
+            const double c = sums[lane], whole = sums[CHUNK - 1];
+            float *to = w.rows + at * 4 * CHUNK;
+            const bool here = lane < rows;
+            to[lane] = here ? fast_exp2((float)c) * knorm[lane] + spoilt[lane] : 0.0f;
+            to[CHUNK + lane] = here ? fast_exp2((float)c) * qnorm[lane] : 0.0f;
+            to[2 * CHUNK + lane] = here ? fast_exp2((float)(whole - c)) * knorm[lane] : 0.0f;
+            if (lane == 0) to[3 * CHUNK] = fast_exp2((float)whole);
+        }
     }
     __syncthreads();
     f32x4 X[4];
@@ -391,6 +397,7 @@ template <typename T, int DK>
 __global__ void __launch_bounds__(DELTA_CHUNK_THREADS) k_delta_chunks(DeltaArgs a, DeltaWork w) {
     constexpr int NP = parts_of<T>(), NO = out_parts<T>(), STEPS = DK / 32, TILES = DK / 64, SS = DK + 8, TS = 72;
     __shared__ __attribute__((aligned(16))) bhalf_t state[3][16 * SS], right[3][16 * TS], values[NO][16 * TS], update[3][16 * TS];
+    __shared__ uint32_t spoilt[2][16]; // of every other chunk, a column's first token whose right side is not finite
     const uint32_t tid = threadIdx.x, lane = tid % 64, all = __builtin_amdgcn_readfirstlane(tid / 64), wave = all % 4;
     const bool follows = all >= 4; // with the output
     const uint32_t col = lane % 16, quad = lane / 16;
@@ -424,6 +431,7 @@ __global__ void __launch_bounds__(DELTA_CHUNK_THREADS) k_delta_chunks(DeltaArgs 
                 S[m][i] = x;
             }
         publish();
+        if (tid < 16) spoilt[0][tid] = CHUNK;
     }
 
     // Addresses are the wave's plus the lane's share.
@@ -506,7 +514,9 @@ __global__ void __launch_bounds__(DELTA_CHUNK_THREADS) k_delta_chunks(DeltaArgs 
             load_k(next, st);
         }
     };
-    auto right_side = [&](uint32_t next) { // R = V - K S
+    // From a token on that holds what is not finite its columns are NaN, and no token before it is touched: it takes part
+    // as a zero (T is triangular, so it reaches none before), and the outputs from there on and the state are replaced.
+    auto right_side = [&](uint32_t c, uint32_t next) { // R = V - K S
         f32x4 ks[3], r;
         times_state(std::integral_constant<int, 3>{}, next, ks);
 #pragma unroll
@@ -514,10 +524,16 @@ __global__ void __launch_bounds__(DELTA_CHUNK_THREADS) k_delta_chunks(DeltaArgs 
             using U = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
             r[i] = (float)__builtin_bit_cast(T, (U)x.v[i]) - x.of_k[i] * (ks[0][i] + (ks[1][i] + ks[2][i]));
         }
+        uint32_t from = CHUNK;
+#pragma unroll
+        for (int i = 3; i >= 0; i--)
+            if (!(fabsf(r[i]) < INFINITY)) from = token + i, r[i] = 0.0f;
+        if (from < CHUNK) atomicMin(&spoilt[c % 2][col], from);
         split_store<3>(right[0] + mine, 16 * TS, r);
         load_v(next);
     };
-    auto correct = [&](uint32_t next) { // U = T R
+    auto correct = [&](uint32_t c, uint32_t next) { // U = T R
+        if (tid < 16) spoilt[(c + 1) % 2][tid] = CHUNK;
         f32x4 u[3];
         u[0] = u[1] = u[2] = f32x4{0, 0, 0, 0};
 #pragma unroll
@@ -535,7 +551,8 @@ __global__ void __launch_bounds__(DELTA_CHUNK_THREADS) k_delta_chunks(DeltaArgs 
         split_store<NO>(values[0] + mine, 16 * TS, u[0]);
         x.of_u = factors(next, 2);
     };
-    auto renew = [&](uint32_t next) { // the state
+    auto renew = [&](uint32_t c, uint32_t next) { // the state
+        const bool ends = spoilt[c % 2][col] < CHUNK;
         f32x4 add[TILES][3];
 #pragma unroll
         for (int m = 0; m < TILES; m++) {
@@ -557,7 +574,7 @@ __global__ void __launch_bounds__(DELTA_CHUNK_THREADS) k_delta_chunks(DeltaArgs 
             }
         }
 #pragma unroll
-        for (int m = 0; m < TILES; m++) S[m] = add[m][0] + (add[m][1] + add[m][2]);
+        for (int m = 0; m < TILES; m++) S[m] = ends ? f32x4{NAN, NAN, NAN, NAN} : add[m][0] + (add[m][1] + add[m][2]);
         publish();
     };
     f32x4 qs[3];
@@ -580,11 +597,11 @@ __global__ void __launch_bounds__(DELTA_CHUNK_THREADS) k_delta_chunks(DeltaArgs 
             load_p(next, st);
         }
         x.of_q = factors(next, 1);
-        const uint32_t rows = min(n - c * CHUNK, CHUNK);
+        const uint32_t rows = min(n - c * CHUNK, CHUNK), from = spoilt[c % 2][col];
         T *out = (T *)a.out + (uint64_t)(begin + c * CHUNK) * a.out_row + head * a.out_head + dv;
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (token + i < rows) out[out_off[i]] = (T)(o[0][i] + (o[1][i] + o[2][i]));
+            if (token + i < rows) out[out_off[i]] = (T)(token + i < from ? o[0][i] + (o[1][i] + o[2][i]) : NAN);
     };
 
     // Each kind of wave has a loop of its own, of the same three barriers a chunk (a barrier counts the workgroup's waves,
@@ -627,11 +644,11 @@ __global__ void __launch_bounds__(DELTA_CHUNK_THREADS) k_delta_chunks(DeltaArgs 
     barrier();
     for (uint32_t c = 0; c < chunks; c++) {
         const uint32_t next = min(c + 1, chunks - 1);
-        right_side(next);
+        right_side(c, next);
         barrier();
-        correct(next);
+        correct(c, next);
         barrier();
-        renew(next);
+        renew(c, next);
         barrier();
     }
     if (to < 0 || (uint64_t)to >= a.state_slots) return;

@@ -181,3 +181,75 @@ def test_nothing_to_do(device):
     delta.rows(x, x, x, empty(0, 1), empty(0, 1), x, states, ids[:2], ids[2:], empty(3, t=torch.int32))
     torch.cuda.synchronize()
     assert torch.equal(states[:2], before[:2]) and torch.equal(states[2:], before[:2])
+
+
+@pytest.mark.parametrize("what", ["k", "q", "v", "gate", "beta", "state", "zero key"])
+@pytest.mark.parametrize("dtype,dk", [("f32", 64), ("bf16", 128), ("f16", 32)])
+def test_delta_what_is_not_finite_goes_forward_only(device, dtype, dk, what):
+    # Nothing before the token, no other sequence, head or column changes by a bit, in either form.
+    g = np.random.default_rng(21)
+    lens, kh, vh, dv = [150, 90], 2, 4, 32
+    inputs = delta_inputs(g, device, lens, kh, vh, dk, dv, dtype, True, 0.2)
+    starts = torch.tensor([0, 150, 240], dtype=torch.int32, device=device)
+    slots = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=device)
+    h = M.DeviceDelta(240, 2, kh, vh, dk, dv)
+    eps = 0.0 if what == "zero key" else 1e-6
+
+    def run(x, most):
+        q, k, v, gates, beta, states = (y.clone() for y in x)
+        out = torch.empty_like(v)
+        h.rows(q, k, v, gates, beta, out, states, slots[0], slots[1], starts, normalise=True, eps=eps, most_rows=most)
+        torch.cuda.synchronize()
+        return F.as64(out), F.as64(states)[2:4]
+
+    for t, bad in ((70, float("inf")), (131, float("nan")), (149, float("-inf")), (0, float("nan"))):
+        if what == "gate" and bad == float("-inf"):
+            continue  # forgets the state, and is finite
+        spoilt = [x.clone() for x in inputs]
+        q, k, v, gates, beta, states = spoilt
+        if what == "k":
+            k[t, 1, 5] = bad
+        elif what == "q":
+            q[t, 1, 5] = bad
+        elif what == "v":
+            v[t, 2, 3] = bad
+        elif what == "gate":
+            gates[t, 2] = bad
+        elif what == "beta":
+            beta[t, 2] = bad
+        elif what == "state":
+            states[0, 2, 5, 3] = bad
+        else:
+            k[t, 1] = 0.0
+        wants = []
+        with np.errstate(all="ignore"):
+            for s, rows in enumerate((slice(0, 150), slice(150, 240))):
+                x = [F.as64(y)[rows] for y in spoilt[:5]]
+                wants.append(F.delta(*x, F.as64(states)[s], dk ** -0.5, eps))
+        for most in (1, 150):
+            print("delta", what, t, bad, dtype, most, flush=True)
+            clean, clean_state = run(inputs, most)
+            out, state = run(spoilt, most)
+            for s, rows in enumerate((slice(0, 150), slice(150, 240))):
+                odd, odd_state = ~np.isfinite(wants[s][0]), ~np.isfinite(wants[s][1])
+                assert np.array_equal(~np.isfinite(out[rows]), odd)
+                assert np.array_equal(~np.isfinite(state[s]), odd_state)
+                assert np.array_equal(out[rows][~odd], clean[rows][~odd])
+                assert np.array_equal(state[s][~odd_state], clean_state[s][~odd_state])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [1, 17, 40, 64, 70, 129])
+def test_delta_norms_without_epsilon(device, dtype, n):
+    # The oracle's 1e-6 moves a norm of about 8 by a part in 10^8, far inside the bounds.
+    g = np.random.default_rng(22)
+    inputs = delta_inputs(g, device, [n], 1, 2, 64, 32, dtype, True, 0.2)
+    q, k, v, gates, beta, states = inputs
+    before, out = F.as64(states), torch.empty_like(v)
+    h = M.DeviceDelta(n, 1, 1, 2, 64, 32)
+    slots = torch.tensor([0, 1], dtype=torch.int32, device=device)
+    starts = torch.tensor([0, n], dtype=torch.int32, device=device)
+    for most in (1, n):
+        h.rows(q, k, v, gates, beta, out, states, slots[:1], slots[1:], starts, normalise=True, eps=0.0, most_rows=most)
+        torch.cuda.synchronize()
+        delta_check([n], inputs, F.as64(out), before[:1], F.as64(states)[1:2], 64, dtype, True, 64 ** -0.5, n)
