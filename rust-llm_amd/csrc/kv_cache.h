@@ -33,20 +33,29 @@ struct CacheRows {
 
 constexpr uint32_t CACHE_THREADS = 256;
 constexpr uint32_t CACHE_MAX_ROWS = 16; // rows a workgroup, LDS holds their angles
-constexpr int CACHE_AHEAD = 2;          // vectors that a group of lanes has on their way
+// Vectors that a group of lanes has on their way: 20000 rows of 4 heads of 256 take 31.0 us with 1, 29.1 with 2, 29.2
+// with 3, 29.6 with 4; 5003 rows 10.5, 11.1, 11.6, 12.1.
+constexpr int CACHE_AHEAD = 2;
 
-// Turns eight values of a head's key if they are among the turned ones, y their partners where they are eight in a row
-// (half layout of a multiple of 8 pairs; another lane's, read again), else read here.
-template <typename T>
-__device__ inline void turn8(const RotaryArgs &r, const T *in, uint32_t at, const float2 *cs, const vec<T, 8> &y, float (&x)[8]) {
+// Turns the eight values x of a head's key, at on, if they are among the turned ones. raw: as they were read. Their
+// partners in the half layout of a multiple of 8 pairs are another lane's eight, elsewhere read again.
+template <typename T, int G>
+__device__ inline void turn8(const RotaryArgs &r, const T *in, uint32_t at, const float2 *cs, const vec<T, 8> &raw, float (&x)[8]) {
     const uint32_t turned = 2 * r.pairs;
     if (at >= turned) return;
     if (!r.interleaved && r.pairs % 8 == 0) {
         const bool second = at >= r.pairs;
         const uint32_t i = second ? at - r.pairs : at;
+        const vec<uint32_t, 2 * sizeof(T)> mine = __builtin_bit_cast(vec<uint32_t, 2 * sizeof(T)>, raw);
+        vec<uint32_t, 2 * sizeof(T)> theirs;
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            x[j] = second ? turn_b((float)y[j], x[j], cs[i + j]) : turn_a(x[j], (float)y[j], cs[i + j]);
+        for (int j = 0; j < 2 * (int)sizeof(T); j++) theirs[j] = __shfl(mine[j], i / 8 + (second ? 0 : r.pairs / 8), G);
+        const vec<T, 8> y = __builtin_bit_cast(vec<T, 8>, theirs);
+#pragma unroll
+        for (int j = 0; j < 8; j++) { // turn_a or turn_b
+            const float2 w = cs[i + j];
+            x[j] = x[j] * w.x + (float)y[j] * (second ? w.y : -w.y);
+        }
     } else if (r.interleaved && at + 8 <= turned) {
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
@@ -56,15 +65,17 @@ __device__ inline void turn8(const RotaryArgs &r, const T *in, uint32_t at, cons
             x[j + 1] = turn_b(p, q, w);
         }
     } else {
-        for (int j = 0; j < 8 && at + j < turned; j++) {
+        // One value after the other: unrolled, this takes twice the registers of everything else.
+#pragma unroll 1
+        for (uint32_t j = 0; j < 8 && at + j < turned; j++) {
             const uint32_t e = at + j;
-            if (r.interleaved) {
-                const float2 w = cs[e / 2];
-                x[j] = e & 1 ? turn_b((float)in[e - 1], (float)in[e], w) : turn_a((float)in[e], (float)in[e + 1], w);
-            } else if (e < r.pairs)
-                x[j] = turn_a((float)in[e], (float)in[e + r.pairs], cs[e]);
-            else
-                x[j] = turn_b((float)in[e - r.pairs], (float)in[e], cs[e - r.pairs]);
+            const bool second = r.interleaved ? e & 1 : e >= r.pairs;
+            const uint32_t i = r.interleaved ? e / 2 : second ? e - r.pairs : e;
+            const uint32_t other = r.interleaved ? e ^ 1 : second ? i : e + r.pairs;
+            const float2 w = cs[i];
+            const float z = (float)in[e] * w.x + (float)in[other] * (second ? w.y : -w.y);
+#pragma unroll
+            for (uint32_t k = 0; k < 8; k++) x[k] = k == j ? z : x[k];
         }
     }
 }
@@ -73,7 +84,11 @@ __device__ inline void turn8(const RotaryArgs &r, const T *in, uint32_t at, cons
 // rows: keys of every head, then values of every head. One pass: the largest
 // magnitude is reduced over the lanes while the values stay in registers. The
 // first CACHE_AHEAD vectors of a group are loaded before the angles are formed and
-// waited for. Bound by HBM for a prompt, by its chain of loads for a few tokens.
+// waited for. A workgroup is one chain (position, angles, barrier, codes), so what
+// counts is how many share a CU: with partners and the rare layouts at 110
+// registers four did, 5003 rows of 4 heads of 256 bf16 to f8 (31 MB) took 14.6 us;
+// with 55 eight do, 10.9 us (2.8 TB/s). 64 int8 rows of 8 heads of 128: 3.0 us,
+// all chain.
 template <typename T, int FMT, int G>
 __global__ void __launch_bounds__(CACHE_THREADS) k_cache_write(CacheArgs c, CacheRows in, const int64_t *slots,
                                                                uint32_t rows_a_group, RotaryArgs r,
@@ -84,15 +99,12 @@ __global__ void __launch_bounds__(CACHE_THREADS) k_cache_write(CacheArgs c, Cach
     const uint32_t lane = threadIdx.x % G, at = lane * 8, all = n * 2 * c.heads;
     const bool here = at < c.dim, wide = in.wide;
     const uint32_t from = here ? at : 0; // lanes past the head's end load its start
-    // The partners of the lane's values, if they are turned and lie eight in a row.
-    const bool pairs8 = !r.interleaved && r.pairs % 8 == 0 && at < 2 * r.pairs;
-    const uint32_t other = !pairs8 ? from : at >= r.pairs ? at - r.pairs : at + r.pairs;
     struct Item {
         const T *p;
         bool is_value;
         uint32_t rr, head;
         int64_t slot;
-        vec<T, 8> x, y;
+        vec<T, 8> x;
     };
     auto load = [&](uint32_t i, Item &t) { // past the end the last vector again
         i = min(i, all - 1);
@@ -113,23 +125,16 @@ __global__ void __launch_bounds__(CACHE_THREADS) k_cache_write(CacheArgs c, Cach
 #pragma unroll
                 for (int e = 0; e < PER; e++) t.x[j + e] = x[e];
             }
-            if (pairs8 && !t.is_value)
-#pragma unroll
-                for (int j = 0; j < 8; j += PER) {
-                    const vec<T, PER> y = *(const vec<T, PER> *)(t.p + other + j);
-#pragma unroll
-                    for (int e = 0; e < PER; e++) t.y[j + e] = y[e];
-                }
         } else
 #pragma unroll
-            for (int j = 0; j < 8; j++) t.x[j] = t.p[from + j], t.y[j] = t.p[other + j];
+            for (int j = 0; j < 8; j++) t.x[j] = t.p[from + j];
     };
     auto store = [&](const Item &t) {
         if (t.slot < 0 || (uint64_t)t.slot >= c.slots) return;
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) x[j] = here ? (float)t.x[j] : 0.0f;
-        if (here && !t.is_value) turn8(r, t.p, at, cs + t.rr * r.pairs, t.y, x);
+        if (here && !t.is_value) turn8<T, G>(r, t.p, at, cs + t.rr * r.pairs, t.x, x);
         const uint64_t v = cache_vector(c, (uint32_t)t.slot, t.head);
         if constexpr (FMT == RL_F16 || FMT == RL_BF16) {
             using S = std::conditional_t<FMT == RL_F16, half_t, bhalf_t>;
@@ -182,7 +187,7 @@ __global__ void __launch_bounds__(CACHE_THREADS) k_cache_write(CacheArgs c, Cach
     }
 }
 
-// The same mapping the other way.
+// The same mapping the other way: no work but the bytes. The 5003 rows above 6.9 us (4.5 TB/s), 64 int8 rows 2.2 us.
 template <typename T, int FMT, int G>
 __global__ void __launch_bounds__(CACHE_THREADS) k_cache_read(CacheArgs c, CacheRows out, const int64_t *slots) {
     const uint32_t lane = threadIdx.x % G, at = lane * 8;

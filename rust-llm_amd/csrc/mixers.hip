@@ -382,8 +382,12 @@ int rl_kv_cache_write(rl_kv_cache *c, const rl_heads *keys, const rl_heads *valu
         with_format(c->format, [&](auto f) {
             with_group(c->args.dim, [&](auto g) {
                 constexpr int G = decltype(g)::value;
-                // As many rows as give each group of lanes the vectors it loads ahead, while that leaves two workgroups a CU.
-                const uint32_t vectors = CACHE_THREADS / G * (rows >= 2 * CUS * 4 ? CACHE_AHEAD : 1);
+                // As many rows as give each group of lanes the vectors it loads ahead where the workgroups are four a CU or
+                // more with one; with fewer the shorter chain counts (8 heads of 128 to int8, us, ahead / one: 64 rows
+                // 3.7 / 3.0, 512 3.9 / 3.5, 1024 4.4 / 4.4, 2048 5.9 / 6.5, 4096 9.1 / 10.1).
+                constexpr uint32_t GROUPS = CACHE_THREADS / G;
+                const bool many = (uint64_t)rows * 2 * c->args.heads / GROUPS >= 4 * CUS;
+                const uint32_t vectors = GROUPS * (many ? CACHE_AHEAD : 1);
                 const uint32_t per = std::min(std::max(vectors / (2 * c->args.heads), 1u), CACHE_MAX_ROWS);
                 hipLaunchKernelGGL((k_cache_write<decltype(t), decltype(f)::value, G>), dim3((rows + per - 1) / per),
                                    dim3(CACHE_THREADS), 0, static_cast<hipStream_t>(stream), c->args, in, slots, per, r,
