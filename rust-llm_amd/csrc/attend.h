@@ -36,10 +36,13 @@ struct AttendArgs {
     float2 *part_sum;     // [row * q_heads + head][part]: maximum and sum
     uint32_t *part_count; // [row * q_heads + head]: parts written, ATTEND_NONE if the row sees nothing
     uint32_t parts;       // parts a row has room for
+    uint32_t *arrived;    // [row * q_heads + head], of a block's first: its parts that are done; zero between calls
+    uint32_t joins;       // whether the last part's workgroup joins them, else k_attend_join does
 };
 
 constexpr uint32_t ATTEND_THREADS = 256, ATTEND_WAVES = 4, ATTEND_TILE = 32;
-constexpr uint32_t ATTEND_MAX_PARTS = 256, ATTEND_NONE = 1u << 31;
+constexpr uint32_t ATTEND_MAX_PARTS = 256, ATTEND_NONE = 1u << 31, ATTEND_FEW = 16;
+constexpr int ATTEND_STORED = 0x0F70; // s_waitcnt vmcnt(0)
 
 constexpr int attend_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
@@ -94,6 +97,14 @@ __device__ inline uint32_t pair_bf16(uint32_t u) {
                                    (bhalf_t)(float)(int8_t)(u >> (HIGH ? 24 : 8))};
         return __builtin_bit_cast(uint32_t, w);
     }
+}
+
+// Two values that workgroups on other XCDs read, or have written, in this launch.
+__device__ inline void shared_store(float *p, float2 x) {
+    __hip_atomic_store((uint64_t *)p, __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline float2 shared_load(const float *p) {
+    return __builtin_bit_cast(float2, __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
 // Four columns of a finished row: its weighted values over its sum, which holds the
@@ -164,7 +175,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
             const uint64_t row = first + e / G, qh = head * G + e % G;
             ((T *)a.out)[row * a.out_row + qh * a.out_head + d] = (T)NAN;
             if (d == 0 && a.lse) a.lse[row * a.q_heads + qh] = NAN;
-            if (d == 0) a.part_count[row * a.q_heads + qh] = 1; // nothing to join
+            if (d == 0 && !a.joins) a.part_count[row * a.q_heads + qh] = 1; // nothing to join
         }
         return;
     }
@@ -604,12 +615,76 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
             const uint64_t row = first + e / G, qh = head * G + e % G, at = row * a.q_heads + qh;
             const bool none = span.end(e / G) <= span.begin(e / G);
             if (parts == 1) attend_write<T>(a, row, qh, d, none, ms, x, LIFT);
-            else {
+            else if (a.joins) {
+                shared_store(a.part_out + (at * a.parts + part) * HD + d, float2{x[0], x[1]});
+                shared_store(a.part_out + (at * a.parts + part) * HD + d + 2, float2{x[2], x[3]});
+                if (d == 0) shared_store((float *)(a.part_sum + at * a.parts + part), ms);
+            } else {
                 *(f32x4 *)(a.part_out + (at * a.parts + part) * HD + d) = x;
                 if (d == 0) a.part_sum[at * a.parts + part] = ms;
             }
-            if (d == 0 && part == 0) a.part_count[at] = parts | (none ? ATTEND_NONE : 0);
+            if (d == 0 && part == 0 && !a.joins) a.part_count[at] = parts | (none ? ATTEND_NONE : 0);
         }
+    }
+    if (parts == 1 || !a.joins) return;
+    // The last of the block's parts to arrive joins them. Every wave's results are written before the arrival, and both
+    // sides go past the caches that XCDs do not share.
+    __builtin_amdgcn_s_waitcnt(ATTEND_STORED);
+    __syncthreads();
+    uint32_t *last = (uint32_t *)biases;
+    const auto of = [&](uint32_t r) {
+        const uint32_t e = r0 + r;
+        return (uint64_t)(first + e / G) * a.q_heads + head * G + e % G;
+    };
+    if (tid == 0) {
+        uint32_t *arrived = a.arrived + of(0);
+        *last = atomicAdd(arrived, 1u) == parts - 1;
+        if (*last) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // ready for the next call
+    }
+    __syncthreads();
+    if (!*last) return;
+    float *factor = (float *)lds; // [ROWS][ATTEND_FEW]
+    {
+        constexpr uint32_t EACH = ATTEND_FEW / TPR;
+        const uint32_t j = tid % TPR;
+        const float2 *sum_of = a.part_sum + of(q_row < count ? q_row : 0) * a.parts;
+        float2 ms[EACH];
+        float most = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; i++) {
+            const uint32_t p = j + i * TPR;
+            ms[i] = shared_load((const float *)(sum_of + (p < parts ? p : 0)));
+            if (p >= parts) ms[i] = make_float2(-INFINITY, 0.0f);
+            most = fmaxf(most, ms[i].x);
+        }
+        most = group_max<TPR>(most);
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; i++) {
+            const float f = ms[i].x == -INFINITY ? 0.0f : exp2_fast(ms[i].x - most);
+            factor[q_row * ATTEND_FEW + j + i * TPR] = f;
+            sum += ms[i].x == -INFINITY ? ms[i].y : ms[i].y * f; // a part without tokens has 0, or NaN
+        }
+        sum = group_sum<TPR>(sum);
+        if (j == 0) maxima[0][q_row] = most, sums[0][q_row] = sum;
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < count * (HD / 4); i += ATTEND_THREADS) {
+        const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4, e = r0 + r;
+        const float *x = a.part_out + of(r) * a.parts * HD + d;
+        f32x4 all = {0, 0, 0, 0};
+        for (uint32_t p0 = 0; p0 < parts; p0 += 8) {
+            float2 y[8][2];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) {
+                const float *z = x + (p0 + j < parts ? p0 + j : p0) * HD;
+                y[j][0] = shared_load(z), y[j][1] = shared_load(z + 2);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++)
+                if (p0 + j < parts) all += f32x4{y[j][0].x, y[j][0].y, y[j][1].x, y[j][1].y} * factor[r * ATTEND_FEW + p0 + j];
+        }
+        attend_write<T>(a, first + e / G, head * G + e % G, d, span.end(e / G) <= span.begin(e / G),
+                        make_float2(maxima[0][r], sums[0][r]), all, LIFT);
     }
 }
 

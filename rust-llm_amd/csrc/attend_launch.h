@@ -10,7 +10,7 @@ void launch_attend_rows(const AttendArgs &a, uint32_t groups, hipStream_t s) {
         hipLaunchKernelGGL((k_attend<T, FMT, HD, RT, true>), dim3(groups), dim3(ATTEND_THREADS), 0, s, a);
     else
         hipLaunchKernelGGL((k_attend<T, FMT, HD, RT, false>), dim3(groups), dim3(ATTEND_THREADS), 0, s, a);
-    if (a.parts > 1) hipLaunchKernelGGL((k_attend_join<T, FMT, HD>), dim3(a.rows * a.q_heads), dim3(ATTEND_THREADS), 0, s, a);
+    if (a.parts > 1 && !a.joins) hipLaunchKernelGGL((k_attend_join<T, FMT, HD>), dim3(a.rows * a.q_heads), dim3(ATTEND_THREADS), 0, s, a);
 }
 
 template <typename T, int FMT>

@@ -42,11 +42,12 @@ struct rl_attention {
     uint64_t slots = 0; // partial results of a row and head
     float *part_out = nullptr;
     float2 *part_sum = nullptr;
-    uint32_t *part_count = nullptr;
+    uint32_t *part_count = nullptr, *arrived = nullptr;
     ~rl_attention() {
         (void)hipFree(part_out);
         (void)hipFree(part_sum);
         (void)hipFree(part_count);
+        (void)hipFree(arrived);
     }
 };
 
@@ -444,7 +445,9 @@ int rl_attention_create(int device, uint32_t max_rows, uint32_t q_heads, uint32_
     hipError_t e = hipMalloc(&a->part_out, a->slots * attend_dim(dim) * sizeof(float));
     if (e == hipSuccess) e = hipMalloc(&a->part_sum, a->slots * sizeof(float2));
     if (e == hipSuccess) e = hipMalloc(&a->part_count, heads * sizeof(uint32_t));
+    if (e == hipSuccess) e = hipMalloc(&a->arrived, heads * sizeof(uint32_t));
     if (e == hipSuccess) e = hipMemset(a->part_count, 0, heads * sizeof(uint32_t));
+    if (e == hipSuccess) e = hipMemset(a->arrived, 0, heads * sizeof(uint32_t));
     if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e != hipSuccess) {
         delete a;
@@ -496,7 +499,7 @@ int rl_attention_rows(rl_attention *h, const rl_kv_cache *cache, const rl_heads 
     a.scale = scale;
     a.group = h->q_heads / h->kv_heads;
     a.wide = wide(q) && wide(out);
-    a.part_out = h->part_out, a.part_sum = h->part_sum, a.part_count = h->part_count;
+    a.part_out = h->part_out, a.part_sum = h->part_sum, a.part_count = h->part_count, a.arrived = h->arrived;
     // Two row tiles a workgroup where a sequence has more than one: the keys and values are read once for both.
     const uint64_t expanded = (uint64_t)a.most_rows * a.group;
     const bool two = expanded > 16 && attend_two(type_bytes(q->dtype), cache->format, h->dim);
@@ -511,6 +514,7 @@ int rl_attention_rows(rl_attention *h, const rl_kv_cache *cache, const rl_heads 
     a.part_tiles = (uint32_t)((tiles + parts - 1) / parts);
     a.part_tiles = (a.part_tiles + ATTEND_WAVES - 1) / ATTEND_WAVES * ATTEND_WAVES;
     a.parts = (tiles + a.part_tiles - 1) / a.part_tiles;
+    a.joins = a.parts <= ATTEND_FEW;
     // Jobs (sequence, head and part) in eights, the row blocks of each eight together.
     const uint64_t groups = ((uint64_t)seqs * h->kv_heads * a.parts + 7) / 8 * 8 * a.blocks;
     if (groups > 2 * MAX_ROWS - 1) return fail(RL_ERR_CAPACITY, "too many sequences times row blocks in a call");
