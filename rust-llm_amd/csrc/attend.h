@@ -41,24 +41,34 @@ struct AttendArgs {
 };
 
 constexpr uint32_t ATTEND_THREADS = 256, ATTEND_WAVES = 4, ATTEND_TILE = 32;
-constexpr uint32_t ATTEND_MAX_PARTS = 256, ATTEND_NONE = 1u << 31, ATTEND_FEW = 16;
+constexpr uint32_t ATTEND_MAX_PARTS = 256, ATTEND_NONE = 1u << 31;
+// Parts that the last of their workgroups joins, which saves a launch (one sequence of 611 tokens, 5 parts: 11.2 us with
+// it, 10.1 without); more are too much for one CU (21 parts of 16 rows of 256: 31.4 us with the launch, 40.5 without).
+constexpr uint32_t ATTEND_FEW = 16;
 constexpr int ATTEND_STORED = 0x0F70; // s_waitcnt vmcnt(0)
 
 constexpr int attend_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-// Whether a workgroup can take two row tiles: the sums of 32 rows of 256 columns beside a tile of 16-bit keys and values,
-// or with f32 queries, do not fit a wave's registers.
-constexpr bool attend_two(uint32_t query_bytes, uint32_t format, uint32_t dim) {
-    return attend_dim(dim) <= 128 || (query_bytes == 2 && (format == RL_I8 || format == RL_F8));
+// Whether a workgroup takes two row tiles of `count` that a sequence has: keys and values are read once for both, but
+// fewer workgroups share a CU. bf16 queries, us, two / one, sequences x tokens, query / key-value heads x dim:
+//   64:  1 x 20011 tokens, 16/8, 18 rows 15.3 / 17.0, 36 rows 18.3 / 19.7; 32 x 3001 39.7 / 42.0, 52.5 / 58.6
+//   128: a tile left over costs a block's time (32 x 3001, 32/8, 36 rows: bf16 134 / 116, int8 84.0 / 76.3); else int8
+//        20 rows 46.0 / 57.0, 64 rows 88.1 / 102, bf16 85.0 / 91.6, 141 / 145, with columns for half the CUs or fewer
+//        (4 x 8001) bf16 30.4 / 29.2, 59.8 / 48.7
+//   256: the sums take the registers (32 x 3001, 16/4, 32 rows of int8 61.5 / 53.9)
+inline bool attend_two(uint32_t format, uint32_t dim, uint64_t count, uint64_t columns) {
+    if (count < 2 || attend_dim(dim) == 256) return false;
+    if (attend_dim(dim) == 64) return true;
+    return count % 2 == 0 && (format == RL_I8 || format == RL_F8 || columns >= 256);
 }
 
-// Workgroups of k_attend that share a CU, by its registers.
+// Workgroups of k_attend that share a CU: as many as its registers allow without spills.
 constexpr int attend_resident(uint32_t query_bytes, uint32_t format, uint32_t dim, int row_tiles) {
     const bool eight = format == RL_I8 || format == RL_F8;
     switch (attend_dim(dim)) {
     case 64: return row_tiles == 1 ? 3 : 2;
     case 128: return row_tiles == 1 ? (eight && query_bytes == 2 ? 3 : 2) : eight ? 2 : 1;
-    default: return row_tiles == 1 && eight ? 2 : 1;
+    default: return eight ? 2 : 1;
     }
 }
 

@@ -18,10 +18,7 @@ void launch_attend_format(const AttendArgs &a, bool two, uint32_t groups, hipStr
     switch (attend_dim(a.cache.dim)) {
     case 64: return two ? launch_attend_rows<T, FMT, 64, 2>(a, groups, s) : launch_attend_rows<T, FMT, 64, 1>(a, groups, s);
     case 128: return two ? launch_attend_rows<T, FMT, 128, 2>(a, groups, s) : launch_attend_rows<T, FMT, 128, 1>(a, groups, s);
-    default:
-        if constexpr (attend_two(sizeof(T), FMT, 256))
-            if (two) return launch_attend_rows<T, FMT, 256, 2>(a, groups, s);
-        return launch_attend_rows<T, FMT, 256, 1>(a, groups, s);
+    default: return launch_attend_rows<T, FMT, 256, 1>(a, groups, s);
     }
 }
 

@@ -500,9 +500,8 @@ int rl_attention_rows(rl_attention *h, const rl_kv_cache *cache, const rl_heads 
     a.group = h->q_heads / h->kv_heads;
     a.wide = wide(q) && wide(out);
     a.part_out = h->part_out, a.part_sum = h->part_sum, a.part_count = h->part_count, a.arrived = h->arrived;
-    // Two row tiles a workgroup where a sequence has more than one: the keys and values are read once for both.
     const uint64_t expanded = (uint64_t)a.most_rows * a.group;
-    const bool two = expanded > 16 && attend_two(type_bytes(q->dtype), cache->format, h->dim);
+    const bool two = attend_two(cache->format, h->dim, (expanded + 15) / 16, (uint64_t)seqs * h->kv_heads);
     a.blocks = (uint32_t)((expanded + (two ? 31 : 15)) / (two ? 32 : 16));
     const uint64_t columns = (uint64_t)seqs * h->kv_heads * a.blocks;
     const uint64_t seen = window ? std::min<uint64_t>(a.max_len, (uint64_t)window + a.most_rows - 1) : a.max_len;
