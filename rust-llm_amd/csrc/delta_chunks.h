@@ -31,7 +31,7 @@ constexpr uint32_t CHUNK = 64;
 // Operands of the chunks, zeros where a chunk or a head ends early, as fragments: for each of 64 lanes eight values, row
 // lane % 16 of a 16-row tile, columns 8 (lane / 16) on of a step of 32. K and
 // Q too: read where they are, a token's 4 KB or so from the next, all rows of a
-// head come from one channel of the L2 (3.1 us a chunk; 8192 tokens took 464 us).
+// head come from one channel of the L2 (3.1 us a chunk; now 1.9).
 struct DeltaWork {
     void *kt;    // [chunk][key head][DK/16 tiles][2 steps]: K^T in the call's type
     void *kf;    // [chunk][key head][4 tiles][DK/32 steps]: K in the call's type
@@ -149,8 +149,9 @@ __device__ inline void with_flag(bool x, F f) {
 // wave; the inverse of 1 + L goes by 16 x 16 blocks: the four diagonal ones by
 // substitution, a lane a column, the rest column by column of blocks,
 // X_ij = -D_i sum_k L_ik X_kj, in f32 products whose results are the next product's
-// operand where they stand. Bound by its chain of small steps; four workgroups
-// share a CU.
+// operand where they stand. Bound by what it writes and its chain of small steps;
+// four workgroups share a CU. 8192 bf16 tokens of 16 / 32 heads of 128: 70 us, about
+// 260 MB read and written (3.7 TB/s).
 template <typename T, int DK>
 __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_delta_prepare(DeltaArgs a, DeltaWork w) {
     using TP = p_type<T>;
@@ -391,7 +392,10 @@ struct DeltaChunk {
 // parts (three barriers a chunk). Four more waves follow with the output, Q S and
 // P U of the chunk before, in the gaps. Everything else comes from memory, loaded
 // while the chunk before is computed. Bound by the first four's chain: LDS, the
-// products (36 of 16 cycles) and the barriers.
+// products (36 of 16 cycles) and the barriers: 1.9 us a chunk, 240 us for 8192
+// tokens of 32 heads of 128 x 128, where the 256 workgroups have a CU each.
+// Registers for two workgroups a CU spill, and gain only where there are more:
+// 16 sequences of 64 tokens 82.6 -> 70.9 us with them, one of 8192 305 -> 338.
 constexpr uint32_t DELTA_CHUNK_THREADS = 512;
 template <typename T, int DK>
 __global__ void __launch_bounds__(DELTA_CHUNK_THREADS) k_delta_chunks(DeltaArgs a, DeltaWork w) {

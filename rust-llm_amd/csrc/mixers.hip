@@ -165,7 +165,10 @@ int check_cache_rows(const rl_kv_cache *c, const rl_heads *k, const rl_heads *v,
 
 // Parts of a row's length are at most ATTEND_LONG tokens, so that a batch of very
 // different lengths is shared out evenly, and otherwise as many as give each CU
-// the workgroups it holds at a time, each a tile of 32 tokens a wave or more.
+// the workgroups it holds at a time, each a tile of 32 tokens a wave or more. 64
+// int8 sequences of 128 to 8192 tokens: 70.2 us with 768 or 1024, 71.0 with 1536,
+// 71.7 with 2048, 83 with 4096; 1536 joins less where lengths are alike. One
+// sequence of 131071 tokens took 114 us with the limit, 97 without.
 constexpr uint32_t ATTEND_LONG = 1536, CUS = 256;
 
 uint32_t attend_tiles(uint64_t tokens) { return (uint32_t)((tokens + ATTEND_TILE - 1) / ATTEND_TILE) + 1; }
@@ -179,8 +182,8 @@ uint32_t attend_least_parts(uint32_t tiles, uint32_t seqs) {
 
 // Rows of a sequence from which chunks are faster than one token after the other (us, steps / chunks; 32 heads of 128 x
 // 128). While every workgroup of the chunks has a CU to itself they cost the same for any rows up to 64: one bf16
-// sequence of 9 rows 13.7 / 16, of 16 21.6 / 16; f32, more products, 16 rows 18.2 / 22.7, 24 rows 25.7 / 22.7. Beyond
-// that they wait for each other: 16 sequences of 16 rows 54 / 75, of 24 75 / 75.
+// sequence of 9 rows 12.5 / 15.7, of 16 19.3 / 15.7; f32, more products, 16 rows 16.9 / 22.0, 24 rows 23.5 / 22.1. Beyond
+// that they wait for each other: 16 sequences of 16 rows 54.5 / 75.0, of 24 74.8 / 75.2.
 constexpr uint32_t DELTA_CHUNKED = 13, DELTA_CHUNKED_WIDE = 20, DELTA_CHUNKED_MANY = 24;
 
 int launched(const char *what) {
