@@ -19,8 +19,10 @@
 // chunk to chunk: with two it was 9e-6 off f64 at the end of 700 tokens, with three
 // it is as near as f32 arithmetic. Rounded to fewer bits, where the output is
 // bf16: P to one part, the state and the corrected values to two in the products
-// that only the output takes. Decays are differences of f64 sums, so that a token
-// after a strong decay is as exact as one before.
+// that only the output takes (0.0021 off f64 in the mean, 0.0017 of it the output's
+// own rounding; P in two parts, 0.0017, took 8192 tokens from 311 to 333 us).
+// Decays are differences of f64 sums, so that a token after a strong decay is as
+// exact as one before.
 #pragma once
 #include "delta.h"
 
