@@ -2,10 +2,11 @@
 (include/rl_mixers.h): rotary positions, the paged key-value cache, attention of
 new tokens over it, and the gated delta rule.
 
-As in rl_sampler.py this only marshals arguments: tensors are torch tensors on a
-ROCm device, [rows][heads][dim] with the last axis contiguous and any strides
+As in rl_sampler.py this only marshals arguments: tensors are torch tensors on the
+handle's device, [rows][heads][dim] with the last axis contiguous and any strides
 before it, calls go to the current stream unless one is given, and a refusal of
-the library raises rl_sampler.SamplerError.
+the library raises rl_sampler.SamplerError. Every tensor is checked before the
+call: a kernel given an address of the host or of another device would fault.
 """
 import ctypes
 import struct
@@ -63,17 +64,23 @@ def lib():
 _codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-def _stream(t, stream):
-    """The stream given, or the current one of the tensor's device (without the
-    Stream object of torch.cuda.current_stream, which costs 3 us a call)."""
-    device = t.get_device()
-    if device < 0:
-        raise ValueError("the tensors of a call are on a device")
+def _on(t, device):
+    """Refuses a tensor that is not on the handle's device."""
+    if t.get_device() != device:
+        raise ValueError("the tensors of a call are on the handle's device, cuda:%d, not %s" % (device, t.device))
+
+
+def _stream(device, stream):
+    """The stream given, or the device's current one (without the Stream object of
+    torch.cuda.current_stream, which costs 3 us a call)."""
     return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream
 
 
-def _heads(t):
-    """A tensor [rows][heads][dim] as a packed rl_heads."""
+def _heads(t, device=None):
+    """A tensor [rows][heads][dim] as a packed rl_heads; on the device, if one is
+    named."""
+    if device is not None:
+        _on(t, device)
     _, heads, dim = t.shape
     rows, per, one = t.stride()
     if one != 1 or t.dtype not in _codes:
@@ -81,8 +88,9 @@ def _heads(t):
     return _HEADS.pack(t.data_ptr(), rows, per, heads, dim, _codes[t.dtype], 0)
 
 
-def _index(t, dtype, count):
+def _index(t, dtype, count, device):
     """The address of a contiguous index tensor of at least `count` values."""
+    _on(t, device)
     if t.dtype != dtype or not t.is_contiguous() or t.numel() < count:
         raise ValueError("a contiguous %s tensor of %d values" % (dtype, count))
     return t.data_ptr()
@@ -90,6 +98,7 @@ def _index(t, dtype, count):
 
 class _Handle:
     _destroy = None
+    device = 0
 
     def close(self):
         if getattr(self, "h", None):
@@ -115,7 +124,7 @@ class DeviceRotary(_Handle):
                           magnitude)
         h = _vp()
         _check(lib().rl_rotary_create(device, ctypes.byref(spec), ctypes.byref(h)))
-        self.h, self.dims = h, dims
+        self.h, self.dims, self.device = h, dims, device
 
     def frequencies(self):
         """(radians a position of every pair, the magnitude)."""
@@ -126,18 +135,18 @@ class DeviceRotary(_Handle):
     def apply(self, x, positions, out=None, second=None, second_out=None, inverse=False, stream=None):
         """Turns x [rows][heads][dim] by positions [rows] (int64) into `out` (x
         itself if None), and `second` likewise in the same launch."""
-        rows = x.shape[0]
+        rows, device = x.shape[0], self.device
         out = x if out is None else out
-        ins, outs, tensors = _heads(x), _heads(out), 1
+        ins, outs, tensors = _heads(x, device), _heads(out, device), 1
         if out.shape != x.shape:
             raise ValueError("out has another shape")
         if second is not None:
             second_out = second if second_out is None else second_out
             if second.shape[0] != rows or second_out.shape != second.shape:
                 raise ValueError("the second tensor has other rows, or its output another shape")
-            ins, outs, tensors = ins + _heads(second), outs + _heads(second_out), 2
-        _check(lib().rl_rotary_rows(self.h, _index(positions, torch.int64, rows), rows, ins, outs, tensors,
-                                    int(inverse), _stream(x, stream)))
+            ins, outs, tensors = ins + _heads(second, device), outs + _heads(second_out, device), 2
+        _check(lib().rl_rotary_rows(self.h, _index(positions, torch.int64, rows, device), rows, ins, outs, tensors,
+                                    int(inverse), _stream(device, stream)))
 
 
 class DeviceCache(_Handle):
@@ -149,7 +158,7 @@ class DeviceCache(_Handle):
     def __init__(self, pages, page, kv_heads, dim, format="bf16", device=0):
         h = _vp()
         _check(lib().rl_kv_cache_create(device, pages, page, kv_heads, dim, TYPES[format], ctypes.byref(h)))
-        self.h = h
+        self.h, self.device = h, device
         self.pages, self.page, self.kv_heads, self.dim, self.format = pages, page, kv_heads, dim, format
 
     def bytes(self):
@@ -158,20 +167,21 @@ class DeviceCache(_Handle):
     def write(self, keys, values, slots, rotary=None, positions=None, stream=None):
         """Rows keys[i], values[i] to slots[i] (int64; negative: left out), the keys
         turned by positions[i] first if a DeviceRotary is given."""
-        rows = keys.shape[0]
+        rows, device = keys.shape[0], self.device
         if values.shape[0] != rows:
             raise ValueError("keys and values have one row a slot")
-        at = None if rotary is None else _index(positions, torch.int64, rows)
-        _check(lib().rl_kv_cache_write(self.h, _heads(keys), _heads(values), _index(slots, torch.int64, rows), rows,
-                                       None if rotary is None else rotary.h, at, _stream(keys, stream)))
+        at = None if rotary is None else _index(positions, torch.int64, rows, device)
+        _check(lib().rl_kv_cache_write(self.h, _heads(keys, device), _heads(values, device),
+                                       _index(slots, torch.int64, rows, device), rows,
+                                       None if rotary is None else rotary.h, at, _stream(device, stream)))
 
     def read(self, slots, keys, values, stream=None):
         """Into keys[i], values[i] what slots[i] holds (NaN outside the cache)."""
-        rows = keys.shape[0]
+        rows, device = keys.shape[0], self.device
         if values.shape[0] != rows:
             raise ValueError("keys and values have one row a slot")
-        _check(lib().rl_kv_cache_read(self.h, _index(slots, torch.int64, rows), rows, _heads(keys), _heads(values),
-                                      _stream(keys, stream)))
+        _check(lib().rl_kv_cache_read(self.h, _index(slots, torch.int64, rows, device), rows, _heads(keys, device),
+                                      _heads(values, device), _stream(device, stream)))
 
 
 class DeviceAttention(_Handle):
@@ -183,22 +193,22 @@ class DeviceAttention(_Handle):
     def __init__(self, max_rows, q_heads, kv_heads, dim, max_len, device=0):
         h = _vp()
         _check(lib().rl_attention_create(device, max_rows, q_heads, kv_heads, dim, max_len, ctypes.byref(h)))
-        self.h, self.q_heads, self.scale = h, q_heads, dim ** -0.5
+        self.h, self.q_heads, self.scale, self.device = h, q_heads, dim ** -0.5, device
 
     def rows(self, cache, q, out, lens, pages, starts=None, lse=None, scale=None, window=0, most_rows=0, max_len=0,
              stream=None):
         """q, out [rows][q_heads][dim]; lens int32 [seqs]; pages int32
         [seqs][width]; starts int32 [seqs + 1] (None: one row a sequence); lse f32
         [rows][q_heads] if wanted; scale: dim^-1/2 if None."""
-        rows, seqs, width = q.shape[0], pages.shape[0], pages.shape[1]
+        rows, seqs, width, device = q.shape[0], pages.shape[0], pages.shape[1], self.device
         if out.shape != q.shape:
             raise ValueError("out has another shape than q")
         _check(lib().rl_attention_rows(
-            self.h, cache.h, _heads(q), _heads(out),
-            None if lse is None else _index(lse, torch.float32, rows * self.q_heads), rows,
-            None if starts is None else _index(starts, torch.int32, seqs + 1), _index(lens, torch.int32, seqs), seqs,
-            _index(pages, torch.int32, seqs * width), width, self.scale if scale is None else scale, window, most_rows,
-            max_len, _stream(q, stream)))
+            self.h, cache.h, _heads(q, device), _heads(out, device),
+            None if lse is None else _index(lse, torch.float32, rows * self.q_heads, device), rows,
+            None if starts is None else _index(starts, torch.int32, seqs + 1, device),
+            _index(lens, torch.int32, seqs, device), seqs, _index(pages, torch.int32, seqs * width, device), width,
+            self.scale if scale is None else scale, window, most_rows, max_len, _stream(device, stream)))
 
 
 class DeviceDelta(_Handle):
@@ -211,7 +221,7 @@ class DeviceDelta(_Handle):
         h = _vp()
         _check(lib().rl_delta_create(device, max_rows, max_seqs, key_heads, value_heads, key_dim, value_dim,
                                      ctypes.byref(h)))
-        self.h, self.scale = h, key_dim ** -0.5
+        self.h, self.scale, self.device = h, key_dim ** -0.5, device
         self.state = (value_heads, key_dim, value_dim)
 
     def rows(self, q, k, v, g, beta, out, states, slots_in, slots_out, starts=None, scale=None, normalise=False,
@@ -220,17 +230,19 @@ class DeviceDelta(_Handle):
         g, beta f32 [rows][value_heads]; states f32 [slots][value_heads][key_dim]
         [value_dim], contiguous; slots_in, slots_out int32 [seqs]; starts int32
         [seqs + 1] (None: one row a sequence); scale: key_dim^-1/2 if None."""
-        rows, seqs = q.shape[0], slots_in.shape[0]
+        rows, seqs, device = q.shape[0], slots_in.shape[0], self.device
         if k.shape[0] != rows or v.shape[0] != rows or out.shape[0] != rows:
             raise ValueError("q, k, v and out have one row a token")
+        for x in (g, beta, states):
+            _on(x, device)
         for x in (g, beta):
             if x.dtype != torch.float32 or x.shape != (rows, self.state[0]) or x.stride(1) != 1:
                 raise ValueError("g and beta are f32 [rows][value_heads], heads contiguous")
         if states.dtype != torch.float32 or not states.is_contiguous() or states.shape[1:] != self.state:
             raise ValueError("states are contiguous f32 [slots][value_heads][key_dim][value_dim]")
         _check(lib().rl_delta_rows(
-            self.h, _heads(q), _heads(k), _heads(v), _heads(out), g.data_ptr(), g.stride(0), beta.data_ptr(),
-            beta.stride(0), states.data_ptr(), states.shape[0], _index(slots_in, torch.int32, seqs),
-            _index(slots_out, torch.int32, seqs), None if starts is None else _index(starts, torch.int32, seqs + 1),
-            rows, seqs, self.scale if scale is None else scale, eps if normalise else -1.0, most_rows,
-            _stream(q, stream)))
+            self.h, _heads(q, device), _heads(k, device), _heads(v, device), _heads(out, device), g.data_ptr(),
+            g.stride(0), beta.data_ptr(), beta.stride(0), states.data_ptr(), states.shape[0],
+            _index(slots_in, torch.int32, seqs, device), _index(slots_out, torch.int32, seqs, device),
+            None if starts is None else _index(starts, torch.int32, seqs + 1, device), rows, seqs,
+            self.scale if scale is None else scale, eps if normalise else -1.0, most_rows, _stream(device, stream)))
