@@ -236,7 +236,8 @@ class DeviceDelta(_Handle):
         for x in (g, beta, states):
             _on(x, device)
         for x in (g, beta):
-            if x.dtype != torch.float32 or x.shape != (rows, self.state[0]) or x.stride(1) != 1:
+            # One head has no next one: its stride says nothing.
+            if x.dtype != torch.float32 or x.shape != (rows, self.state[0]) or (x.stride(1) != 1 and x.shape[1] > 1):
                 raise ValueError("g and beta are f32 [rows][value_heads], heads contiguous")
         if states.dtype != torch.float32 or not states.is_contiguous() or states.shape[1:] != self.state:
             raise ValueError("states are contiguous f32 [slots][value_heads][key_dim][value_dim]")

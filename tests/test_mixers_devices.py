@@ -1,6 +1,7 @@
-"""The token mixers' binding refuses every tensor that is not on the handle's
-device, before the library is called: a kernel would fault on such an address.
-No GPU: host tensors that say where they are take the place of the device's."""
+"""What the token mixers' binding accepts and refuses before the library is called:
+every tensor has to be on the handle's device (a kernel would fault on another
+address), and only strides that are used are looked at. No GPU: host tensors that
+say where they are take the place of the device's."""
 import ctypes
 
 import pytest
@@ -82,3 +83,17 @@ def test_every_tensor_has_to_be_on_the_handles_device(no_library, call):
             with pytest.raises(ValueError, match="device"):
                 f(**dict(tensors, **{name: other}))
                 pytest.fail("%s passed" % name)
+
+
+def test_gates_of_one_head_have_any_head_stride(no_library):
+    delta = handle(M.DeviceDelta, scale=1.0, state=(1, 16, 16))
+    x, slots, starts = tensor(3, 1, 16), tensor(2, t=torch.int32), tensor(3, t=torch.int32)
+    call = lambda g, beta: delta.rows(x, x, x, g, beta, x, tensor(4, 1, 16, 16), slots, slots, starts)  # noqa: E731
+    turned = tensor(1, 3).t()  # [3][1] with strides (1, 3): a row a token, as the library reads it
+    assert turned.stride() == (1, 3)
+    with pytest.raises(Reached):
+        call(turned, turned)
+    delta.state = (2, 16, 16)
+    x = tensor(3, 2, 16)
+    with pytest.raises(ValueError, match="contiguous"):
+        call(tensor(2, 3).t(), tensor(3, 2))
