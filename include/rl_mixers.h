@@ -141,8 +141,8 @@ void rl_attention_destroy(rl_attention *attention);
 /* q and out: [rows][q_heads][dim] of one type; a cache in RL_F16 takes f16 or f32
  * queries, one in RL_BF16 bf16 or f32, the 8-bit ones all three. starts i32
  * [seqs + 1] rising from 0 to rows, or NULL for one row a sequence (rows == seqs);
- * lens i32 [seqs]; pages i32 [seqs][table_width]; lse f32 [rows][q_heads] or
- * NULL. most_rows and max_len bound the rows and tokens of any one sequence
+ * lens i32 [seqs], a negative one as 0; pages i32 [seqs][table_width]; lse f32
+ * [rows][q_heads] or NULL. most_rows and max_len bound the rows and tokens of any one sequence
  * (0: as many as the call has rows, and the handle's max_len); a sequence past
  * either bound, or one that needs a page outside its table or the cache, gives
  * NaN. Only entries of `pages` that hold tokens in sight are read. */

@@ -87,7 +87,8 @@ __device__ inline f32x4 mfma(vec<bhalf_t, 8> a, vec<bhalf_t, 8> b, f32x4 c) {
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The sequence's rows, and what a row sees: [begin, end).
+// The sequence's rows, and what a row sees: [begin, end). len is 0 or more and n at most 2^23, so no sum here leaves 32
+// bits; tokens past a tile's or a block's end are counted unsigned, since len may be the largest.
 struct AttendSpan {
     int32_t len, n, window;
     __device__ int32_t end(int32_t i) const { return max(len - n + i + 1, 0); }
@@ -174,8 +175,9 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     typedef const __attribute__((address_space(4))) int32_t constant_i32;
     const constant_i32 *starts = (constant_i32 *)(uintptr_t)a.starts, *lens = (constant_i32 *)(uintptr_t)a.lens;
     const int32_t first = starts ? starts[s] : (int32_t)s;
-    AttendSpan span{lens[s], starts ? starts[s + 1] - first : 1, (int32_t)a.window};
-    if (span.n <= 0 || first < 0 || (uint32_t)first + span.n > a.rows) return; // no rows, or `starts` is not what it should be
+    const int64_t rows = starts ? (int64_t)starts[s + 1] - first : 1;
+    if (rows <= 0 || first < 0 || first + rows > a.rows) return; // no rows, or `starts` is not what it should be
+    AttendSpan span{max(lens[s], 0), (int32_t)rows, (int32_t)a.window}; // a negative length is none
     const uint32_t expanded = (uint32_t)span.n * G;
     const int32_t longest = span.end(span.n - 1);
     const uint32_t page = a.cache.page;
@@ -199,7 +201,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     const int32_t i0 = r0 / G, i1 = (r0 + count - 1) / G; // query rows of the block
     const int32_t begin_min = span.begin(i0), begin_max = span.begin(i1), end_min = span.end(i0), end_max = span.end(i1);
     const bool mixed = begin_min != begin_max || end_min != end_max;
-    const int32_t tile0 = begin_min / (int)ATTEND_TILE, tiles = (end_max + (int)ATTEND_TILE - 1) / (int)ATTEND_TILE - tile0;
+    const int32_t tile0 = begin_min / (int)ATTEND_TILE, tiles = (int32_t)((end_max + ATTEND_TILE - 1) / ATTEND_TILE) - tile0;
     const uint32_t parts = tiles > 0 ? (tiles + a.part_tiles - 1) / a.part_tiles : 1; // of this block
     if (part >= parts) return;
 
@@ -363,7 +365,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
         // In the order of the loop's own loads: a wait in the loop has to hold for the first tile too.
         const int32_t t0 = tile * (int)ATTEND_TILE;
         const Pages now = fetch(t0);
-        ahead = fetch(t0 + (int)(ATTEND_WAVES * ATTEND_TILE));
+        ahead = fetch((int32_t)(t0 + ATTEND_WAVES * ATTEND_TILE)); // may be past the last token, and past 2^31: any in sight
         const Place at = place(t0, now);
         __builtin_amdgcn_sched_barrier(0);
         load_keys(at);
@@ -474,13 +476,13 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
         if constexpr (MORE) {
             const int32_t t1 = t0 + (int)(ATTEND_WAVES * ATTEND_TILE);
             next = place(t1, ahead);
-            ahead = fetch(t1 + (int)(ATTEND_WAVES * ATTEND_TILE));
+            ahead = fetch((int32_t)(t1 + ATTEND_WAVES * ATTEND_TILE));
             __builtin_amdgcn_sched_barrier(0);
             load_keys(next);
             __builtin_amdgcn_sched_barrier(0);
         }
         // A tile that some row of the block does not see all of.
-        const bool edge = t0 < begin_max || t0 + (int)ATTEND_TILE > end_min;
+        const bool edge = t0 < begin_max || end_min - t0 < (int)ATTEND_TILE;
         vec<MV, 8> w[RT][PP];
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
