@@ -96,7 +96,9 @@ struct AttendSpan {
 };
 
 // Two 8-bit codes, the low or high half of u, as two 16-bit values. Keys: int8 codes lie in the cache with their sign
-// bit flipped, and 0x6400 | b is 1024 + b in f16, so each reads as the code and 1152, exactly.
+// bit flipped, and 0x6400 | b is 1024 + b in f16, so each reads as the code and 1152, exactly. The 1152 comes off each key
+// before its product, again exactly: taken off the finished score as 1152 sum q it costs a score what f32 sums of numbers
+// a hundred times the codes lose, 2e-4 for queries of mean 0 and 1e-2 for a mean of 8 (256 dims).
 constexpr float KEY_BIAS = 1152.0f;
 template <int FMT, bool HIGH>
 __device__ inline uint32_t pair_f16(uint32_t u) {
@@ -155,14 +157,12 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     constexpr int VW = VD * SIZE / 4;         // dwords of a value that a lane holds
     constexpr int STEPS = HD / 32;            // products a score tile
     constexpr float LIFT = FMT == RL_F16 ? ATTEND_LIFT : 0.0f; // weights up to 2^8: their second f16 parts stay normal
-    // int8 keys with their bias: q (c + 1152) - 1152 sum q, where f32's 24 bits leave 16-bit queries' scores exact enough
-    // (4e-6 off at most); f32 queries take the bias off every key.
-    constexpr bool BIASED = FMT == RL_I8 && !F32Q;
     constexpr bool Q_REGS = RT * QP * STEPS <= 4;
     constexpr int QS = HD + 8;
     constexpr size_t Q_BYTES = (size_t)QP * ROWS * QS * 2, O_BYTES = (size_t)ATTEND_WAVES * 16 * (HD + 4) * 4;
     __shared__ __attribute__((aligned(16))) uint8_t lds[Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES];
-    __shared__ float mults[ROWS], biases[ROWS], maxima[ATTEND_WAVES][ROWS], sums[ATTEND_WAVES][ROWS];
+    __shared__ float mults[ROWS], maxima[ATTEND_WAVES][ROWS], sums[ATTEND_WAVES][ROWS];
+    __shared__ bool last;
 
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     // The row blocks of one sequence, head and part are eight workgroups apart: on one XCD, so that its L2 has the keys
@@ -390,20 +390,14 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
 #pragma unroll
             for (uint32_t j = 0; j < EPT; j++) x[j] *= down;
         }
-        float sum = 0.0f;
 #pragma unroll
         for (int p = 0; p < QP; p++)
 #pragma unroll
             for (uint32_t j = 0; j < EPT; j++) {
                 const MK y = (MK)x[j];
                 qs[(p * ROWS + q_row) * QS + q_at + j] = y;
-                if (BIASED) sum += (float)y;
                 x[j] -= (float)y;
             }
-        if (BIASED) {
-            sum = group_sum<TPR>(sum);
-            if (tid % TPR == 0) biases[q_row] = KEY_BIAS * sum;
-        }
         if (tid % TPR == 0) mults[q_row] = a.scale * 1.44269504088896341f * unit;
     }
     __syncthreads();
@@ -423,13 +417,12 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
 #pragma unroll
                 for (int st = 0; st < STEPS; st++) qf[rt][p][st] = q_fragment(rt, p, st);
     }
-    float mult[RT], bias[RT];
+    float mult[RT];
     int32_t row_begin[RT], row_end[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         const uint32_t r = rt * 16 + col;
         mult[rt] = mults[r];
-        bias[rt] = BIASED ? biases[r] : 0.0f;
         const int32_t i = r < count ? (r0 + r) / G : 0;
         row_begin[rt] = r < count ? span.begin(i) : begin_min; // rows past the block's see what any of it sees
         row_end[rt] = r < count ? span.end(i) : end_max;
@@ -453,7 +446,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
                     const uint32_t x = kr[u][st / 2][st % 2 * 2], y = kr[u][st / 2][st % 2 * 2 + 1];
                     const u32x4 w = {pair_f16<FMT, false>(x), pair_f16<FMT, true>(x), pair_f16<FMT, false>(y), pair_f16<FMT, true>(y)};
                     k[u] = __builtin_bit_cast(vec<MK, 8>, w);
-                    if constexpr (FMT == RL_I8 && !BIASED) k[u] -= (MK)KEY_BIAS;
+                    if constexpr (FMT == RL_I8) k[u] -= (MK)KEY_BIAS;
                 } else {
                     k[u] = __builtin_bit_cast(vec<MK, 8>, kr[u][st]);
                     // Queries are zeros past the head's end; 16-bit keys may hold what a zero does not cancel.
@@ -489,7 +482,6 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
             float x[8], most = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                if constexpr (BIASED) S[rt][j / 4][j % 4] -= bias[rt];
                 if constexpr (EIGHT) x[j] = S[rt][j / 4][j % 4] * (step[j / 4][j % 4] * mult[rt]);
                 else x[j] = S[rt][j / 4][j % 4] * mult[rt];
                 if (edge) {
@@ -647,18 +639,17 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     // sides go past the caches that XCDs do not share.
     __builtin_amdgcn_s_waitcnt(ATTEND_STORED);
     __syncthreads();
-    uint32_t *last = (uint32_t *)biases;
     const auto of = [&](uint32_t r) {
         const uint32_t e = r0 + r;
         return (uint64_t)(first + e / G) * a.q_heads + head * G + e % G;
     };
     if (tid == 0) {
         uint32_t *arrived = a.arrived + of(0);
-        *last = atomicAdd(arrived, 1u) == parts - 1;
-        if (*last) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // ready for the next call
+        last = atomicAdd(arrived, 1u) == parts - 1;
+        if (last) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // ready for the next call
     }
     __syncthreads();
-    if (!*last) return;
+    if (!last) return;
     float *factor = (float *)lds; // [ROWS][ATTEND_FEW]
     {
         constexpr uint32_t EACH = ATTEND_FEW / TPR;
