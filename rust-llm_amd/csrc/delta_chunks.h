@@ -17,10 +17,10 @@
 // of split operands leave out what lies below 2^-24 of them (lo lo, mid lo). Two
 // parts would do for 16-bit outputs, but the state is an f32 result that goes from
 // chunk to chunk: with two it was 9e-6 off f64 at the end of 700 tokens, with three
-// it is as near as f32 arithmetic. Rounded to fewer bits, where the output is
-// bf16: P to one part, the state and the corrected values to two in the products
-// that only the output takes (0.0021 off f64 in the mean, 0.0017 of it the output's
-// own rounding; P in two parts, 0.0017, took 8192 tokens from 311 to 333 us).
+// it is as near as f32 arithmetic. Where the output is bf16, what only the output
+// takes (P, and there the state and the corrected values) has two parts, 16 bits:
+// they add less than a thousandth to the error of its rounding. With P in one part
+// that error was 1.38 times as large, and 8192 tokens took 288 us instead of 305.
 // Decays are differences of f64 sums, so that a token after a strong decay is as
 // exact as one before.
 #pragma once
@@ -39,17 +39,36 @@ struct DeltaWork {
     void *kf;    // [chunk][key head][4 tiles][DK/32 steps]: K in the call's type
     void *qf;    // the same of Q
     bhalf_t *tm; // [chunk][value head][4 tiles][2 steps][3 parts]: T
-    void *pm;    // [chunk][value head][4 tiles][2 steps]: P, bf16 for bf16 calls, else f32
+    void *pm;    // [chunk][value head][4 tiles][2 steps]: P, two bf16 parts for bf16 calls, else f32
     float *rows; // [chunk][value head][4][64]: factors of the rows of K S, of Q S and of U in the state; [3][0] e^c_n
 };
 
-// Parts of a value of the call's type, of P, and of the state and corrected values where only the output takes them.
+// Parts of a value of the call's type, and of P, the state and the corrected values where only the output takes them.
 template <typename T>
 constexpr int parts_of() { return std::is_same_v<T, bhalf_t> ? 1 : std::is_same_v<T, half_t> ? 2 : 3; }
 template <typename T>
 constexpr int out_parts() { return std::is_same_v<T, bhalf_t> ? 2 : 3; }
+
+// P as it is kept for a product: bf16 calls split it once, when it is formed.
 template <typename T>
-using p_type = std::conditional_t<std::is_same_v<T, bhalf_t>, bhalf_t, float>;
+struct DeltaP {
+    vec<float, 8> x;
+    __device__ void load(const void *pm, uint64_t fragment, uint32_t lane) {
+        x = ((const vec<float, 8> *)pm)[fragment * 64 + lane];
+    }
+    static __device__ void store(void *pm, uint64_t fragment, uint32_t lane, const vec<float, 8> &y) {
+        ((vec<float, 8> *)pm)[fragment * 64 + lane] = y;
+    }
+};
+template <>
+struct DeltaP<bhalf_t> {
+    vec<bhalf_t, 8> x[2];
+    __device__ void load(const void *pm, uint64_t fragment, uint32_t lane) {
+#pragma unroll
+        for (int p = 0; p < 2; p++) x[p] = ((const vec<bhalf_t, 8> *)pm)[(fragment * 2 + p) * 64 + lane];
+    }
+    static __device__ void store(void *pm, uint64_t fragment, uint32_t lane, const vec<float, 8> &y);
+};
 
 constexpr int delta_dim(uint32_t key_dim) { return key_dim <= 64 ? 64 : key_dim <= 128 ? 128 : 256; }
 
@@ -64,15 +83,15 @@ typedef vec<bhalf_t, 4> bf16x4;
 
 __device__ inline f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-// acc += x y for operands in parts, without the products of parts that lie three or more steps down. Sums of equal size
+// acc += x y for operands in parts, without the products of parts that lie LEVELS or more steps down. Sums of equal size
 // go to one accumulator each, so that no chain is longer than it has to be; the caller adds them.
-template <int NX, int NY, int NA>
+template <int LEVELS = 3, int NX, int NY, int NA>
 __device__ inline void mma_parts(const bf16x8 (&x)[NX], const bf16x8 (&y)[NY], f32x4 (&acc)[NA]) {
 #pragma unroll
     for (int i = 0; i < NX; i++)
 #pragma unroll
         for (int j = 0; j < NY; j++)
-            if (i + j < 3) acc[i + j < NA ? i + j : NA - 1] = mma(x[i], y[j], acc[i + j < NA ? i + j : NA - 1]);
+            if (i + j < LEVELS) acc[i + j < NA ? i + j : NA - 1] = mma(x[i], y[j], acc[i + j < NA ? i + j : NA - 1]);
 }
 
 __device__ inline float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -108,6 +127,13 @@ __device__ inline void split8(const vec<T, 8> &x, bf16x8 (&part)[NP]) {
                 if (p + 1 < NP) y -= (float)part[p][j];
             }
         }
+}
+
+__device__ inline void DeltaP<bhalf_t>::store(void *pm, uint64_t fragment, uint32_t lane, const vec<float, 8> &y) {
+    bf16x8 part[2];
+    split8(y, part);
+#pragma unroll
+    for (int p = 0; p < 2; p++) ((bf16x8 *)pm)[(fragment * 2 + p) * 64 + lane] = part[p];
 }
 
 // Four consecutive f32 values into the rows of their parts, `apart` values from part to part. All parts but the last are
@@ -156,7 +182,6 @@ __device__ inline void with_flag(bool x, F f) {
 // 260 MB read and written (3.7 TB/s).
 template <typename T, int DK>
 __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_delta_prepare(DeltaArgs a, DeltaWork w) {
-    using TP = p_type<T>;
     constexpr int NP = parts_of<T>(), STEPS = DK / 32, LS = 68, KS = DK + 16 / (int)sizeof(T);
     constexpr size_t K_BYTES = (size_t)CHUNK * KS * sizeof(T), L_BYTES = CHUNK * LS * 4;
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * L_BYTES > K_BYTES ? 2 * L_BYTES : K_BYTES];
@@ -322,11 +347,7 @@ __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_de
 #pragma unroll
             for (int st = 0; st < 2; st++) {
                 if (st * 32 > tile * 16 || (tile ? tile : 1) != (int)wave) continue; // tiles 0 and 1 are the first wave's
-                const vec<float, 8> y = eight(tile, st);
-                vec<TP, 8> z;
-#pragma unroll
-                for (int j = 0; j < 8; j++) z[j] = (TP)y[j];
-                *(vec<TP, 8> *)((TP *)w.pm + at * SQUARE + (tile * 2 + st) * FRAGMENT + lane * 8) = z;
+                DeltaP<T>::store(w.pm, at * 8 + tile * 2 + st, lane, eight(tile, st));
             }
         if (wave == 3) {
             const double c = sums[lane], whole = sums[CHUNK - 1];
@@ -382,7 +403,7 @@ template <typename T, int DK>
 struct DeltaChunk {
     vec<T, 8> k[DK / 32], kt[DK / 64][2]; // k: Q for the output's waves
     bf16x8 t[2][3];
-    vec<p_type<T>, 8> p[2];
+    DeltaP<T> p[2];
     f32x4 of_k, of_q, of_u;
     float keep;
     uint32_t v[4]; // a value a register
@@ -391,9 +412,10 @@ struct DeltaChunk {
 // A workgroup has 16 columns of one head's state. Four waves carry the state, wave
 // w the rows DK/4 w on, and of a chunk's tokens the 16 w on: K S, the corrected
 // values and the new state, which pass between them through LDS as operands in
-// parts (three barriers a chunk). Four more waves follow with the output, Q S and
-// P U of the chunk before, in the gaps. Everything else comes from memory, loaded
-// while the chunk before is computed. Bound by the first four's chain: LDS, the
+// parts (three barriers a chunk). Four more waves follow with the output: Q S beside
+// U, P U beside the new state, their stores beside the next chunk's K S (P U there
+// too took 8192 tokens 317 us instead of 305). Everything else comes from memory,
+// loaded while the chunk before is computed. Bound by the first four's chain: LDS, the
 // products (36 of 16 cycles) and the barriers: 1.9 us a chunk, 240 us for 8192
 // tokens of 32 heads of 128 x 128, where the 256 workgroups have a CU each.
 // Registers for two workgroups a CU spill, and gain only where there are more:
@@ -488,7 +510,7 @@ __global__ void __launch_bounds__(DELTA_CHUNK_THREADS) k_delta_chunks(DeltaArgs 
             x.t[st][p] = fragment(w.tm + (head_at(c) * 8 + wave * 2 + (st ? second : 0)) * 3 * FRAGMENT + p * FRAGMENT);
     };
     auto load_p = [&](uint32_t c, int st) {
-        x.p[st] = fragment((const p_type<T> *)w.pm + head_at(c) * SQUARE + (wave * 2 + (st ? second : 0)) * FRAGMENT);
+        x.p[st].load(w.pm, head_at(c) * 8 + wave * 2 + (st ? second : 0), lane);
     };
     auto load_kt = [&](uint32_t c, int m, int st) {
         x.kt[m][st] = fragment((const T *)w.kt + key_at(c) + ((wave * TILES + m) * 2 + st) * FRAGMENT);
@@ -587,22 +609,27 @@ __global__ void __launch_bounds__(DELTA_CHUNK_THREADS) k_delta_chunks(DeltaArgs 
     uint64_t out_off[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) out_off[i] = (uint64_t)(token + i) * a.out_row;
+    f32x4 o[3];
     auto output = [&](uint32_t c, uint32_t next) { // out = Q S + P U of a chunk whose Q S stands in qs
-        f32x4 o[3];
         o[0] = (qs[0] + (qs[1] + qs[2])) * x.of_q, o[1] = o[2] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int st = 0; st < 2; st++) {
             if (st <= (int)second) {
-                constexpr int PP = std::is_same_v<T, bhalf_t> ? 1 : 3;
-                bf16x8 b[NO], p[PP];
+                bf16x8 b[NO];
 #pragma unroll
                 for (int i = 0; i < NO; i++) b[i] = *(const bf16x8 *)(values[i] + col * TS + st * 32 + quad * 8);
-                split8(x.p[st], p);
-                mma_parts(p, b, o);
+                if constexpr (std::is_same_v<T, bhalf_t>) mma_parts<2>(x.p[st].x, b, o);
+                else {
+                    bf16x8 p[3];
+                    split8(x.p[st].x, p);
+                    mma_parts(p, b, o);
+                }
             }
             load_p(next, st);
         }
         x.of_q = factors(next, 1);
+    };
+    auto write = [&](uint32_t c) { // behind the next barrier, where these waves have nothing else to do
         const uint32_t rows = min(n - c * CHUNK, CHUNK), from = spoilt[c % 2][col];
         T *out = (T *)a.out + (uint64_t)(begin + c * CHUNK) * a.out_row + head * a.out_head + dv;
 #pragma unroll
@@ -623,13 +650,14 @@ __global__ void __launch_bounds__(DELTA_CHUNK_THREADS) k_delta_chunks(DeltaArgs 
         }
         barrier();
         for (uint32_t c = 0; c < chunks; c++) {
-            if (c) output(c - 1, c); // its U stands until the next barrier
+            if (c) write(c - 1); // its first bad tokens stand until the next barrier
             barrier();
             times_state(std::integral_constant<int, NO>{}, min(c + 1, chunks - 1), qs); // before this chunk, until the next
             barrier();
+            output(c, min(c + 1, chunks - 1));
             barrier();
         }
-        if (chunks > 0) output(chunks - 1, chunks - 1);
+        if (chunks > 0) write(chunks - 1);
         return;
     }
     if (chunks > 0) {
