@@ -15,7 +15,9 @@ inline int fail(int code, const std::string &msg) {
     return code;
 }
 
+// The runtime keeps a failed call's error until it is asked for: reported here, it must not be the next launch's too.
 inline int hip_fail(hipError_t e, const char *what) {
+    (void)hipGetLastError();
     return fail(RL_ERR_DEVICE, std::string(what) + ": " + hipGetErrorString(e));
 }
 
@@ -26,6 +28,7 @@ struct DeviceGuard {
     explicit DeviceGuard(int dev) {
         if (hipGetDevice(&prev) != hipSuccess) prev = -1;
         if (prev != dev) ok = hipSetDevice(dev) == hipSuccess;
+        if (!ok) (void)hipGetLastError(); // as in hip_fail: the caller reports it
     }
     ~DeviceGuard() {
         int cur = -1;
