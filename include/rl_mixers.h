@@ -104,8 +104,10 @@ void rl_kv_cache_destroy(rl_kv_cache *cache);
 uint64_t rl_kv_cache_bytes(const rl_kv_cache *cache);
 
 /* Writes rows keys[i], values[i] to slots[i] (i64 [rows] on the device). A slot
- * that is negative or past the cache is left out, so a batch may hold padding;
- * of rows with the same slot any one may stay. With `rotary` the keys are turned
+ * that is negative or past the cache is left out, so a batch may hold padding. The
+ * others are to be distinct: rows are written side by side, so a slot that a call
+ * gives twice holds a mixture of the rows' keys, values, codes and steps until it is
+ * written again (no other slot is touched by it). With `rotary` the keys are turned
  * by positions[i] first (in f32, before the one rounding); NULL stores them as
  * they are and reads no positions. keys and values have one type and shape. */
 int rl_kv_cache_write(rl_kv_cache *cache, const rl_heads *keys, const rl_heads *values, const int64_t *slots,

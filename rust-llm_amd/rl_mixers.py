@@ -165,8 +165,8 @@ class DeviceCache(_Handle):
         return lib().rl_kv_cache_bytes(self.h)
 
     def write(self, keys, values, slots, rotary=None, positions=None, stream=None):
-        """Rows keys[i], values[i] to slots[i] (int64; negative: left out), the keys
-        turned by positions[i] first if a DeviceRotary is given."""
+        """Rows keys[i], values[i] to slots[i] (int64; negative: left out, the others
+        distinct), the keys turned by positions[i] first if a DeviceRotary is given."""
         rows, device = keys.shape[0], self.device
         if values.shape[0] != rows:
             raise ValueError("keys and values have one row a slot")
