@@ -129,8 +129,9 @@ int rl_kv_cache_read(rl_kv_cache *cache, const int64_t *slots, uint32_t rows, co
  * nothing gives zeros and an lse of -inf. Scores, softmax and sums are f32; the
  * weights go into the product with the values as sums of 16-bit parts, good to 16
  * bits or more for 16-bit queries and to 22 or more for f32 ones. What a
- * row does not see does not reach it, whatever it holds; an infinity among the f16
- * or bf16 values that only some rows of a sequence see may be NaN to those. */
+ * row does not see does not reach it, whatever it holds. An infinity among the f16 or
+ * bf16 values that a row sees may read as NaN (a part of its weight may be 0), and so
+ * may one among such keys to f32 queries. */
 typedef struct rl_attention rl_attention;
 
 /* Workspace for calls of up to max_rows query rows over caches of kv_heads heads
