@@ -163,11 +163,12 @@ int rl_attention_rows(rl_attention *attention, const rl_kv_cache *cache, const r
  * sums are f32. */
 typedef struct rl_delta rl_delta;
 
-/* Workspace for calls of up to max_rows tokens in up to max_seqs sequences (none is
- * needed below 13 rows; else about 64 KB a value head for every 64 rows, and
- * for every sequence that has 16 rows or more to itself on average). value_heads:
- * a multiple of key_heads. key_dim, value_dim: 16 to 256, multiples
- * of 16. */
+/* Workspace for calls of up to max_rows tokens in up to max_seqs sequences: none below
+ * 13 rows, else for max_rows / 64 + min(max_seqs, max_rows / 16 + 1) chunks, each of
+ * 41 KiB a value head and 768 D bytes a key head (D: key_dim rounded up to 64, 128 or
+ * 256). A call of more sequences than its chunks have room for goes token by token.
+ * value_heads: a multiple of key_heads. key_dim, value_dim: 16 to 256, multiples of
+ * 16. */
 int rl_delta_create(int device, uint32_t max_rows, uint32_t max_seqs, uint32_t key_heads, uint32_t value_heads,
                     uint32_t key_dim, uint32_t value_dim, rl_delta **out);
 void rl_delta_destroy(rl_delta *delta);
@@ -181,10 +182,11 @@ void rl_delta_destroy(rl_delta *delta);
  * may be equal; else no slot that a sequence of the call reads may be one that
  * another writes. A slot from state_slots on reads as NaN and is not written. A
  * sequence without rows passes its state on. most_rows bounds the rows of any one
- * sequence (0: as many as the call has); it picks the form that is used (one
- * token after the other, or chunks on the matrix cores) and no result depends on
- * its being exact. What is not finite reaches the tokens after it, none before;
- * where chunks are used an infinity reads as NaN. */
+ * sequence (0: as many as the call has); it may be any number, since it only picks
+ * the form that is used for all of them, one token after the other or chunks on the
+ * matrix cores. Both are as exact as f32 sums, but do not give the same bits, and in
+ * chunks an infinity reads as NaN. What is not finite reaches the tokens after it,
+ * none before. */
 int rl_delta_rows(rl_delta *delta, const rl_heads *q, const rl_heads *k, const rl_heads *v, const rl_heads *out,
                   const float *g, uint64_t g_stride, const float *beta, uint64_t beta_stride, float *states,
                   uint64_t state_slots, const int32_t *slots_in, const int32_t *slots_out, const int32_t *starts,
