@@ -135,8 +135,10 @@ int rl_kv_cache_read(rl_kv_cache *cache, const int64_t *slots, uint32_t rows, co
 typedef struct rl_attention rl_attention;
 
 /* Workspace for calls of up to max_rows query rows over caches of kv_heads heads
- * and up to max_len tokens a sequence. q_heads: a multiple of kv_heads;
- * max_rows * q_heads at most 2^23. */
+ * and up to max_len tokens a sequence: 8 bytes a row and head, and 4 D + 8 bytes for
+ * each partial result (D: dim rounded up to 64, 128 or 256), of which there are about
+ * max_rows * q_heads * min(max_len / 1536 + 1, 256), at most 2^20, at least 24576.
+ * q_heads: a multiple of kv_heads; max_rows * q_heads at most 2^23. */
 int rl_attention_create(int device, uint32_t max_rows, uint32_t q_heads, uint32_t kv_heads, uint32_t dim,
                         uint32_t max_len, rl_attention **out);
 void rl_attention_destroy(rl_attention *attention);

@@ -173,6 +173,11 @@ constexpr uint32_t ATTEND_LONG = 1536, CUS = 256;
 
 uint32_t attend_tiles(uint64_t tokens) { return (uint32_t)((tokens + ATTEND_TILE - 1) / ATTEND_TILE) + 1; }
 
+// Partial results that a handle has room for at most, 0.5 GB of them for heads of 128. Calls of more rows times heads than
+// this holds parts for have row blocks enough to fill the device. Without a limit 8192 rows of 32 heads and lengths up to
+// 131072 took 11.7 GB, a million tokens 35.
+constexpr uint64_t ATTEND_ROOM = 1u << 20;
+
 // Parts that lengths up to `tiles` need at the least; one sequence has no others to wait for.
 uint32_t attend_least_parts(uint32_t tiles, uint32_t seqs) {
     if (seqs == 1) return 1;
@@ -442,9 +447,9 @@ int rl_attention_create(int device, uint32_t max_rows, uint32_t q_heads, uint32_
     if (!a) return fail(RL_ERR_CAPACITY, "out of host memory");
     a->device = device;
     a->max_rows = max_rows, a->q_heads = q_heads, a->kv_heads = kv_heads, a->dim = dim, a->max_len = max_len;
-    // Room for the least parts of every row, and for as many workgroups of 32 rows as the device holds.
+    // Room for the least parts of every row within the limit, and for as many workgroups of 32 rows as the device holds.
     const uint64_t heads = (uint64_t)max_rows * q_heads;
-    a->slots = std::max<uint64_t>(heads * attend_least_parts(attend_tiles(max_len), 2), CUS * 3 * 32);
+    a->slots = std::max<uint64_t>(std::min(heads * attend_least_parts(attend_tiles(max_len), 2), ATTEND_ROOM), CUS * 3 * 32);
     hipError_t e = hipMalloc(&a->part_out, a->slots * attend_dim(dim) * sizeof(float));
     if (e == hipSuccess) e = hipMalloc(&a->part_sum, a->slots * sizeof(float2));
     if (e == hipSuccess) e = hipMalloc(&a->part_count, heads * sizeof(uint32_t));
