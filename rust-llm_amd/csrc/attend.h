@@ -33,7 +33,8 @@ struct AttendArgs {
     uint32_t rows, seqs, q_heads, table_width, window, most_rows, max_len;
     float scale;
     uint32_t group;       // query heads of a key-value head
-    uint32_t blocks;      // row blocks a sequence
+    uint32_t blocks;      // row blocks a sequence, or with `packed` of all
+    uint32_t packed;      // whether a workgroup's sequence is found from its row block
     uint32_t part_tiles;  // tiles of 32 tokens a part
     uint32_t wide;        // whether q and out are aligned for 16-byte accesses
     float *part_out;      // [row * q_heads + head][part][HD]: sums of the weighted values
@@ -41,10 +42,14 @@ struct AttendArgs {
     uint32_t *part_count; // [row * q_heads + head]: parts written, ATTEND_NONE if the row sees nothing
     uint32_t parts;       // parts a row has room for
     uint32_t *arrived;    // [row * q_heads + head], of a block's first: its parts that are done; zero between calls
+    uint32_t group_inv, blocks_inv, columns_inv, heads_inv, tiles_inv; // inverse_of group, blocks, seqs * kv heads, kv heads, part_tiles
     uint32_t joins;       // whether the last part's workgroup joins them, else k_attend_join does
 };
 
 constexpr uint32_t ATTEND_THREADS = 256, ATTEND_WAVES = 4, ATTEND_TILE = 32;
+// Row blocks side by side, where those of a batch are counted through: eight of a run are on one XCD, whose L2 then has the
+// keys and values for all but the first.
+constexpr uint32_t ATTEND_RUN = 8;
 constexpr uint32_t ATTEND_MAX_PARTS = 256, ATTEND_NONE = 1u << 31;
 // Parts that the last of their workgroups joins, which saves a launch (one sequence of 611 tokens, 5 parts: 11.2 us with
 // it, 10.1 without); more are too much for one CU (21 parts of 16 rows of 256: 31.4 us with the launch, 40.5 without).
@@ -165,15 +170,35 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     __shared__ bool last;
 
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
-    // The row blocks of one sequence, head and part are eight workgroups apart: on one XCD, so that its L2 has the keys
-    // and values for all but the first.
-    const uint32_t job = blockIdx.x / (8 * a.blocks) * 8 + blockIdx.x % 8, block = blockIdx.x / 8 % a.blocks;
-    const uint32_t columns = a.seqs * a.cache.heads, part = job / columns, sh = job - part * columns;
-    if (part >= a.parts) return;
-    const uint32_t s = sh / a.cache.heads, head = sh - s * a.cache.heads, G = a.group;
+    const uint32_t G = a.group;
     // Not written while the kernel runs: read through the scalar cache where the index is the wave's.
     typedef const __attribute__((address_space(4))) int32_t constant_i32;
     const constant_i32 *starts = (constant_i32 *)(uintptr_t)a.starts, *lens = (constant_i32 *)(uintptr_t)a.lens;
+    uint32_t s, head, part, block;
+    if (a.packed) {
+        const uint32_t y = blockIdx.x / 8, at = (y / ATTEND_RUN * 8 + blockIdx.x % 8) * ATTEND_RUN + y % ATTEND_RUN;
+        const uint2 column = split_by(at, a.blocks, a.blocks_inv), of = split_by(column.x, a.cache.heads, a.heads_inv);
+        const uint32_t b = column.y;
+        part = of.x, head = of.y;
+        if (part >= a.parts) return;
+        // The last sequence whose row blocks begin at or before this one; no two begin at the same.
+        const auto first_block = [&](uint32_t i) { return (uint32_t)min(max(starts[i], 0), (int32_t)a.rows) * G / ROWS + i; };
+        s = 0;
+        for (uint32_t hi = a.seqs; hi - s > 1;) {
+            const uint32_t mid = s + (hi - s) / 2;
+            if (first_block(mid) <= b) s = mid;
+            else hi = mid;
+        }
+        if (first_block(s) > b) return;
+        block = b - first_block(s);
+    } else {
+        // The row blocks of one sequence, head and part are eight workgroups apart: on one XCD.
+        const uint2 eight = split_by(blockIdx.x / 8, a.blocks, a.blocks_inv);
+        const uint2 job = split_by(eight.x * 8 + blockIdx.x % 8, a.seqs * a.cache.heads, a.columns_inv);
+        const uint2 of = split_by(job.y, a.cache.heads, a.heads_inv);
+        block = eight.y, part = job.x, s = of.x, head = of.y;
+        if (part >= a.parts) return;
+    }
     const int32_t first = starts ? starts[s] : (int32_t)s;
     const int64_t rows = starts ? (int64_t)starts[s + 1] - first : 1;
     if (rows <= 0 || first < 0 || first + rows > a.rows) return; // no rows, or `starts` is not what it should be
@@ -195,14 +220,15 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
         }
         return;
     }
+    if (block >= (expanded + ROWS - 1) / ROWS) return;
     const uint32_t r0 = block * ROWS;
-    if (r0 >= expanded) return;
     const uint32_t count = min(expanded - r0, (uint32_t)ROWS);
-    const int32_t i0 = r0 / G, i1 = (r0 + count - 1) / G; // query rows of the block
+    const auto by_group = [&](uint32_t e) { return split_by(e, G, a.group_inv); }; // (query row, query head of the group)
+    const int32_t i0 = by_group(r0).x, i1 = by_group(r0 + count - 1).x; // query rows of the block
     const int32_t begin_min = span.begin(i0), begin_max = span.begin(i1), end_min = span.end(i0), end_max = span.end(i1);
     const bool mixed = begin_min != begin_max || end_min != end_max;
     const int32_t tile0 = begin_min / (int)ATTEND_TILE, tiles = (int32_t)((end_max + ATTEND_TILE - 1) / ATTEND_TILE) - tile0;
-    const uint32_t parts = tiles > 0 ? (tiles + a.part_tiles - 1) / a.part_tiles : 1; // of this block
+    const uint32_t parts = tiles > 0 ? split_by(tiles + a.part_tiles - 1, a.part_tiles, a.tiles_inv).x : 1; // of this block
     if (part >= parts) return;
 
     // The block's queries, a few values a thread; they go to LDS while the first tile is on its way.
@@ -210,8 +236,8 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     const uint32_t q_row = tid / TPR, q_at = tid % TPR * EPT;
     float x[EPT] = {};
     if (q_row < count) {
-        const uint32_t e = r0 + q_row;
-        const T *q = (const T *)a.q + (uint64_t)(first + e / G) * a.q_row + (uint64_t)(head * G + e % G) * a.q_head;
+        const uint2 e = by_group(r0 + q_row);
+        const T *q = (const T *)a.q + (uint64_t)(first + e.x) * a.q_row + (uint64_t)(head * G + e.y) * a.q_head;
 #pragma unroll
         for (uint32_t j = 0; j < EPT; j += 4)
             if (q_at + j < a.cache.dim) { // dim is a multiple of 16
@@ -423,7 +449,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     for (int rt = 0; rt < RT; rt++) {
         const uint32_t r = rt * 16 + col;
         mult[rt] = mults[r];
-        const int32_t i = r < count ? (r0 + r) / G : 0;
+        const int32_t i = r < count ? by_group(r0 + r).x : 0;
         row_begin[rt] = r < count ? span.begin(i) : begin_min; // rows past the block's see what any of it sees
         row_end[rt] = r < count ? span.end(i) : end_max;
     }
@@ -608,8 +634,9 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
                     f32x4{O[rt][m][i], O[rt][m + 1][i], O[rt][m + 2][i], O[rt][m + 3][i]};
         __syncthreads();
         for (uint32_t i = tid; i < 16 * (HD / 4); i += ATTEND_THREADS) {
-            const uint32_t r = rt * 16 + i / (HD / 4), d = i % (HD / 4) * 4, e = r0 + r;
+            const uint32_t r = rt * 16 + i / (HD / 4), d = i % (HD / 4) * 4;
             if (r >= count) break;
+            const uint2 e = by_group(r0 + r);
             float2 ms = make_float2(maxima[0][r], 0.0f);
 #pragma unroll
             for (uint32_t v = 1; v < ATTEND_WAVES; v++) ms.x = fmaxf(ms.x, maxima[v][r]);
@@ -620,8 +647,8 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
                 ms.y += sums[v][r] * f;
                 x += *(const f32x4 *)(ob + (v * 16 + i / (HD / 4)) * (HD + 4) + d) * f;
             }
-            const uint64_t row = first + e / G, qh = head * G + e % G, at = row * a.q_heads + qh;
-            const bool none = span.end(e / G) <= span.begin(e / G);
+            const uint64_t row = first + e.x, qh = head * G + e.y, at = row * a.q_heads + qh;
+            const bool none = span.end(e.x) <= span.begin(e.x);
             if (parts == 1) attend_write<T>(a, row, qh, d, none, ms, x, LIFT);
             else if (a.joins) {
                 shared_store(a.part_out + (at * a.parts + part) * HD + d, float2{x[0], x[1]});
@@ -640,8 +667,8 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     __builtin_amdgcn_s_waitcnt(ATTEND_STORED);
     __syncthreads();
     const auto of = [&](uint32_t r) {
-        const uint32_t e = r0 + r;
-        return (uint64_t)(first + e / G) * a.q_heads + head * G + e % G;
+        const uint2 e = by_group(r0 + r);
+        return (uint64_t)(first + e.x) * a.q_heads + head * G + e.y;
     };
     if (tid == 0) {
         uint32_t *arrived = a.arrived + of(0);
@@ -676,7 +703,8 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     }
     __syncthreads();
     for (uint32_t i = tid; i < count * (HD / 4); i += ATTEND_THREADS) {
-        const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4, e = r0 + r;
+        const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4;
+        const uint2 e = by_group(r0 + r);
         const float *x = a.part_out + of(r) * a.parts * HD + d;
         f32x4 all = {0, 0, 0, 0};
         for (uint32_t p0 = 0; p0 < parts; p0 += 8) {
@@ -690,7 +718,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
             for (uint32_t j = 0; j < 8; j++)
                 if (p0 + j < parts) all += f32x4{y[j][0].x, y[j][0].y, y[j][1].x, y[j][1].y} * factor[r * ATTEND_FEW + p0 + j];
         }
-        attend_write<T>(a, first + e / G, head * G + e % G, d, span.end(e / G) <= span.begin(e / G),
+        attend_write<T>(a, first + e.x, head * G + e.y, d, span.end(e.x) <= span.begin(e.x),
                         make_float2(maxima[0][r], sums[0][r]), all, LIFT);
     }
 }

@@ -510,8 +510,15 @@ int rl_attention_rows(rl_attention *h, const rl_kv_cache *cache, const rl_heads 
     a.part_out = h->part_out, a.part_sum = h->part_sum, a.part_count = h->part_count, a.arrived = h->arrived;
     const uint64_t expanded = (uint64_t)a.most_rows * a.group;
     const bool two = attend_two(cache->format, h->dim, (expanded + 15) / 16, (uint64_t)seqs * h->kv_heads);
-    a.blocks = (uint32_t)((expanded + (two ? 31 : 15)) / (two ? 32 : 16));
-    const uint64_t columns = (uint64_t)seqs * h->kv_heads * a.blocks;
+    const uint32_t block_rows = two ? 32 : 16;
+    // A grid of the longest sequence's row blocks for every sequence, or of the sum of all. The second asks each workgroup to
+    // find its sequence, and is taken where it is less than half as large; the first can pass what a launch takes. 64
+    // sequences of 2048 tokens, 32 / 8 heads of 128 bf16, us, first / second: all with 64 rows 844 / 899, 21 of them (the
+    // others one) 509 / 374, one 361 / 133; eight with 9 rows 115 / 121.
+    const uint64_t longest = (expanded + block_rows - 1) / block_rows, sum = (uint64_t)rows * a.group / block_rows + seqs;
+    a.packed = sum * 2 < longest * seqs;
+    a.blocks = (uint32_t)(a.packed ? sum : longest);
+    const uint64_t columns = (uint64_t)(a.packed ? 1 : seqs) * h->kv_heads * a.blocks;
     const uint64_t seen = window ? std::min<uint64_t>(a.max_len, (uint64_t)window + a.most_rows - 1) : a.max_len;
     const uint32_t tiles = attend_tiles(seen);
     const uint64_t room = std::min<uint64_t>(h->slots / ((uint64_t)rows * h->q_heads), ATTEND_MAX_PARTS);
@@ -522,8 +529,12 @@ int rl_attention_rows(rl_attention *h, const rl_kv_cache *cache, const rl_heads 
     a.part_tiles = (a.part_tiles + ATTEND_WAVES - 1) / ATTEND_WAVES * ATTEND_WAVES;
     a.parts = (tiles + a.part_tiles - 1) / a.part_tiles;
     a.joins = a.parts <= ATTEND_FEW;
-    // Jobs (sequence, head and part) in eights, the row blocks of each eight together.
-    const uint64_t groups = ((uint64_t)seqs * h->kv_heads * a.parts + 7) / 8 * 8 * a.blocks;
+    a.group_inv = inverse_of(a.group), a.blocks_inv = inverse_of(a.blocks), a.heads_inv = inverse_of(h->kv_heads);
+    a.columns_inv = inverse_of(seqs * h->kv_heads), a.tiles_inv = inverse_of(a.part_tiles);
+    // Jobs (sequence, head and part) in eights, the row blocks of each eight together; or eight runs of row blocks at a time.
+    constexpr uint64_t RUNS = 8 * ATTEND_RUN;
+    const uint64_t groups = a.packed ? (columns * a.parts + RUNS - 1) / RUNS * RUNS
+                                     : ((uint64_t)seqs * h->kv_heads * a.parts + 7) / 8 * 8 * a.blocks;
     if (groups > 2 * MAX_ROWS - 1) return fail(RL_ERR_CAPACITY, "too many sequences times row blocks in a call");
     with_type(q->dtype, [&](auto t) {
         launch_attend<decltype(t)>(a, cache->format, two, (uint32_t)groups, static_cast<hipStream_t>(stream));
