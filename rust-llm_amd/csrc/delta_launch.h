@@ -14,6 +14,11 @@ void launch_delta_chunks(const DeltaArgs &a, const DeltaWork &w, hipStream_t s);
 // bf16 sequence (256 waves) 13.7 / 12.5, f32 12.4 / 11.0. With every SIMD busy the reductions cost, and 16 columns need fewer.
 constexpr uint32_t DELTA_FEW = 512;
 
+// Workgroups of k_delta_chunks: a sequence's heads in eights, 16 columns each.
+inline uint64_t delta_groups(const DeltaArgs &a) {
+    return ((uint64_t)a.seqs * a.value_heads + 7) / 8 * 8 * (a.value_dim / 16);
+}
+
 #ifdef RL_DELTA_UNIT
 template <typename T, int Q>
 void launch_delta_steps_of(const DeltaArgs &a, hipStream_t s) {
@@ -31,8 +36,7 @@ void launch_delta_steps(const DeltaArgs &a, hipStream_t s) {
 template <typename T, int DK>
 void launch_delta_chunks_dim(const DeltaArgs &a, const DeltaWork &w, hipStream_t s) {
     hipLaunchKernelGGL((k_delta_prepare<T, DK>), dim3((a.rows / CHUNK + a.seqs) * a.value_heads), dim3(256), 0, s, a, w);
-    const uint32_t jobs = (a.seqs * a.value_heads + 7) / 8 * 8;
-    hipLaunchKernelGGL((k_delta_chunks<T, DK>), dim3(jobs * (a.value_dim / 16)), dim3(DELTA_CHUNK_THREADS), 0, s, a, w);
+    hipLaunchKernelGGL((k_delta_chunks<T, DK>), dim3((uint32_t)delta_groups(a)), dim3(DELTA_CHUNK_THREADS), 0, s, a, w);
 }
 
 template <typename T>

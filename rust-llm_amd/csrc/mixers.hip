@@ -626,11 +626,12 @@ int rl_delta_rows(rl_delta *h, const rl_heads *q, const rl_heads *k, const rl_he
     a.key_dim = h->key_dim, a.value_dim = h->value_dim;
     a.scale = scale, a.eps = norm_eps;
     a.wide = wide(q) && wide(k) && wide(v) && wide(out);
-    // Chunks where some sequence has the rows for them and the workspace holds all.
+    // Chunks where some sequence has the rows for them, the workspace holds all and one launch too (below 2^32 threads).
     const uint32_t most = !starts ? 1 : most_rows ? std::min(most_rows, rows) : rows;
     const bool alone = (uint64_t)seqs * h->value_heads * (h->value_dim / 16) <= CUS;
     const uint32_t least = !alone ? DELTA_CHUNKED_MANY : q->dtype == RL_BF16 ? DELTA_CHUNKED : DELTA_CHUNKED_WIDE;
-    const bool chunked = most >= least && rows / CHUNK + seqs <= h->chunks;
+    const uint64_t groups = delta_groups(a);
+    const bool chunked = most >= least && rows / CHUNK + seqs <= h->chunks && groups * DELTA_CHUNK_THREADS < 1ull << 32;
     with_type(q->dtype, [&](auto t) {
         if (chunked) launch_delta_chunks<decltype(t)>(a, h->work, static_cast<hipStream_t>(stream));
         else launch_delta_steps<decltype(t)>(a, static_cast<hipStream_t>(stream));

@@ -1,12 +1,12 @@
-"""Attention of one prompt in a batch of thousands of single tokens: the work is the
-sum of the sequences', and so is the grid."""
+"""Batches of thousands of sequences, most of them of one token or none: their grids
+have to fit a launch."""
 import numpy as np
 import pytest
 import torch
 
 import mixer_fixtures as F
 import rl_mixers as M
-from test_gpu_mixers import randn
+from test_gpu_mixers import delta_check, delta_inputs, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +52,21 @@ def test_a_prompt_among_thousands_of_single_tokens(device, at):
     slack = mass * (2 * d + 2.0 ** -15)[..., None]  # the weights' 16 bits, their scores' errors and a few sums
     assert (np.abs(F.as64(out) - want) / (slack + F.rounding(np.abs(want) + slack, "bf16"))).max() <= 1
     assert (np.abs(F.as64(lse) - want_lse) / (d + 2.0 ** -20 + np.abs(want_lse) * 2.0 ** -23)).max() <= 1
+
+
+def test_more_states_than_a_launch_of_chunks_takes(device):
+    # 8192 sequences of 64 heads of 256 columns are 2^23 workgroups of 512 threads; one sequence has rows.
+    g = np.random.default_rng(71)
+    seqs, n, kh, vh, dk, dv, at = 8192, 24, 1, 64, 16, 256, 5003
+    h = M.DeviceDelta(2 ** 17, seqs, kh, vh, dk, dv)
+    inputs = delta_inputs(g, device, [n], kh, vh, dk, dv, "bf16", True, 0.2)
+    q, k, v, gates, beta, states = inputs
+    before, out = F.as64(states), torch.empty_like(v)
+    slots = np.full((2, seqs), -1)
+    slots[:, at] = 0, 1
+    starts = np.where(np.arange(seqs + 1) > at, n, 0)
+    i32 = lambda x: torch.from_numpy(np.ascontiguousarray(x, np.int32)).to(device)  # noqa: E731
+    h.rows(q, k, v, gates, beta, out, states, i32(slots[0]), i32(slots[1]), i32(starts), normalise=True, most_rows=n)
+    torch.cuda.synchronize()
+    delta_check([n], inputs, F.as64(out), before[:1], F.as64(states)[1:2], dk, "bf16", True, dk ** -0.5, n)
+    h.close()
