@@ -187,9 +187,9 @@ uint32_t attend_least_parts(uint32_t tiles, uint32_t seqs) {
 
 // Rows of a sequence from which chunks are faster than one token after the other (us, steps / chunks; 32 heads of 128 x
 // 128). While every workgroup of the chunks has a CU to itself they cost the same for any rows up to 64: one bf16
-// sequence of 9 rows 12.5 / 15.7, of 16 19.3 / 15.7; f32, more products, 16 rows 16.9 / 22.0, 24 rows 23.5 / 22.1. Beyond
-// that they wait for each other: 16 sequences of 16 rows 54.5 / 75.0, of 24 74.8 / 75.2.
-constexpr uint32_t DELTA_CHUNKED = 13, DELTA_CHUNKED_WIDE = 20, DELTA_CHUNKED_MANY = 24;
+// sequence of 12 rows 15.4 / 16.1, of 16 19.3 / 16.1; f32, more products, 16 rows 17.0 / 22.5, 24 rows 23.2 / 22.5. Beyond
+// that they wait for each other: 16 sequences of 16 rows 54.6 / 79, of 24 76.2 / 78.7, of 32 98.7 / 78.3.
+constexpr uint32_t DELTA_CHUNKED = 13, DELTA_CHUNKED_WIDE = 20, DELTA_CHUNKED_MANY = 25;
 
 int launched(const char *what) {
     const hipError_t e = hipGetLastError();
