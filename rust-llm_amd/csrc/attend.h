@@ -60,10 +60,10 @@ constexpr int attend_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 12
 
 // Whether a workgroup takes two row tiles of `count` that a sequence has: keys and values are read once for both, but
 // fewer workgroups share a CU. bf16 queries, us, two / one, sequences x tokens, query / key-value heads x dim:
-//   64:  1 x 20011 tokens, 16/8, 18 rows 15.3 / 17.0, 36 rows 18.3 / 19.7; 32 x 3001 39.7 / 42.0, 52.5 / 58.6
-//   128: a tile left over costs a block's time (32 x 3001, 32/8, 36 rows: bf16 134 / 116, int8 84.0 / 76.3); else int8
-//        20 rows 46.0 / 57.0, 64 rows 88.1 / 102, bf16 85.0 / 91.6, 141 / 145, with columns for half the CUs or fewer
-//        (4 x 8001) bf16 30.4 / 29.2, 59.8 / 48.7
+//   64:  1 x 20011 tokens, 16/8, 18 rows 15.7 / 17.5, 36 rows 19.0 / 20.0; 32 x 3001 37.8 / 42.7, 53.2 / 59.7
+//   128: a tile left over costs a block's time (32 x 3001, 32/8, 36 rows: bf16 137 / 118, int8 84.6 / 80.9); else int8
+//        20 rows 45.6 / 57.3, 64 rows 86.4 / 104, bf16 83.2 / 89.9, 134 / 144, with columns for half the CUs or fewer
+//        (4 x 8001) bf16 30.2 / 29.1, 58.9 / 48.6
 //   256: the sums take the registers (32 x 3001, 16/4, 32 rows of int8 61.5 / 53.9)
 inline bool attend_two(uint32_t format, uint32_t dim, uint64_t count, uint64_t columns) {
     if (count < 2 || attend_dim(dim) == 256) return false;

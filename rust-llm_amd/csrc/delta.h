@@ -39,8 +39,9 @@ __device__ inline float quad_sum(float x) {
 // depend on the others, so a state splits over as many waves as it has column
 // groups and no wave waits for another. Lane l has the columns 4 (l % Q) .. + 4 of
 // the rows R (l / Q) .. + R; the two products with the state are summed over the
-// 64 / Q lanes of a column, in registers. A step's inputs are loaded, and made ready,
-// while the one before is computed. For single tokens bound by HBM (the state is
+// 64 / Q lanes of a column, in registers. A step's inputs are loaded while the one
+// before is computed; their norms, roots and e^g are formed at its own start. For single
+// tokens bound by HBM (the state is
 // read and written once): 64 sequences of 32 heads of 128 x 128 take 63.5 us, 4.2
 // TB/s. For several by the chain of a step, two reductions over the wave: 9 rows of
 // one sequence 11.9 us, about 1 us a row.

@@ -178,8 +178,8 @@ __device__ inline void with_flag(bool x, F f) {
 // substitution, a lane a column, the rest column by column of blocks,
 // X_ij = -D_i sum_k L_ik X_kj, in f32 products whose results are the next product's
 // operand where they stand. Bound by what it writes and its chain of small steps;
-// four workgroups share a CU. 8192 bf16 tokens of 16 / 32 heads of 128: 70 us, about
-// 260 MB read and written (3.7 TB/s).
+// four workgroups share a CU. 8192 bf16 tokens of 16 / 32 heads of 128: 74 us, about
+// 290 MB read and written (4.0 TB/s).
 template <typename T, int DK>
 __global__ void __launch_bounds__(256, DK <= 128 && sizeof(T) == 2 ? 4 : 2) k_delta_prepare(DeltaArgs a, DeltaWork w) {
     constexpr int NP = parts_of<T>(), STEPS = DK / 32, LS = 68, KS = DK + 16 / (int)sizeof(T);
@@ -416,10 +416,12 @@ struct DeltaChunk {
 // U, P U beside the new state, their stores beside the next chunk's K S (P U there
 // too took 8192 tokens 317 us instead of 305). Everything else comes from memory,
 // loaded while the chunk before is computed. Bound by the first four's chain: LDS, the
-// products (36 of 16 cycles) and the barriers: 1.9 us a chunk, 240 us for 8192
+// products (36 of 16 cycles) and the barriers: 2.0 us a chunk, 250 us for 8192
 // tokens of 32 heads of 128 x 128, where the 256 workgroups have a CU each.
 // Registers for two workgroups a CU spill, and gain only where there are more:
-// 16 sequences of 64 tokens 82.6 -> 70.9 us with them, one of 8192 305 -> 338.
+// 16 sequences of 64 tokens 82.6 -> 70.9 us with them, one of 8192 305 -> 338 (both
+// with P in one part). f32 with more than 128 key dims spills as it is (256 bytes a
+// lane): 10 us a chunk.
 constexpr uint32_t DELTA_CHUNK_THREADS = 512;
 template <typename T, int DK>
 __global__ void __launch_bounds__(DELTA_CHUNK_THREADS) k_delta_chunks(DeltaArgs a, DeltaWork w) {

@@ -86,8 +86,8 @@ __device__ inline void turn8(const RotaryArgs &r, const T *in, uint32_t at, cons
 // first CACHE_AHEAD vectors of a group are loaded before the angles are formed and
 // waited for. A workgroup is one chain (position, angles, barrier, codes), so what
 // counts is how many share a CU: with partners and the rare layouts at 110
-// registers four did, 5003 rows of 4 heads of 256 bf16 to f8 (31 MB) took 14.6 us;
-// with 55 eight do, 10.9 us (2.8 TB/s). 64 int8 rows of 8 heads of 128: 3.0 us,
+// registers four did, 5003 rows of 4 heads of 256 bf16 to f8 (31 MB) took 16.7 us;
+// with 55 eight do, 11.8 us (2.6 TB/s). 64 int8 rows of 8 heads of 128: 3.4 us,
 // all chain.
 template <typename T, int FMT, int G>
 __global__ void __launch_bounds__(CACHE_THREADS) k_cache_write(CacheArgs c, CacheRows in, const int64_t *slots,
@@ -150,8 +150,8 @@ __global__ void __launch_bounds__(CACHE_THREADS) k_cache_write(CacheArgs c, Cach
             float y[8];
             if (step > 0x1p-90f && step < 0x1p90f) {
                 // The IEEE quotient by one reciprocal: x r and its remainder's correction are correctly rounded where r is
-                // the rounded 1 / step and nothing leaves the normal numbers (Markstein); quotients below 2^-9 round to 0
-                // either way.
+                // the rounded 1 / step and nothing leaves the normal numbers (Markstein); a quotient so small that its remainder
+                // does is far below 2^-10, where the smallest code begins, and rounds to 0 either way.
                 const float r = 1.0f / step;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(CACHE_THREADS) k_cache_write(CacheArgs c, Cach
     }
 }
 
-// The same mapping the other way: no work but the bytes. The 5003 rows above 6.9 us (4.5 TB/s), 64 int8 rows 2.2 us.
+// The same mapping the other way: no work but the bytes. The 5003 rows above 7.8 us, 6.8 at least (4.6 TB/s), 64 int8 rows 2.5.
 template <typename T, int FMT, int G>
 __global__ void __launch_bounds__(CACHE_THREADS) k_cache_read(CacheArgs c, CacheRows out, const int64_t *slots) {
     const uint32_t lane = threadIdx.x % G, at = lane * 8;
