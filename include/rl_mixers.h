@@ -128,10 +128,11 @@ int rl_kv_cache_read(rl_kv_cache *cache, const int64_t *slots, uint32_t rows, co
  * Query head h reads the key-value head h / (q_heads / kv_heads). A row that sees
  * nothing gives zeros and an lse of -inf. Scores, softmax and sums are f32; the
  * weights go into the product with the values as sums of 16-bit parts, good to 16
- * bits or more for 16-bit queries and to 22 or more for f32 ones. What a
- * row does not see does not reach it, whatever it holds. An infinity among the f16 or
- * bf16 values that a row sees may read as NaN (a part of its weight may be 0), and so
- * may one among such keys to f32 queries. */
+ * bits or more for 16-bit queries and to 22 or more for f32 ones (over f16 values no
+ * finer than 2^-33 of the largest weight so far). What a row does not see does not
+ * reach it, whatever it holds. An infinity among the f16 or bf16 values that a row
+ * sees may read as NaN (a part of its weight may be 0), and so may one among such
+ * keys to f32 queries. */
 typedef struct rl_attention rl_attention;
 
 /* Workspace for calls of up to max_rows query rows over caches of kv_heads heads
@@ -147,9 +148,9 @@ void rl_attention_destroy(rl_attention *attention);
  * queries, one in RL_BF16 bf16 or f32, the 8-bit ones all three. starts i32
  * [seqs + 1] rising from 0 to rows, or NULL for one row a sequence (rows == seqs);
  * lens i32 [seqs], a negative one as 0; pages i32 [seqs][table_width]; lse f32
- * [rows][q_heads] or NULL. most_rows and max_len bound the rows and tokens of any one sequence
- * (0: as many as the call has rows, and the handle's max_len); a sequence past
- * either bound, or one that needs a page outside its table or the cache, gives
+ * [rows][q_heads] or NULL. most_rows and max_len bound the rows and tokens of any one
+ * sequence (0: as many as the call has rows, and the handle's max_len); a sequence
+ * past either bound, or one that needs a page outside its table or the cache, gives
  * NaN. Only entries of `pages` that hold tokens in sight are read. */
 int rl_attention_rows(rl_attention *attention, const rl_kv_cache *cache, const rl_heads *q, const rl_heads *out,
                       float *lse, uint32_t rows, const int32_t *starts, const int32_t *lens, uint32_t seqs,
@@ -168,7 +169,8 @@ typedef struct rl_delta rl_delta;
 /* Workspace for calls of up to max_rows tokens in up to max_seqs sequences: none below
  * 13 rows, else for max_rows / 64 + min(max_seqs, max_rows / 16 + 1) chunks, each of
  * 41 KiB a value head and 768 D bytes a key head (D: key_dim rounded up to 64, 128 or
- * 256). A call of more sequences than its chunks have room for goes token by token.
+ * 256). A call of more sequences than its chunks have room for, or of 2^27 columns of
+ * states (seqs * value_heads * value_dim) or more, goes token by token.
  * value_heads: a multiple of key_heads. key_dim, value_dim: 16 to 256, multiples of
  * 16. */
 int rl_delta_create(int device, uint32_t max_rows, uint32_t max_seqs, uint32_t key_heads, uint32_t value_heads,
@@ -182,7 +184,7 @@ void rl_delta_destroy(rl_delta *delta);
  * sequence s begins from states[slots_in[s]] (zeros if that is negative) and
  * leaves its state in states[slots_out[s]] (nowhere if that is negative). The two
  * may be equal; else no slot that a sequence of the call reads may be one that
- * another writes. A slot from state_slots on reads as NaN and is not written. A
+ * another writes, and no two sequences write one slot. A slot from state_slots on reads as NaN and is not written. A
  * sequence without rows passes its state on. most_rows bounds the rows of any one
  * sequence (0: as many as the call has); it may be any number, since it only picks
  * the form that is used for all of them, one token after the other or chunks on the

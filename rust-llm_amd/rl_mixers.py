@@ -230,8 +230,9 @@ class DeviceDelta(_Handle):
              eps=1e-6, most_rows=0, stream=None):
         """q, k [rows][key_heads][key_dim]; v, out [rows][value_heads][value_dim];
         g, beta f32 [rows][value_heads]; states f32 [slots][value_heads][key_dim]
-        [value_dim], contiguous; slots_in, slots_out int32 [seqs]; starts int32
-        [seqs + 1] (None: one row a sequence); scale: key_dim^-1/2 if None."""
+        [value_dim], contiguous; slots_in, slots_out int32 [seqs] (negative: none;
+        the slots written distinct); starts int32 [seqs + 1] (None: one row a
+        sequence); scale: key_dim^-1/2 if None."""
         rows, seqs, device = q.shape[0], slots_in.shape[0], self.device
         if k.shape[0] != rows or v.shape[0] != rows or out.shape[0] != rows:
             raise ValueError("q, k, v and out have one row a token")
