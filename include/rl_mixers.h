@@ -157,6 +157,21 @@ int rl_attention_rows(rl_attention *attention, const rl_kv_cache *cache, const r
                       const int32_t *pages, uint32_t table_width, float scale, uint32_t window, uint32_t most_rows,
                       uint32_t max_len, void *stream);
 
+/* The same where sequences share long beginnings, whose keys and values are then read
+ * once for a group and not once for each sequence. The sequences group_starts[g] ..
+ * group_starts[g + 1] (i32 [groups + 1], rising from 0 to seqs) have the same
+ * prefix_lens[g] tokens (i32, a negative one as 0) before their own, the t-th of them in
+ * slot prefix_pages[g * prefix_width + t / page] * page + t % page. lens and pages are
+ * those of their own tokens, which begin a page: every row sees its whole prefix and its
+ * own sequence's tokens up to its own, as above without a window. max_prefix bounds the
+ * tokens of any one prefix (0: the handle's max_len); past it the rows of the group are
+ * NaN. rows * q_heads at most 2^20. */
+int rl_attention_shared(rl_attention *attention, const rl_kv_cache *cache, const rl_heads *q, const rl_heads *out,
+                        float *lse, uint32_t rows, const int32_t *starts, const int32_t *lens, uint32_t seqs,
+                        const int32_t *pages, uint32_t table_width, const int32_t *group_starts,
+                        const int32_t *prefix_lens, uint32_t groups, const int32_t *prefix_pages, uint32_t prefix_width,
+                        float scale, uint32_t most_rows, uint32_t max_len, uint32_t max_prefix, void *stream);
+
 /* --------------------------------------------------------- delta rule --
  * Every value head of a sequence has a state S [key_dim][value_dim], and each
  * token, in order, does
@@ -195,6 +210,62 @@ int rl_delta_rows(rl_delta *delta, const rl_heads *q, const rl_heads *k, const r
                   const float *g, uint64_t g_stride, const float *beta, uint64_t beta_stride, float *states,
                   uint64_t state_slots, const int32_t *slots_in, const int32_t *slots_out, const int32_t *starts,
                   uint32_t rows, uint32_t seqs, float scale, float norm_eps, uint32_t most_rows, void *stream);
+
+/* -------------------------------------------------- short convolution --
+ * Every channel's row is the sum of its last `width` rows:
+ *   y[t][c] = act(bias[c] + sum_j weight[c][j] x[t - width + 1 + j][c])
+ * with act(y) = y or y / (1 + e^-y). The width - 1 rows before a sequence's first are
+ * its state, as they came in. Sums are f32, rounded once to the output's type. */
+enum { RL_CONV_PLAIN = 0, RL_CONV_SILU = 1 };
+
+typedef struct rl_conv rl_conv;
+
+/* weight [channels][width] and bias [channels] (or NULL) f32 on the host, copied. width
+ * 2 to 8, channels at most 2^20. */
+int rl_conv_create(int device, uint32_t channels, uint32_t width, const float *weight, const float *bias,
+                   uint32_t activation, rl_conv **out);
+void rl_conv_destroy(rl_conv *conv);
+
+/* x, out [rows][1][channels] of one type; out must not overlap x. starts i32 [seqs + 1]
+ * rising from 0 to rows, or NULL for one row a sequence. states [state_slots][width - 1]
+ * [channels] of x's type: sequence s has its rows before the first in
+ * states[slots_in[s]] (zeros if that is negative) and leaves its last ones, the old ones
+ * among them if it is shorter, in states[slots_out[s]] (nowhere if that is negative),
+ * under the rules of rl_delta_rows: the two may be equal; else no slot that a sequence
+ * reads is one that another writes, and none is written twice. A slot from state_slots
+ * on reads as NaN and is not written. A sequence without rows passes its state on. */
+int rl_conv_rows(rl_conv *conv, const rl_heads *x, const rl_heads *out, void *states, uint64_t state_slots,
+                 const int32_t *slots_in, const int32_t *slots_out, const int32_t *starts, uint32_t rows, uint32_t seqs,
+                 void *stream);
+
+/* --------------------------------------------------------- state space --
+ * Every channel has a state h [state_dim], and each token, in order, does
+ *   s = softplus(dt + dt_bias);  h[n] <- e^(s a[n]) h[n] + s x b[n]
+ *   out = (sum_n c[n] h[n] + skip x) (z / (1 + e^-z))
+ * with b and c of the channel's group (channel / (channels / groups)). State and sums
+ * are f32. */
+typedef struct rl_scan rl_scan;
+
+/* a [channels][state_dim] (negative in use), skip and dt_bias [channels] (or NULL:
+ * zeros) f32 on the host, copied. state_dim 4 to 256, a multiple of 4; channels a
+ * multiple of groups, at most 2^20. Workspace for calls of up to max_rows tokens in up to
+ * max_seqs sequences: at most 22 MB and two states more. */
+int rl_scan_create(int device, uint32_t max_rows, uint32_t max_seqs, uint32_t channels, uint32_t groups,
+                   uint32_t state_dim, const float *a, const float *skip, const float *dt_bias, rl_scan **out);
+void rl_scan_destroy(rl_scan *scan);
+
+/* x, dt, z, out [rows][1][channels] and b, c [rows][groups][state_dim] of one type; z NULL
+ * leaves the last factor out, softplus 0 takes s = dt + dt_bias. out may be x, dt or z
+ * itself (same data and strides) or must not overlap them. states f32 [state_slots][channels]
+ * [state_dim], slots_in, slots_out and starts as in rl_delta_rows. most_rows bounds the
+ * rows of any one sequence (0: as many as the call has); it may be any number, since it
+ * only picks the form that is used for all of them: one token after the other, or long
+ * sequences in pieces side by side. Both are as exact as f32 sums, but do not give the
+ * same bits. An infinity may read as NaN. */
+int rl_scan_rows(rl_scan *scan, const rl_heads *x, const rl_heads *dt, const rl_heads *z, const rl_heads *b,
+                 const rl_heads *c, const rl_heads *out, float *states, uint64_t state_slots, const int32_t *slots_in,
+                 const int32_t *slots_out, const int32_t *starts, uint32_t rows, uint32_t seqs, int softplus,
+                 uint32_t most_rows, void *stream);
 
 #ifdef __cplusplus
 }

@@ -44,7 +44,15 @@ struct AttendArgs {
     uint32_t *arrived;    // [row * q_heads + head], of a block's first: its parts that are done; zero between calls
     uint32_t group_inv, blocks_inv, columns_inv, heads_inv, tiles_inv; // inverse_of group, blocks, seqs * kv heads, kv heads, part_tiles
     uint32_t joins;       // whether the last part's workgroup joins them, else k_attend_join does
+    // Shared prefixes. The rows of a group's sequences group_starts[g] .. group_starts[g + 1] see all of its prefix: part p
+    // of it is partial result `shared` + p of their `stride`, with a maximum of -inf where it has no tokens.
+    const int32_t *group_starts;
+    uint32_t shared, shared_parts, stride, group_end; // group_end: the sequences of the call
 };
+
+// What a launch does: sequences by themselves; the prefixes of groups of sequences, in which `seqs`, `lens`, `pages` and
+// `max_len` are the groups' and their prefixes'; sequences whose rows have a prefix's partial results beside their own.
+enum AttendMode { ATTEND_ALONE, ATTEND_PREFIX, ATTEND_JOINED };
 
 constexpr uint32_t ATTEND_THREADS = 256, ATTEND_WAVES = 4, ATTEND_TILE = 32;
 // Row blocks side by side, where those of a batch are counted through: eight of a run are on one XCD, whose L2 then has the
@@ -94,10 +102,11 @@ __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The sequence's rows, and what a row sees: [begin, end). len is 0 or more and n at most 2^23, so no sum here leaves 32
 // bits; tokens past a tile's or a block's end are counted unsigned, since len may be the largest.
+template <AttendMode MODE>
 struct AttendSpan {
     int32_t len, n, window;
-    __device__ int32_t end(int32_t i) const { return max(len - n + i + 1, 0); }
-    __device__ int32_t begin(int32_t i) const { return window ? max(end(i) - window, 0) : 0; }
+    __device__ int32_t end(int32_t i) const { return MODE == ATTEND_PREFIX ? len : max(len - n + i + 1, 0); }
+    __device__ int32_t begin(int32_t i) const { return MODE == ATTEND_ALONE && window ? max(end(i) - window, 0) : 0; }
 };
 
 // Two 8-bit codes, the low or high half of u, as two 16-bit values. Keys: int8 codes lie in the cache with their sign
@@ -145,7 +154,18 @@ __device__ inline void attend_write(const AttendArgs &a, uint64_t row, uint64_t 
         a.lse[row * a.q_heads + head] = none ? -INFINITY : ((ms.x - lift) + log2f(ms.y)) * 0.693147180559945309f;
 }
 
-template <typename T, int FMT, int HD, int RT, bool P16>
+// One partial result more of four columns of a row, at its maximum and sum.
+__device__ inline void attend_add(float2 &ms, f32x4 &x, float2 more, f32x4 y) {
+    if (more.x == -INFINITY && more.y == 0.0f) return; // no tokens: its columns may be anything
+    const float most = fmaxf(ms.x, more.x), f = ms.x == -INFINITY ? 1.0f : exp2_fast(ms.x - most), g = exp2_fast(more.x - most);
+    ms = make_float2(most, ms.y * f + more.y * g);
+    x = x * f + y * g;
+}
+
+// The maximum of a part whose tokens all have scores of -inf: it has tokens, but no weight beside any other.
+constexpr float ATTEND_LOWEST = -3.402823466e38f;
+
+template <typename T, int FMT, int HD, int RT, bool P16, AttendMode MODE>
 __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT, HD, RT)) k_attend(AttendArgs a) {
     constexpr bool EIGHT = FMT == RL_I8 || FMT == RL_F8, F32Q = sizeof(T) == 4;
     // Element types of the two products. 8-bit codes are exact in either; queries fit f16 scaled by a power of two
@@ -174,6 +194,14 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     // Not written while the kernel runs: read through the scalar cache where the index is the wave's.
     typedef const __attribute__((address_space(4))) int32_t constant_i32;
     const constant_i32 *starts = (constant_i32 *)(uintptr_t)a.starts, *lens = (constant_i32 *)(uintptr_t)a.lens;
+    // The first row of sequence or group i.
+    const auto first_of = [&](uint32_t i) {
+        if constexpr (MODE == ATTEND_PREFIX) {
+            const int32_t at = min(max(((constant_i32 *)(uintptr_t)a.group_starts)[i], 0), (int32_t)a.group_end);
+            return starts ? starts[at] : at;
+        } else
+            return starts ? starts[i] : (int32_t)i;
+    };
     uint32_t s, head, part, block;
     if (a.packed) {
         const uint32_t y = blockIdx.x / 8, at = (y / ATTEND_RUN * 8 + blockIdx.x % 8) * ATTEND_RUN + y % ATTEND_RUN;
@@ -182,7 +210,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
         part = of.x, head = of.y;
         if (part >= a.parts) return;
         // The last sequence whose row blocks begin at or before this one; no two begin at the same.
-        const auto first_block = [&](uint32_t i) { return (uint32_t)min(max(starts[i], 0), (int32_t)a.rows) * G / ROWS + i; };
+        const auto first_block = [&](uint32_t i) { return (uint32_t)min(max(first_of(i), 0), (int32_t)a.rows) * G / ROWS + i; };
         s = 0;
         for (uint32_t hi = a.seqs; hi - s > 1;) {
             const uint32_t mid = s + (hi - s) / 2;
@@ -199,10 +227,10 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
         block = eight.y, part = job.x, s = of.x, head = of.y;
         if (part >= a.parts) return;
     }
-    const int32_t first = starts ? starts[s] : (int32_t)s;
-    const int64_t rows = starts ? (int64_t)starts[s + 1] - first : 1;
+    const int32_t first = first_of(s);
+    const int64_t rows = MODE == ATTEND_PREFIX ? (int64_t)first_of(s + 1) - first : starts ? (int64_t)starts[s + 1] - first : 1;
     if (rows <= 0 || first < 0 || first + rows > a.rows) return; // no rows, or `starts` is not what it should be
-    AttendSpan span{max(lens[s], 0), (int32_t)rows, (int32_t)a.window}; // a negative length is none
+    AttendSpan<MODE> span{max(lens[s], 0), (int32_t)rows, (int32_t)a.window}; // a negative length is none
     const uint32_t expanded = (uint32_t)span.n * G;
     const int32_t longest = span.end(span.n - 1);
     const uint32_t page = a.cache.page;
@@ -214,9 +242,15 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
         for (uint64_t i = tid; i < (uint64_t)expanded * dim; i += ATTEND_THREADS) {
             const uint32_t e = (uint32_t)(i / dim), d = (uint32_t)(i - (uint64_t)e * dim);
             const uint64_t row = first + e / G, qh = head * G + e % G;
+            if constexpr (MODE == ATTEND_PREFIX) { // one part that is NaN, and no others
+                if (d < a.shared_parts)
+                    a.part_sum[(row * a.q_heads + qh) * a.stride + a.shared + d] = d ? make_float2(-INFINITY, 0.0f) : make_float2(0.0f, NAN);
+                continue;
+            }
             ((T *)a.out)[row * a.out_row + qh * a.out_head + d] = (T)NAN;
             if (d == 0 && a.lse) a.lse[row * a.q_heads + qh] = NAN;
-            if (d == 0 && !a.joins) a.part_count[row * a.q_heads + qh] = 1; // nothing to join
+            if (d == 0 && MODE == ATTEND_ALONE && !a.joins) a.part_count[row * a.q_heads + qh] = 1; // nothing to join
+            if (d == 0 && MODE == ATTEND_JOINED && a.parts > 1) a.part_count[row * a.q_heads + qh] = 0; // likewise
         }
         return;
     }
@@ -229,7 +263,14 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
     const bool mixed = begin_min != begin_max || end_min != end_max;
     const int32_t tile0 = begin_min / (int)ATTEND_TILE, tiles = (int32_t)((end_max + ATTEND_TILE - 1) / ATTEND_TILE) - tile0;
     const uint32_t parts = tiles > 0 ? split_by(tiles + a.part_tiles - 1, a.part_tiles, a.tiles_inv).x : 1; // of this block
-    if (part >= parts) return;
+    if (part >= parts) {
+        if constexpr (MODE == ATTEND_PREFIX) // nothing here
+            for (uint32_t i = tid; i < count; i += ATTEND_THREADS) {
+                const uint2 e = by_group(r0 + i);
+                a.part_sum[((uint64_t)(first + e.x) * a.q_heads + head * G + e.y) * a.stride + a.shared + part] = make_float2(-INFINITY, 0.0f);
+            }
+        return;
+    }
 
     // The block's queries, a few values a thread; they go to LDS while the first tile is on its way.
     constexpr uint32_t TPR = ATTEND_THREADS / ROWS, EPT = HD / TPR;
@@ -648,7 +689,27 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
                 x += *(const f32x4 *)(ob + (v * 16 + i / (HD / 4)) * (HD + 4) + d) * f;
             }
             const uint64_t row = first + e.x, qh = head * G + e.y, at = row * a.q_heads + qh;
-            const bool none = span.end(e.x) <= span.begin(e.x);
+            bool none = span.end(e.x) <= span.begin(e.x);
+            if constexpr (MODE != ATTEND_ALONE)
+                if (!none && ms.x == -INFINITY) ms.x = ATTEND_LOWEST;
+            if constexpr (MODE == ATTEND_PREFIX) {
+                const uint64_t slot = at * a.stride + a.shared + part;
+                *(f32x4 *)(a.part_out + slot * HD + d) = x;
+                if (d == 0) a.part_sum[slot] = ms;
+                continue;
+            } else if constexpr (MODE == ATTEND_JOINED) {
+                if (a.parts == 1) {
+                    const uint64_t slot = at * a.stride + a.shared;
+                    for (uint32_t p = 0; p < a.shared_parts; p++)
+                        attend_add(ms, x, a.part_sum[slot + p], *(const f32x4 *)(a.part_out + (slot + p) * HD + d));
+                    attend_write<T>(a, row, qh, d, ms.x == -INFINITY, ms, x, LIFT);
+                } else {
+                    *(f32x4 *)(a.part_out + (at * a.stride + part) * HD + d) = x;
+                    if (d == 0) a.part_sum[at * a.stride + part] = ms;
+                    if (d == 0 && part == 0) a.part_count[at] = parts;
+                }
+                continue;
+            }
             if (parts == 1) attend_write<T>(a, row, qh, d, none, ms, x, LIFT);
             else if (a.joins) {
                 shared_store(a.part_out + (at * a.parts + part) * HD + d, float2{x[0], x[1]});
@@ -661,7 +722,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
             if (d == 0 && part == 0 && !a.joins) a.part_count[at] = parts | (none ? ATTEND_NONE : 0);
         }
     }
-    if (parts == 1 || !a.joins) return;
+    if (MODE != ATTEND_ALONE || parts == 1 || !a.joins) return;
     // The last of the block's parts to arrive joins them. Every wave's results are written before the arrival, and both
     // sides go past the caches that XCDs do not share.
     __builtin_amdgcn_s_waitcnt(ATTEND_STORED);
@@ -726,23 +787,26 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
 // Joins the parts of a row and head where they are more than ATTEND_FEW: one
 // workgroup each, a thread four columns of every PER-th part, all loaded before the
 // first is needed. Latency only: 4.2 us for 64 parts of 32 rows of 128.
-template <typename T, int FMT, int HD>
+template <typename T, int FMT, int HD, AttendMode MODE>
 __global__ void __launch_bounds__(ATTEND_THREADS) k_attend_join(AttendArgs a) {
     constexpr uint32_t COLS = HD / 4, PER = ATTEND_THREADS / COLS, AHEAD = 8;
     __shared__ float factor[ATTEND_MAX_PARTS], reduce[2][ATTEND_WAVES];
     __shared__ f32x4 partial[PER][COLS];
     const uint64_t at = blockIdx.x;
-    const uint32_t tid = threadIdx.x, count = a.part_count[at], n = min(count & ~ATTEND_NONE, a.parts);
-    if (n <= 1) return; // written already
+    constexpr bool JOINED = MODE == ATTEND_JOINED;
+    const uint32_t tid = threadIdx.x, count = a.part_count[at], own = min(count & ~ATTEND_NONE, a.parts);
+    if (own <= (JOINED ? 0 : 1)) return; // written already
+    const uint32_t n = own + (JOINED ? a.shared_parts : 0), stride = JOINED ? a.stride : a.parts;
     const uint32_t c = tid % COLS, p0 = tid / COLS;
-    const f32x4 *x = (const f32x4 *)(a.part_out + at * a.parts * HD) + c;
+    const f32x4 *x = (const f32x4 *)(a.part_out + at * stride * HD) + c;
+    const auto slot = [&](uint32_t p) { return JOINED && p >= own ? a.shared + (p - own) : p; };
     f32x4 ahead[AHEAD];
 #pragma unroll
     for (uint32_t j = 0; j < AHEAD; j++) {
         const uint32_t p = p0 + j * PER;
-        ahead[j] = x[(uint64_t)(p < n ? p : 0) * COLS];
+        ahead[j] = x[(uint64_t)slot(p < n ? p : 0) * COLS];
     }
-    const float2 ms = tid < n ? a.part_sum[at * a.parts + tid] : make_float2(-INFINITY, 0.0f);
+    const float2 ms = tid < n ? a.part_sum[at * stride + slot(tid)] : make_float2(-INFINITY, 0.0f);
     float most = group_max<64>(ms.x);
     if (tid % 64 == 0) reduce[0][tid / 64] = most;
     __syncthreads();
@@ -756,19 +820,20 @@ __global__ void __launch_bounds__(ATTEND_THREADS) k_attend_join(AttendArgs a) {
     f32x4 total = {0, 0, 0, 0};
 #pragma unroll
     for (uint32_t j = 0; j < AHEAD; j++)
-        if (p0 + j * PER < n) total += ahead[j] * factor[p0 + j * PER];
-    for (uint32_t p = p0 + AHEAD * PER; p < n; p += PER) total += x[(uint64_t)p * COLS] * factor[p];
+        if (p0 + j * PER < n && (!JOINED || factor[p0 + j * PER] != 0.0f)) total += ahead[j] * factor[p0 + j * PER];
+    for (uint32_t p = p0 + AHEAD * PER; p < n; p += PER)
+        if (!JOINED || factor[p] != 0.0f) total += x[(uint64_t)slot(p) * COLS] * factor[p]; // of no tokens: may be anything
     partial[p0][c] = total;
     __syncthreads();
     if (p0) return;
 #pragma unroll
     for (uint32_t j = 1; j < PER; j++) total += partial[j][c];
-    attend_write<T>(a, at / a.q_heads, at % a.q_heads, c * 4, count & ATTEND_NONE, make_float2(most, sum), total,
+    attend_write<T>(a, at / a.q_heads, at % a.q_heads, c * 4, JOINED ? most == -INFINITY : (count & ATTEND_NONE) != 0, make_float2(most, sum), total,
                     FMT == RL_F16 ? ATTEND_LIFT : 0.0f);
 }
 
 // Launches the kernel for queries of type T (attend_*.hip, one unit a type).
 template <typename T>
-void launch_attend(const AttendArgs &a, uint32_t format, bool two_tiles, uint32_t groups, hipStream_t s);
+void launch_attend(const AttendArgs &a, AttendMode mode, uint32_t format, bool two_tiles, uint32_t groups, hipStream_t s);
 
 }  // namespace rl

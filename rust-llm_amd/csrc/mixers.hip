@@ -10,7 +10,7 @@
 
 #include "attend.h"
 #include "delta_launch.h"
-#include "rl_runtime.h"
+#include "mix_args.h"
 
 using namespace rl;
 
@@ -68,32 +68,6 @@ struct rl_delta {
 
 namespace {
 
-constexpr uint32_t MAX_ROWS = 1u << 23; // a workgroup of 256 threads a row stays below 2^32 threads
-
-uint32_t type_bytes(uint32_t dtype) { return dtype == RL_F32 ? 4 : dtype == RL_F16 || dtype == RL_BF16 ? 2 : 1; }
-
-// What is wrong with a tensor argument of a call of `rows` rows, or null.
-const char *wrong(const rl_heads *h, uint32_t rows, bool written) {
-    if (!h) return "is null";
-    if (!h->data && rows) return "has no data";
-    if (h->dtype > RL_BF16) return "must be f32, f16 or bf16";
-    if (h->heads == 0 || h->dim == 0) return "has no heads or no values";
-    if ((uintptr_t)h->data % type_bytes(h->dtype)) return "is not aligned to its type";
-    if (written && h->heads > 1 && h->head_stride < h->dim) return "is written with overlapping heads";
-    if (written && rows > 1 && h->row_stride < h->dim) return "is written with overlapping rows";
-    return nullptr;
-}
-
-#define CHECK_HEADS(h, name, written) /* of a call's `rows` */                                                     \
-    do {                                                                                           \
-        if (const char *w = wrong(h, rows, written)) return fail(RL_ERR_ARGUMENT, std::string(name) + " " + w); \
-    } while (0)
-
-bool wide(const rl_heads *h) {
-    const uint64_t b = type_bytes(h->dtype);
-    return (uintptr_t)h->data % 16 == 0 && h->row_stride * b % 16 == 0 && h->head_stride * b % 16 == 0;
-}
-
 RotaryArgs rotary_args(const rl_rotary *r, bool inverse) {
     RotaryArgs a{};
     if (!r) return a;
@@ -113,14 +87,6 @@ void launch_rotary(const RotaryArgs &r, const int64_t *positions, uint32_t rows,
                            positions, a, b);
     else
         hipLaunchKernelGGL((k_rotary<TI, TO, V, false>), dim3(rows), dim3(ROTARY_THREADS), 0, s, r, positions, a, b);
-}
-
-// Calls f with a value of the element type.
-template <typename F>
-void with_type(uint32_t dtype, F f) {
-    if (dtype == RL_F32) f(float{});
-    else if (dtype == RL_F16) f(half_t{});
-    else f(bhalf_t{});
 }
 
 CacheRows cache_rows(const rl_heads *k, const rl_heads *v, uint32_t rows) {
@@ -185,16 +151,95 @@ uint32_t attend_least_parts(uint32_t tiles, uint32_t seqs) {
     return std::min(n, ATTEND_MAX_PARTS);
 }
 
+// Parts of a shared prefix at most: each of a row's columns is joined by one thread, which loads them one after the other.
+constexpr uint32_t SHARED_PARTS = 16;
+
+// The checks that the attention's calls have in common.
+int check_attention(const rl_attention *h, const rl_kv_cache *cache, const rl_heads *q, const rl_heads *out, uint32_t rows,
+                    const int32_t *starts, const int32_t *lens, uint32_t seqs, const int32_t *pages, uint32_t table_width,
+                    uint32_t max_len) {
+    if (!h) return fail(RL_ERR_ARGUMENT, "attention is null");
+    if (!cache) return fail(RL_ERR_ARGUMENT, "cache is null");
+    CHECK_HEADS(q, "q", false);
+    CHECK_HEADS(out, "out", true);
+    if (cache->device != h->device) return fail(RL_ERR_ARGUMENT, "the cache is on another device");
+    if (cache->args.heads != h->kv_heads || cache->args.dim != h->dim)
+        return fail(RL_ERR_ARGUMENT, "the cache has other heads or another dim than the handle");
+    if (q->heads != h->q_heads || q->dim != h->dim || out->heads != h->q_heads || out->dim != h->dim)
+        return fail(RL_ERR_ARGUMENT, "q and out must have the handle's heads and dim");
+    if (q->dtype != out->dtype) return fail(RL_ERR_ARGUMENT, "q and out differ in type");
+    if ((cache->format == RL_F16 && q->dtype == RL_BF16) || (cache->format == RL_BF16 && q->dtype == RL_F16))
+        return fail(RL_ERR_ARGUMENT, "an f16 cache takes f16 or f32 queries, a bf16 cache bf16 or f32");
+    if (rows > h->max_rows) return fail(RL_ERR_CAPACITY, "rows above the handle's max_rows");
+    if (max_len > h->max_len) return fail(RL_ERR_CAPACITY, "max_len above the handle's");
+    if (rows == 0) return RL_OK;
+    if (!lens || !pages || table_width == 0) return fail(RL_ERR_ARGUMENT, "lens and pages must be device pointers");
+    if (seqs == 0 || (!starts && seqs != rows)) return fail(RL_ERR_ARGUMENT, "without starts there is one row a sequence");
+    return RL_OK;
+}
+
+AttendArgs attend_args(const rl_attention *h, const rl_kv_cache *cache, const rl_heads *q, const rl_heads *out, float *lse,
+                       uint32_t rows, const int32_t *starts, const int32_t *lens, uint32_t seqs, const int32_t *pages,
+                       uint32_t table_width, float scale, uint32_t most_rows, uint32_t max_len) {
+    AttendArgs a{};
+    a.cache = cache->args;
+    a.q = q->data, a.out = out->data, a.lse = lse;
+    a.q_row = q->row_stride, a.q_head = q->head_stride;
+    a.out_row = out->row_stride, a.out_head = out->head_stride;
+    a.starts = starts, a.lens = lens, a.pages = pages;
+    a.rows = rows, a.seqs = seqs, a.q_heads = h->q_heads, a.table_width = table_width;
+    a.most_rows = !starts ? 1 : most_rows ? std::min(most_rows, rows) : rows;
+    a.max_len = max_len ? max_len : h->max_len;
+    a.scale = scale;
+    a.group = h->q_heads / h->kv_heads;
+    a.wide = wide(q) && wide(out);
+    a.part_out = h->part_out, a.part_sum = h->part_sum, a.part_count = h->part_count, a.arrived = h->arrived;
+    return a;
+}
+
+// Workgroups that the device holds at a time.
+uint64_t attend_held(const rl_heads *q, const rl_kv_cache *cache, const rl_attention *h, bool two) {
+    return CUS * attend_resident(type_bytes(q->dtype), cache->format, h->dim, two ? 2 : 1);
+}
+
+// The row blocks, and a call's columns of parts.
+uint64_t attend_blocks(AttendArgs &a, const rl_attention *h, bool two) {
+    const uint64_t expanded = (uint64_t)a.most_rows * a.group;
+    const uint32_t block_rows = two ? 32 : 16;
+    // A grid of the longest sequence's row blocks for every sequence, or of the sum of all. The second asks each workgroup to
+    // find its sequence, and is taken where it is less than half as large; the first can pass what a launch takes. 64
+    // sequences of 2048 tokens, 32 / 8 heads of 128 bf16, us, first / second: all with 64 rows 844 / 899, 21 of them (the
+    // others one) 509 / 374, one 361 / 133; eight with 9 rows 115 / 121.
+    const uint64_t longest = (expanded + block_rows - 1) / block_rows, sum = (uint64_t)a.rows * a.group / block_rows + a.seqs;
+    a.packed = sum * 2 < longest * a.seqs;
+    a.blocks = (uint32_t)(a.packed ? sum : longest);
+    return (uint64_t)(a.packed ? 1 : a.seqs) * h->kv_heads * a.blocks;
+}
+
+// The parts, where a row has `room` for that many partial results, and the workgroups. False if those are too many.
+bool attend_shape(AttendArgs &a, const rl_attention *h, uint64_t columns, uint64_t held, uint64_t room, uint32_t *groups) {
+    const uint64_t seen = a.window ? std::min<uint64_t>(a.max_len, (uint64_t)a.window + a.most_rows - 1) : a.max_len;
+    const uint32_t tiles = attend_tiles(seen);
+    uint64_t parts = std::max<uint64_t>(held / columns, attend_least_parts(tiles, a.seqs));
+    parts = std::max<uint64_t>(std::min(parts, std::min<uint64_t>(room, ATTEND_MAX_PARTS)), 1);
+    a.part_tiles = (uint32_t)((tiles + parts - 1) / parts);
+    a.part_tiles = (a.part_tiles + ATTEND_WAVES - 1) / ATTEND_WAVES * ATTEND_WAVES;
+    a.parts = (tiles + a.part_tiles - 1) / a.part_tiles;
+    a.group_inv = inverse_of(a.group), a.blocks_inv = inverse_of(a.blocks), a.heads_inv = inverse_of(h->kv_heads);
+    a.columns_inv = inverse_of(a.seqs * h->kv_heads), a.tiles_inv = inverse_of(a.part_tiles);
+    // Jobs (sequence, head and part) in eights, the row blocks of each eight together; or eight runs of row blocks at a time.
+    constexpr uint64_t RUNS = 8 * ATTEND_RUN;
+    const uint64_t n = a.packed ? (columns * a.parts + RUNS - 1) / RUNS * RUNS
+                                : ((uint64_t)a.seqs * h->kv_heads * a.parts + 7) / 8 * 8 * a.blocks;
+    *groups = (uint32_t)n;
+    return n <= 2 * MAX_ROWS - 1;
+}
+
 // Rows of a sequence from which chunks are faster than one token after the other (us, steps / chunks; 32 heads of 128 x
 // 128). While every workgroup of the chunks has a CU to itself they cost the same for any rows up to 64: one bf16
 // sequence of 12 rows 15.4 / 16.1, of 16 19.3 / 16.1; f32, more products, 16 rows 17.0 / 22.5, 24 rows 23.2 / 22.5. Beyond
 // that they wait for each other: 16 sequences of 16 rows 54.6 / 79, of 24 76.2 / 78.7, of 32 98.7 / 78.3.
 constexpr uint32_t DELTA_CHUNKED = 13, DELTA_CHUNKED_WIDE = 20, DELTA_CHUNKED_MANY = 25;
-
-int launched(const char *what) {
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? RL_OK : hip_fail(e, what);
-}
 
 }  // namespace
 
@@ -475,71 +520,69 @@ int rl_attention_rows(rl_attention *h, const rl_kv_cache *cache, const rl_heads 
                       uint32_t rows, const int32_t *starts, const int32_t *lens, uint32_t seqs, const int32_t *pages,
                       uint32_t table_width, float scale, uint32_t window, uint32_t most_rows, uint32_t max_len,
                       void *stream) {
-    if (!h) return fail(RL_ERR_ARGUMENT, "attention is null");
-    if (!cache) return fail(RL_ERR_ARGUMENT, "cache is null");
-    CHECK_HEADS(q, "q", false);
-    CHECK_HEADS(out, "out", true);
-    if (cache->device != h->device) return fail(RL_ERR_ARGUMENT, "the cache is on another device");
-    if (cache->args.heads != h->kv_heads || cache->args.dim != h->dim)
-        return fail(RL_ERR_ARGUMENT, "the cache has other heads or another dim than the handle");
-    if (q->heads != h->q_heads || q->dim != h->dim || out->heads != h->q_heads || out->dim != h->dim)
-        return fail(RL_ERR_ARGUMENT, "q and out must have the handle's heads and dim");
-    if (q->dtype != out->dtype) return fail(RL_ERR_ARGUMENT, "q and out differ in type");
-    if ((cache->format == RL_F16 && q->dtype == RL_BF16) || (cache->format == RL_BF16 && q->dtype == RL_F16))
-        return fail(RL_ERR_ARGUMENT, "an f16 cache takes f16 or f32 queries, a bf16 cache bf16 or f32");
-    if (rows > h->max_rows) return fail(RL_ERR_CAPACITY, "rows above the handle's max_rows");
-    if (max_len > h->max_len) return fail(RL_ERR_CAPACITY, "max_len above the handle's");
+    if (const int rc = check_attention(h, cache, q, out, rows, starts, lens, seqs, pages, table_width, max_len)) return rc;
     if (rows == 0) return RL_OK;
-    if (!lens || !pages || table_width == 0) return fail(RL_ERR_ARGUMENT, "lens and pages must be device pointers");
-    if (seqs == 0 || (!starts && seqs != rows)) return fail(RL_ERR_ARGUMENT, "without starts there is one row a sequence");
     if (window > 0x7FFFFFFFu) window = 0; // no length is above it
     DeviceGuard guard(h->device);
     if (!guard.ok) return fail(RL_ERR_DEVICE, "cannot select the handle's device");
-    AttendArgs a{};
-    a.cache = cache->args;
-    a.q = q->data, a.out = out->data, a.lse = lse;
-    a.q_row = q->row_stride, a.q_head = q->head_stride;
-    a.out_row = out->row_stride, a.out_head = out->head_stride;
-    a.starts = starts, a.lens = lens, a.pages = pages;
-    a.rows = rows, a.seqs = seqs, a.q_heads = h->q_heads, a.table_width = table_width, a.window = window;
-    a.most_rows = !starts ? 1 : most_rows ? std::min(most_rows, rows) : rows;
-    a.max_len = max_len ? max_len : h->max_len;
-    a.scale = scale;
-    a.group = h->q_heads / h->kv_heads;
-    a.wide = wide(q) && wide(out);
-    a.part_out = h->part_out, a.part_sum = h->part_sum, a.part_count = h->part_count, a.arrived = h->arrived;
+    AttendArgs a = attend_args(h, cache, q, out, lse, rows, starts, lens, seqs, pages, table_width, scale, most_rows, max_len);
+    a.window = window;
     const uint64_t expanded = (uint64_t)a.most_rows * a.group;
     const bool two = attend_two(cache->format, h->dim, (expanded + 15) / 16, (uint64_t)seqs * h->kv_heads);
-    const uint32_t block_rows = two ? 32 : 16;
-    // A grid of the longest sequence's row blocks for every sequence, or of the sum of all. The second asks each workgroup to
-    // find its sequence, and is taken where it is less than half as large; the first can pass what a launch takes. 64
-    // sequences of 2048 tokens, 32 / 8 heads of 128 bf16, us, first / second: all with 64 rows 844 / 899, 21 of them (the
-    // others one) 509 / 374, one 361 / 133; eight with 9 rows 115 / 121.
-    const uint64_t longest = (expanded + block_rows - 1) / block_rows, sum = (uint64_t)rows * a.group / block_rows + seqs;
-    a.packed = sum * 2 < longest * seqs;
-    a.blocks = (uint32_t)(a.packed ? sum : longest);
-    const uint64_t columns = (uint64_t)(a.packed ? 1 : seqs) * h->kv_heads * a.blocks;
-    const uint64_t seen = window ? std::min<uint64_t>(a.max_len, (uint64_t)window + a.most_rows - 1) : a.max_len;
-    const uint32_t tiles = attend_tiles(seen);
-    const uint64_t room = std::min<uint64_t>(h->slots / ((uint64_t)rows * h->q_heads), ATTEND_MAX_PARTS);
-    const uint64_t held = CUS * attend_resident(type_bytes(q->dtype), cache->format, h->dim, two ? 2 : 1);
-    uint64_t parts = std::max<uint64_t>(held / columns, attend_least_parts(tiles, seqs));
-    parts = std::max<uint64_t>(std::min(parts, room), 1);
-    a.part_tiles = (uint32_t)((tiles + parts - 1) / parts);
-    a.part_tiles = (a.part_tiles + ATTEND_WAVES - 1) / ATTEND_WAVES * ATTEND_WAVES;
-    a.parts = (tiles + a.part_tiles - 1) / a.part_tiles;
+    uint32_t groups;
+    if (!attend_shape(a, h, attend_blocks(a, h, two), attend_held(q, cache, h, two), h->slots / ((uint64_t)rows * h->q_heads), &groups))
+        return fail(RL_ERR_CAPACITY, "too many sequences times row blocks in a call");
     a.joins = a.parts <= ATTEND_FEW;
-    a.group_inv = inverse_of(a.group), a.blocks_inv = inverse_of(a.blocks), a.heads_inv = inverse_of(h->kv_heads);
-    a.columns_inv = inverse_of(seqs * h->kv_heads), a.tiles_inv = inverse_of(a.part_tiles);
-    // Jobs (sequence, head and part) in eights, the row blocks of each eight together; or eight runs of row blocks at a time.
-    constexpr uint64_t RUNS = 8 * ATTEND_RUN;
-    const uint64_t groups = a.packed ? (columns * a.parts + RUNS - 1) / RUNS * RUNS
-                                     : ((uint64_t)seqs * h->kv_heads * a.parts + 7) / 8 * 8 * a.blocks;
-    if (groups > 2 * MAX_ROWS - 1) return fail(RL_ERR_CAPACITY, "too many sequences times row blocks in a call");
     with_type(q->dtype, [&](auto t) {
-        launch_attend<decltype(t)>(a, cache->format, two, (uint32_t)groups, static_cast<hipStream_t>(stream));
+        launch_attend<decltype(t)>(a, ATTEND_ALONE, cache->format, two, groups, static_cast<hipStream_t>(stream));
     });
     return launched("rl_attention_rows launch");
+}
+
+int rl_attention_shared(rl_attention *h, const rl_kv_cache *cache, const rl_heads *q, const rl_heads *out, float *lse,
+                        uint32_t rows, const int32_t *starts, const int32_t *lens, uint32_t seqs, const int32_t *pages,
+                        uint32_t table_width, const int32_t *group_starts, const int32_t *prefix_lens, uint32_t groups,
+                        const int32_t *prefix_pages, uint32_t prefix_width, float scale, uint32_t most_rows,
+                        uint32_t max_len, uint32_t max_prefix, void *stream) {
+    if (const int rc = check_attention(h, cache, q, out, rows, starts, lens, seqs, pages, table_width, max_len)) return rc;
+    if (max_prefix > h->max_len) return fail(RL_ERR_CAPACITY, "max_prefix above the handle's max_len");
+    if (rows == 0) return RL_OK;
+    if (!group_starts || !prefix_lens || !prefix_pages || prefix_width == 0 || groups == 0)
+        return fail(RL_ERR_ARGUMENT, "group_starts, prefix_lens and prefix_pages must be device pointers");
+    if (groups > seqs) return fail(RL_ERR_ARGUMENT, "more groups than sequences");
+    // Partial results that a row has room for: at least one for its prefix.
+    const uint64_t room = h->slots / ((uint64_t)rows * h->q_heads);
+    if (room == 0) return fail(RL_ERR_CAPACITY, "rows times heads above 2^20 have no room for a prefix's results");
+    DeviceGuard guard(h->device);
+    if (!guard.ok) return fail(RL_ERR_DEVICE, "cannot select the handle's device");
+    AttendArgs own = attend_args(h, cache, q, out, lse, rows, starts, lens, seqs, pages, table_width, scale, most_rows, max_len);
+    const uint64_t expanded = (uint64_t)own.most_rows * own.group;
+    const bool two = attend_two(cache->format, h->dim, (expanded + 15) / 16, (uint64_t)seqs * h->kv_heads);
+    AttendArgs shared = attend_args(h, cache, q, out, lse, rows, starts, prefix_lens, groups, prefix_pages, prefix_width, scale,
+                                    rows, max_prefix);
+    shared.group_starts = group_starts, shared.group_end = seqs;
+    shared.most_rows = rows;
+    const bool shared_two = attend_two(cache->format, h->dim, ((uint64_t)rows * own.group + 15) / 16, (uint64_t)groups * h->kv_heads);
+    uint32_t own_groups, shared_groups;
+    // The prefix's parts are joined by each row's own workgroup, so they are few. Room is theirs first: a sequence's own
+    // tokens in one part need none.
+    shared.packed = 1;
+    const uint32_t block_rows = shared_two ? 32 : 16;
+    shared.blocks = (uint32_t)((uint64_t)rows * shared.group / block_rows + groups);
+    bool fits = attend_shape(shared, h, (uint64_t)h->kv_heads * shared.blocks, attend_held(q, cache, h, shared_two),
+                             std::min<uint64_t>(room, SHARED_PARTS), &shared_groups);
+    const uint64_t own_room = room - shared.parts > 1 ? std::min<uint64_t>(room - shared.parts, ATTEND_MAX_PARTS - SHARED_PARTS) : 1;
+    fits = fits && attend_shape(own, h, attend_blocks(own, h, two), attend_held(q, cache, h, two), own_room, &own_groups);
+    if (!fits) return fail(RL_ERR_CAPACITY, "too many sequences times row blocks in a call");
+    own.shared = shared.shared = own.parts > 1 ? own.parts : 0;
+    own.shared_parts = shared.shared_parts = shared.parts;
+    own.stride = shared.stride = own.shared + shared.parts;
+    with_type(q->dtype, [&](auto t) {
+        const hipStream_t s = static_cast<hipStream_t>(stream);
+        launch_attend<decltype(t)>(shared, ATTEND_PREFIX, cache->format, shared_two, shared_groups, s);
+        launch_attend<decltype(t)>(own, ATTEND_JOINED, cache->format, two, own_groups, s);
+    });
+    return launched("rl_attention_shared launch");
 }
 
 int rl_delta_create(int device, uint32_t max_rows, uint32_t max_seqs, uint32_t key_heads, uint32_t value_heads,

@@ -1,6 +1,7 @@
 """Python bindings (ctypes) for the token mixers of librl_sampler.so
 (include/rl_mixers.h): rotary positions, the paged key-value cache, attention of
-new tokens over it, and the gated delta rule.
+new tokens over it, by themselves or behind shared prefixes, the gated delta rule, the
+short causal convolution and the selective state space scan.
 
 As in rl_sampler.py this only marshals arguments: tensors are torch tensors on the
 handle's device, [rows][heads][dim] with the last axis contiguous and any strides
@@ -18,6 +19,7 @@ from rl_sampler import _check, _u32, _u64, _vp
 
 TYPES = {"f32": 0, "f16": 1, "bf16": 2, "i8": 3, "f8": 4}
 LAYOUTS = {"half": 0, "interleaved": 1}
+ACTIVATIONS = {"none": 0, "silu": 1}
 SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 
 _HEADS = struct.Struct("=QQQIIII")  # rl_heads
@@ -55,7 +57,15 @@ def lib():
         L.rl_delta_create.argtypes = [_i32, _u32, _u32, _u32, _u32, _u32, _u32, out]
         L.rl_delta_rows.argtypes = [_vp, heads, heads, heads, heads, _vp, _u64, _vp, _u64, _vp, _u64, _vp, _vp, _vp,
                                     _u32, _u32, _f32, _f32, _u32, _vp]
-        for name in ("rl_rotary_destroy", "rl_kv_cache_destroy", "rl_attention_destroy", "rl_delta_destroy"):
+        L.rl_attention_shared.argtypes = [_vp, _vp, heads, heads, _vp, _u32, _vp, _vp, _u32, _vp, _u32, _vp, _vp, _u32,
+                                          _vp, _u32, _f32, _u32, _u32, _u32, _vp]
+        L.rl_conv_create.argtypes = [_i32, _u32, _u32, _vp, _vp, _u32, out]
+        L.rl_conv_rows.argtypes = [_vp, heads, heads, _vp, _u64, _vp, _vp, _vp, _u32, _u32, _vp]
+        L.rl_scan_create.argtypes = [_i32, _u32, _u32, _u32, _u32, _u32, _vp, _vp, _vp, out]
+        L.rl_scan_rows.argtypes = [_vp, heads, heads, heads, heads, heads, heads, _vp, _u64, _vp, _vp, _vp, _u32, _u32,
+                                   _i32, _u32, _vp]
+        for name in ("rl_rotary_destroy", "rl_kv_cache_destroy", "rl_attention_destroy", "rl_delta_destroy",
+                     "rl_conv_destroy", "rl_scan_destroy"):
             f = getattr(L, name)
             f.argtypes, f.restype = [_vp], None
         _bound = L
@@ -87,6 +97,39 @@ def _heads(t, device=None):
     if one != 1 or t.dtype not in _codes:
         raise ValueError("a tensor of f32, f16 or bf16 whose last axis is contiguous")
     return _pack(t.data_ptr(), rows, per, heads, dim, _codes[t.dtype], 0)
+
+
+def _channels(t, device):
+    """A tensor [rows][channels] as a packed rl_heads of one head."""
+    if t.get_device() != device:
+        raise _elsewhere(t, device)
+    _, channels = t.shape
+    rows, one = t.stride()
+    if (one != 1 and channels > 1) or t.dtype not in _codes:
+        raise ValueError("a tensor of f32, f16 or bf16 whose last axis is contiguous")
+    return _pack(t.data_ptr(), rows, 0, 1, channels, _codes[t.dtype], 0)
+
+
+def _states(states, dtype, shape, device):
+    """The address of a pool of states."""
+    if states.get_device() != device:
+        raise _elsewhere(states, device)
+    if states.dtype != dtype or not states.is_contiguous() or states.shape[1:] != shape:
+        raise ValueError("states are contiguous %s [slots]%s" % (dtype, list(shape)))
+    return states.data_ptr()
+
+
+def _host(t, shape):
+    """A contiguous f32 copy of weights on the host, or None."""
+    if t is None:
+        return None
+    if t.shape != shape:
+        raise ValueError("weights of another shape than %s" % list(shape))
+    return t.detach().to("cpu", torch.float32).contiguous()
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def _index(t, dtype, count, device):
@@ -213,6 +256,25 @@ class DeviceAttention(_Handle):
             self.scale if scale is None else scale, window, most_rows, max_len, _stream(device, stream)))
 
 
+    def shared(self, cache, q, out, lens, pages, groups, prefix_lens, prefix_pages, starts=None, lse=None, scale=None,
+               most_rows=0, max_len=0, max_prefix=0, stream=None):
+        """As rows(), where the sequences groups[g] .. groups[g + 1] (int32
+        [prefixes + 1]) have the prefix_lens[g] (int32) tokens of prefix_pages[g] (int32
+        [prefixes][width]) before their own: lens and pages are of their own tokens."""
+        rows, seqs, width, device = q.shape[0], pages.shape[0], pages.shape[1], self.device
+        count, wide = prefix_pages.shape
+        if out.shape != q.shape:
+            raise ValueError("out has another shape than q")
+        _check(lib().rl_attention_shared(
+            self.h, cache.h, _heads(q, device), _heads(out, device),
+            None if lse is None else _index(lse, torch.float32, rows * self.q_heads, device), rows,
+            None if starts is None else _index(starts, torch.int32, seqs + 1, device),
+            _index(lens, torch.int32, seqs, device), seqs, _index(pages, torch.int32, seqs * width, device), width,
+            _index(groups, torch.int32, count + 1, device), _index(prefix_lens, torch.int32, count, device), count,
+            _index(prefix_pages, torch.int32, count * wide, device), wide, self.scale if scale is None else scale,
+            most_rows, max_len, max_prefix, _stream(device, stream)))
+
+
 class DeviceDelta(_Handle):
     """rl_delta_create / rl_delta_rows: the gated delta rule over a pool of f32
     states."""
@@ -251,3 +313,66 @@ class DeviceDelta(_Handle):
             _index(slots_in, torch.int32, seqs, device), _index(slots_out, torch.int32, seqs, device),
             None if starts is None else _index(starts, torch.int32, seqs + 1, device), rows, seqs,
             self.scale if scale is None else scale, eps if normalise else -1.0, most_rows, _stream(device, stream)))
+
+
+class DeviceConv(_Handle):
+    """rl_conv_create / rl_conv_rows: the short causal convolution of every channel,
+    over a pool of states."""
+
+    _destroy = "rl_conv_destroy"
+
+    def __init__(self, weight, bias=None, activation="silu", device=0):
+        """weight [channels][width], bias [channels] if any: copied."""
+        channels, width = weight.shape
+        w, b, h = _host(weight, weight.shape), _host(bias, (channels,)), _vp()
+        _check(lib().rl_conv_create(device, channels, width, w.data_ptr(), _at(b), ACTIVATIONS[activation],
+                                    ctypes.byref(h)))
+        self.h, self.device, self.state = h, device, (width - 1, channels)
+
+    def rows(self, x, out, states, slots_in, slots_out, starts=None, stream=None):
+        """x, out [rows][channels]; states [slots][width - 1][channels] of x's type,
+        contiguous; slots_in, slots_out int32 [seqs] (negative: none; the slots written
+        distinct); starts int32 [seqs + 1] (None: one row a sequence)."""
+        rows, seqs, device = x.shape[0], slots_in.shape[0], self.device
+        if out.shape != x.shape:
+            raise ValueError("out has another shape than x")
+        _check(lib().rl_conv_rows(
+            self.h, _channels(x, device), _channels(out, device), _states(states, x.dtype, self.state, device),
+            states.shape[0], _index(slots_in, torch.int32, seqs, device), _index(slots_out, torch.int32, seqs, device),
+            None if starts is None else _index(starts, torch.int32, seqs + 1, device), rows, seqs,
+            _stream(device, stream)))
+
+
+class DeviceScan(_Handle):
+    """rl_scan_create / rl_scan_rows: the selective state space scan over a pool of f32
+    states."""
+
+    _destroy = "rl_scan_destroy"
+
+    def __init__(self, max_rows, max_seqs, a, groups=1, skip=None, dt_bias=None, device=0):
+        """a [channels][state_dim], skip and dt_bias [channels] if any: copied."""
+        channels, state = a.shape
+        decay, d, bias, h = _host(a, a.shape), _host(skip, (channels,)), _host(dt_bias, (channels,)), _vp()
+        _check(lib().rl_scan_create(device, max_rows, max_seqs, channels, groups, state, decay.data_ptr(), _at(d),
+                                    _at(bias), ctypes.byref(h)))
+        self.h, self.device, self.state = h, device, (channels, state)
+
+    def rows(self, x, dt, b, c, out, states, slots_in, slots_out, starts=None, z=None, softplus=True, most_rows=0,
+             stream=None):
+        """x, dt, out and z (if any) [rows][channels]; b, c [rows][groups][state_dim];
+        states f32 [slots][channels][state_dim], contiguous; slots_in, slots_out int32
+        [seqs] (negative: none; the slots written distinct); starts int32 [seqs + 1]
+        (None: one row a sequence)."""
+        rows, seqs, device = x.shape[0], slots_in.shape[0], self.device
+        for t in (dt, b, c, out):
+            if t.shape[0] != rows:
+                raise ValueError("the tensors of a call have one row a token")
+        if z is not None and z.shape[0] != rows:
+            raise ValueError("the tensors of a call have one row a token")
+        _check(lib().rl_scan_rows(
+            self.h, _channels(x, device), _channels(dt, device), None if z is None else _channels(z, device),
+            _heads(b, device), _heads(c, device), _channels(out, device),
+            _states(states, torch.float32, self.state, device), states.shape[0],
+            _index(slots_in, torch.int32, seqs, device), _index(slots_out, torch.int32, seqs, device),
+            None if starts is None else _index(starts, torch.int32, seqs + 1, device), rows, seqs, int(softplus),
+            most_rows, _stream(device, stream)))
