@@ -22,7 +22,7 @@ struct ConvArgs {
     const int32_t *slots_in, *slots_out, *starts;
     uint32_t rows, seqs, channels;
     uint32_t columns; // waves that a row takes
-    uint32_t shift;   // rows of a run: 2^shift, at least W - 1
+    RowBlocks runs;   // at least W - 1 rows
 };
 
 constexpr uint32_t CONV_MAX_WIDTH = 8, CONV_LANES = 64;
@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(CONV_LANES) k_conv(ConvArgs a) {
     constexpr int V = WIDE ? 16 / sizeof(T) : 4, AHEAD = 4;
     using Raw = vec<T, V>;
     const uint32_t block = blockIdx.x / a.columns, column = blockIdx.x - block * a.columns, lane = threadIdx.x;
-    const RowBlock r = find_block(a.starts, a.rows, a.seqs, a.shift, block);
+    const RowBlock r = find_block(a.starts, a.rows, a.seqs, a.runs, block);
     if (!r.used) return;
     const auto channel = [&](int i) { return column * 64 * V + (WIDE ? lane * V + i : lane + 64 * i); };
     if (channel(0) >= a.channels) return;
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(CONV_LANES) k_conv(ConvArgs a) {
         for (int i = 0; i < V; i++) v[i] = (T)x;
         return v;
     };
-    const uint32_t t0 = r.block << a.shift, count = min(r.rows - t0, 1u << a.shift); // t0 is 0 where there are no rows
+    const uint32_t t0 = r.block * a.runs.size, count = min(r.rows - t0, a.runs.size); // t0 is 0 where there are no rows
     const T *x = (const T *)a.x + (uint64_t)r.begin * a.x_row;
     const int32_t in = t0 ? -1 : a.slots_in[r.seq];
     // What the sequence's state holds in row j.

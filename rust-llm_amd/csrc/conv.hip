@@ -21,7 +21,7 @@ namespace {
 
 // Rows of a run: 32, which reads W - 1 of 35 twice, where that leaves two waves a SIMD or more; else 8, the least that holds
 // the longest state.
-constexpr uint32_t CONV_LONG = 5, CONV_SHORT = 3, CONV_WAVES = 2048;
+constexpr uint32_t CONV_LONG = 32, CONV_SHORT = 8, CONV_WAVES = 2048;
 
 template <typename T, int W, bool WIDE>
 void launch_conv(const ConvArgs &a, uint32_t blocks, bool silu, hipStream_t s) {
@@ -118,8 +118,8 @@ int rl_conv_rows(rl_conv *h, const rl_heads *x, const rl_heads *out, void *state
     const bool vectors = wide(x) && wide(out) && (uintptr_t)states % 16 == 0 && h->channels % vector == 0;
     const uint32_t per = CONV_LANES * (vectors ? vector : 4);
     a.columns = (h->channels + per - 1) / per;
-    a.shift = (uint64_t)(rows >> CONV_LONG) * a.columns >= CONV_WAVES ? CONV_LONG : CONV_SHORT;
-    const uint64_t blocks = (uint64_t)row_blocks(rows, seqs, a.shift) * a.columns;
+    a.runs = row_blocks((uint64_t)(rows / CONV_LONG) * a.columns >= CONV_WAVES ? CONV_LONG : CONV_SHORT);
+    const uint64_t blocks = (uint64_t)row_block_count(rows, seqs, a.runs.size) * a.columns;
     if (blocks > 1u << 25) return fail(RL_ERR_CAPACITY, "too many rows times channels in a call");
     with_type(x->dtype, [&](auto t) {
         with_width(h->width, [&](auto w) {

@@ -21,7 +21,7 @@ struct ScanArgs {
     uint32_t softplus; // whether steps are softplus(dt + bias), else dt + bias
     uint32_t wide;     // whether four values of b and c are one aligned vector
     uint32_t columns;  // workgroups that a row (prompts: a piece) takes
-    uint32_t shift;    // prompts: tokens of a piece, 2^shift; 31 for whole sequences
+    RowBlocks pieces;  // prompts: tokens of a piece, 0 for whole sequences
     // Pieces of sequences that have several: ends[slot] is a state as the lanes hold it, steps[slot][channel] the sum of a
     // piece's steps. A sequence's slots begin at scan_slot; slot 0 of a sequence has its first state and piece i's end from
     // zeros is in slot i + 1.
@@ -30,18 +30,20 @@ struct ScanArgs {
 
 constexpr uint32_t SCAN_THREADS = 256, SCAN_WAVES = 4;
 
-// Slots of a sequence of more than 2^shift rows, of which it needs one a piece.
-__device__ inline uint64_t scan_slot(uint32_t begin, uint32_t shift) { return 2 * (uint64_t)(begin >> shift); }
-inline uint64_t scan_slots(uint64_t rows, uint32_t shift) { return 2 * (rows >> shift) + 2; }
+// The first slot of a sequence of more rows than a piece has; it needs one slot a piece, which are at most twice as many as
+// whole pieces lie between its first row and the next sequence's.
+__device__ inline uint64_t scan_slot(uint32_t begin, RowBlocks pieces) { return 2 * (uint64_t)split_by(begin, pieces.size, pieces.inv).x; }
+inline uint64_t scan_slots(uint64_t pieces) { return 2 * pieces + 2; } // of a call of that many whole pieces
 
 // ln(1 + e^v), to f32's precision for every v.
 __device__ inline float soft_plus(float v) {
     constexpr float L = 1.44269504088896341f, LOW = 1.92596299e-8f, LN2 = 0.693147180559945309f;
     const float m = -fabsf(v), p = m * L;
-    const float e = __builtin_amdgcn_exp2f(p), t = p > -126.0f ? fmaf(e, (fmaf(m, L, -p) + m * LOW) * LN2, e) : e;
-    // ln(1 + t) by the rounded sum u and what the rounding took: ln(u) + (1 + t - u) / u
+    const float e = __builtin_amdgcn_exp2f(p), t = fmaf(e, (fmaf(m, L, -p) + m * LOW) * LN2, e);
+    // ln(1 + t) by the rounded sum u and what the rounding took, at most 2^-24: ln(u) + (1 + t - u) / u. The last division
+    // by 1 to 2 is left out, which costs at most a unit in the last place.
     const float u = 1.0f + t;
-    return fmaxf(v, 0.0f) + fmaf(__builtin_amdgcn_logf(u), LN2, (t - (u - 1.0f)) * __builtin_amdgcn_rcpf(u));
+    return fmaxf(v, 0.0f) + fmaf(__builtin_amdgcn_logf(u), LN2, t - (u - 1.0f));
 }
 
 template <typename T>
@@ -117,18 +119,19 @@ __global__ void __launch_bounds__(SCAN_THREADS) k_scan(ScanArgs a) {
     __shared__ __attribute__((aligned(16))) float staged[2][TILE][SIDES][N];
     const uint32_t block = blockIdx.x / a.columns, column = blockIdx.x - block * a.columns, tid = threadIdx.x;
     RowBlock r;
-    if (a.shift == 31) { // whole sequences
+    const bool whole = a.pieces.size == 0; // sequences
+    if (whole) {
         r.seq = block, r.block = 0, r.begin = block, r.rows = 1;
         if (a.starts) {
             r.begin = (uint32_t)min(max(a.starts[block], 0), (int32_t)a.rows);
             r.rows = max(min(max(a.starts[block + 1], 0), (int32_t)a.rows) - (int32_t)r.begin, 0);
         }
     } else {
-        r = find_block(a.starts, a.rows, a.seqs, a.shift, block);
+        r = find_block(a.starts, a.rows, a.seqs, a.pieces, block);
         if (!r.used) return;
     }
-    const uint32_t t0 = r.block << a.shift, count = min(r.rows - t0, 1u << a.shift);
-    const bool several = r.rows > 1u << a.shift, last = t0 + count == r.rows;
+    const uint32_t t0 = r.block * a.pieces.size, count = whole ? r.rows : min(r.rows - t0, a.pieces.size);
+    const bool several = count < r.rows, last = t0 + count == r.rows;
     if (!OUT && last) return;
     const uint32_t tiles = a.columns / a.groups; // of a group
     const uint32_t group = column / tiles, ch = (column - group * tiles) * (SCAN_THREADS / L) + tid / L;
@@ -139,7 +142,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) k_scan(ScanArgs a) {
         return a.ends + (((slot * a.columns + column) * (S / 4) + i / 4) * SCAN_THREADS + tid) * 4;
     };
     const auto state = [&](int32_t slot) { return a.states + ((uint64_t)(uint32_t)slot * a.channels + channel) * a.state; };
-    const uint64_t slot0 = scan_slot(r.begin, a.shift);
+    const uint64_t slot0 = whole ? 0 : scan_slot(r.begin, a.pieces);
     float h[S], a2[S];
 #pragma unroll
     for (int i = 0; i < S; i += 4) {
@@ -299,8 +302,8 @@ void launch_scan_steps(const ScanArgs &a, hipStream_t s) {
 
 template <typename T, int S, int L>
 void launch_scan_of(const ScanArgs &a, hipStream_t s) {
-    const dim3 grid((a.shift == 31 ? a.seqs : row_blocks(a.rows, a.seqs, a.shift)) * a.columns);
-    if (a.shift != 31) hipLaunchKernelGGL((k_scan<T, S, L, SCAN_ENDS>), grid, dim3(SCAN_THREADS), 0, s, a);
+    const dim3 grid((a.pieces.size ? row_block_count(a.rows, a.seqs, a.pieces.size) : a.seqs) * a.columns);
+    if (a.pieces.size) hipLaunchKernelGGL((k_scan<T, S, L, SCAN_ENDS>), grid, dim3(SCAN_THREADS), 0, s, a);
     hipLaunchKernelGGL((k_scan<T, S, L, SCAN_OUTPUTS>), grid, dim3(SCAN_THREADS), 0, s, a);
 }
 

@@ -29,16 +29,15 @@ namespace {
 
 // Rows of a sequence up to which one token after the other is the faster form.
 constexpr uint32_t SCAN_SHORT = 16;
-// Waves that pieces are made for: two and a half a SIMD, of which those of a short sequence end early. Pieces of fewer than
-// 2^SCAN_LEAST tokens would wait more for their first state than they compute.
-constexpr uint64_t SCAN_FILL = 2560;
-constexpr uint32_t SCAN_LEAST = 6;
+// Workgroups that pieces are made for, and the fewest tokens of one: shorter ones would wait more for their first state than
+// they compute.
+constexpr uint64_t SCAN_FILL = 1024;
+constexpr uint32_t SCAN_LEAST = 64;
 
-// Tokens of a piece, as a shift.
-uint32_t piece_shift(uint64_t rows, uint32_t columns) {
-    uint32_t shift = SCAN_LEAST;
-    while (shift < 31 && (rows * columns * SCAN_WAVES >> shift) > SCAN_FILL) shift++;
-    return shift;
+// Tokens of a piece.
+uint32_t piece_size(uint64_t rows, uint32_t columns) {
+    const uint64_t pieces = std::max<uint64_t>(SCAN_FILL / columns, 1);
+    return (uint32_t)std::max<uint64_t>((rows + pieces - 1) / pieces, SCAN_LEAST);
 }
 
 }  // namespace
@@ -64,8 +63,7 @@ int rl_scan_create(int device, uint32_t max_rows, uint32_t max_seqs, uint32_t ch
     h->max_rows = max_rows, h->max_seqs = max_seqs, h->channels = channels, h->groups = groups, h->state = state_dim;
     const uint32_t each = scan_each(state_dim), per = SCAN_THREADS / scan_lanes(state_dim, each);
     h->columns = groups * ((channels / groups + per - 1) / per);
-    // A call's pieces are at most 2^-SCAN_LEAST of its rows, and at most what fills the device.
-    h->slots = 2 * std::min<uint64_t>(max_rows >> SCAN_LEAST, SCAN_FILL / (h->columns * SCAN_WAVES)) + 2;
+    h->slots = scan_slots(std::min<uint64_t>(max_rows / SCAN_LEAST, std::max<uint64_t>(SCAN_FILL / h->columns, 1)));
     const size_t size = (size_t)channels * state_dim, all = size + 2 * (size_t)channels;
     float *laid = new (std::nothrow) float[all];
     if (!laid) {
@@ -144,10 +142,10 @@ int rl_scan_rows(rl_scan *h, const rl_heads *x, const rl_heads *dt, const rl_hea
         a.columns = (h->channels + per - 1) / per;
     } else {
         a.columns = h->columns;
-        a.shift = piece_shift(rows, h->columns);
-        if (most <= 1u << a.shift) a.shift = 31;
+        const uint32_t size = piece_size(rows, h->columns);
+        if (most > size) a.pieces = row_blocks(size);
     }
-    const uint64_t blocks = (uint64_t)(steps || a.shift == 31 ? seqs : row_blocks(rows, seqs, a.shift)) * a.columns;
+    const uint64_t blocks = (uint64_t)(steps || !a.pieces.size ? seqs : row_block_count(rows, seqs, a.pieces.size)) * a.columns;
     if (blocks > MAX_ROWS) return fail(RL_ERR_CAPACITY, "too many sequences times channels in a call");
     with_type(x->dtype, [&](auto t) {
         if (steps) launch_scan_steps<decltype(t)>(a, static_cast<hipStream_t>(stream));
