@@ -138,7 +138,7 @@ typedef struct rl_attention rl_attention;
 /* Workspace for calls of up to max_rows query rows over caches of kv_heads heads
  * and up to max_len tokens a sequence: 8 bytes a row and head, and 4 D + 8 bytes for
  * each partial result (D: dim rounded up to 64, 128 or 256), of which there are about
- * max_rows * q_heads * min(max_len / 1536 + 1, 256), at most 2^20, at least 24576.
+ * max_rows * q_heads * min(max_len / 1536 + 1, 256), at most 2^20, at least 2^15.
  * q_heads: a multiple of kv_heads; max_rows * q_heads at most 2^23. */
 int rl_attention_create(int device, uint32_t max_rows, uint32_t q_heads, uint32_t kv_heads, uint32_t dim,
                         uint32_t max_len, rl_attention **out);
@@ -249,7 +249,7 @@ typedef struct rl_scan rl_scan;
 /* a [channels][state_dim] (negative in use), skip and dt_bias [channels] (or NULL:
  * zeros) f32 on the host, copied. state_dim 4 to 256, a multiple of 4; channels a
  * multiple of groups, at most 2^20. Workspace for calls of up to max_rows tokens in up to
- * max_seqs sequences: at most 22 MB and two states more. */
+ * max_seqs sequences: at most 34 MB and four states. */
 int rl_scan_create(int device, uint32_t max_rows, uint32_t max_seqs, uint32_t channels, uint32_t groups,
                    uint32_t state_dim, const float *a, const float *skip, const float *dt_bias, rl_scan **out);
 void rl_scan_destroy(rl_scan *scan);

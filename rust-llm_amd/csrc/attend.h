@@ -82,6 +82,7 @@ inline bool attend_two(uint32_t format, uint32_t dim, uint64_t count, uint64_t c
 // Workgroups of k_attend that share a CU: as many as its registers allow without spills.
 constexpr int attend_resident(uint32_t query_bytes, uint32_t format, uint32_t dim, int row_tiles) {
     const bool eight = format == RL_I8 || format == RL_F8;
+    if (row_tiles == 4 || (row_tiles == 2 && dim > 128)) return 1;
     switch (attend_dim(dim)) {
     case 64: return row_tiles == 1 ? 3 : 2;
     case 128: return row_tiles == 1 ? (eight && query_bytes == 2 ? 3 : 2) : eight ? 2 : 1;
@@ -700,8 +701,19 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
             } else if constexpr (MODE == ATTEND_JOINED) {
                 if (a.parts == 1) {
                     const uint64_t slot = at * a.stride + a.shared;
-                    for (uint32_t p = 0; p < a.shared_parts; p++)
-                        attend_add(ms, x, a.part_sum[slot + p], *(const f32x4 *)(a.part_out + (slot + p) * HD + d));
+                    constexpr uint32_t AHEAD = 8; // parts loaded at a time
+                    for (uint32_t p0 = 0; p0 < a.shared_parts; p0 += AHEAD) {
+                        float2 more[AHEAD];
+                        f32x4 y[AHEAD];
+#pragma unroll
+                        for (uint32_t p = 0; p < AHEAD; p++) {
+                            const uint64_t from = slot + min(p0 + p, a.shared_parts - 1);
+                            more[p] = a.part_sum[from], y[p] = *(const f32x4 *)(a.part_out + from * HD + d);
+                        }
+#pragma unroll
+                        for (uint32_t p = 0; p < AHEAD; p++)
+                            if (p0 + p < a.shared_parts) attend_add(ms, x, more[p], y[p]);
+                    }
                     attend_write<T>(a, row, qh, d, ms.x == -INFINITY, ms, x, LIFT);
                 } else {
                     *(f32x4 *)(a.part_out + (at * a.stride + part) * HD + d) = x;
@@ -834,6 +846,6 @@ __global__ void __launch_bounds__(ATTEND_THREADS) k_attend_join(AttendArgs a) {
 
 // Launches the kernel for queries of type T (attend_*.hip, one unit a type).
 template <typename T>
-void launch_attend(const AttendArgs &a, AttendMode mode, uint32_t format, bool two_tiles, uint32_t groups, hipStream_t s);
+void launch_attend(const AttendArgs &a, AttendMode mode, uint32_t format, uint32_t row_tiles, uint32_t groups, hipStream_t s);
 
 }  // namespace rl

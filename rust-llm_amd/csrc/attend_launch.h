@@ -21,24 +21,32 @@ void launch_attend_rows(const AttendArgs &a, AttendMode mode, uint32_t groups, h
     else launch_attend_mode<T, FMT, HD, RT, ATTEND_JOINED>(a, groups, s);
 }
 
+template <typename T, int FMT, int HD>
+void launch_attend_dim(const AttendArgs &a, AttendMode mode, uint32_t row_tiles, uint32_t groups, hipStream_t s) {
+    if constexpr (sizeof(T) == 2)
+        if (row_tiles == 4) return launch_attend_mode<T, FMT, HD, 4, ATTEND_PREFIX>(a, groups, s);
+    if (row_tiles == 2) launch_attend_rows<T, FMT, HD, 2>(a, mode, groups, s);
+    else launch_attend_rows<T, FMT, HD, 1>(a, mode, groups, s);
+}
+
 template <typename T, int FMT>
-void launch_attend_format(const AttendArgs &a, AttendMode mode, bool two, uint32_t groups, hipStream_t s) {
+void launch_attend_format(const AttendArgs &a, AttendMode mode, uint32_t row_tiles, uint32_t groups, hipStream_t s) {
     switch (attend_dim(a.cache.dim)) {
-    case 64: return two ? launch_attend_rows<T, FMT, 64, 2>(a, mode, groups, s) : launch_attend_rows<T, FMT, 64, 1>(a, mode, groups, s);
-    case 128: return two ? launch_attend_rows<T, FMT, 128, 2>(a, mode, groups, s) : launch_attend_rows<T, FMT, 128, 1>(a, mode, groups, s);
+    case 64: return launch_attend_dim<T, FMT, 64>(a, mode, row_tiles, groups, s);
+    case 128: return launch_attend_dim<T, FMT, 128>(a, mode, row_tiles, groups, s);
     default: return launch_attend_rows<T, FMT, 256, 1>(a, mode, groups, s);
     }
 }
 
 template <typename T>
-void launch_attend(const AttendArgs &a, AttendMode mode, uint32_t format, bool two, uint32_t groups, hipStream_t s) {
+void launch_attend(const AttendArgs &a, AttendMode mode, uint32_t format, uint32_t row_tiles, uint32_t groups, hipStream_t s) {
     // The ABI has refused the 16-bit format that is not the queries' own.
     if constexpr (!std::is_same_v<T, bhalf_t>)
-        if (format == RL_F16) return launch_attend_format<T, RL_F16>(a, mode, two, groups, s);
+        if (format == RL_F16) return launch_attend_format<T, RL_F16>(a, mode, row_tiles, groups, s);
     if constexpr (!std::is_same_v<T, half_t>)
-        if (format == RL_BF16) return launch_attend_format<T, RL_BF16>(a, mode, two, groups, s);
-    if (format == RL_I8) return launch_attend_format<T, RL_I8>(a, mode, two, groups, s);
-    launch_attend_format<T, RL_F8>(a, mode, two, groups, s);
+        if (format == RL_BF16) return launch_attend_format<T, RL_BF16>(a, mode, row_tiles, groups, s);
+    if (format == RL_I8) return launch_attend_format<T, RL_I8>(a, mode, row_tiles, groups, s);
+    launch_attend_format<T, RL_F8>(a, mode, row_tiles, groups, s);
 }
 
 }  // namespace rl

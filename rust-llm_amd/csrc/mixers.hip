@@ -8,7 +8,7 @@
 #include <new>
 #include <string>
 
-#include "attend.h"
+#include "attend_shared.h"
 #include "delta_launch.h"
 #include "mix_args.h"
 
@@ -143,6 +143,8 @@ uint32_t attend_tiles(uint64_t tokens) { return (uint32_t)((tokens + ATTEND_TILE
 // this holds parts for have row blocks enough to fill the device. Without a limit 8192 rows of 32 heads and lengths up to
 // 131072 took 11.7 GB, a million tokens 35.
 constexpr uint64_t ATTEND_ROOM = 1u << 20;
+// And at least: a workgroup of 128 rows a CU.
+constexpr uint64_t ATTEND_LEAST = 1u << 15;
 
 // Parts that lengths up to `tiles` need at the least; one sequence has no others to wait for.
 uint32_t attend_least_parts(uint32_t tiles, uint32_t seqs) {
@@ -153,6 +155,24 @@ uint32_t attend_least_parts(uint32_t tiles, uint32_t seqs) {
 
 // Parts of a shared prefix at most: each of a row's columns is joined by one thread, which loads them one after the other.
 constexpr uint32_t SHARED_PARTS = 16;
+
+// Rows times heads of a group, on average, from which the kernel whose waves share each tile is taken. Behind 8192 tokens, 8
+// key-value heads, us, k_attend / k_attend_shared with 64 and 128 rows: 128 dims bf16 25.8 / 28.2, 33.5 / 29.8, int8 23.9 / 27.7,
+// 31.4 / 29.0, f32 queries 27.1 / 32.9, 35.6 / 34.7; 256 dims 38.5 / 40.4, 54.8 / 42.6; 64 dims 17.1 / 21.2, 21.1 / 21.6.
+constexpr uint64_t SHARED_MANY = 96;
+
+// Own tokens up to which the launch that joins parts costs more than they save: behind a prefix of 1009 tokens, 8 sequences of
+// 16 / 4 heads of 256 bf16, us, one part / several: 128 tokens 18.6 / 20.3, 256 21.0 / 20.5, 512 25.8 / 21.0; behind 4096, 4
+// sequences of 32 / 8 heads of 128: 16.7 / 18.5, 512 tokens 20.8 / 18.9.
+constexpr uint32_t SHARED_OWN = 128;
+
+// Tiles that a workgroup's start and end cost.
+constexpr uint32_t SHARED_START = 4;
+
+// Row blocks of all groups, at most.
+uint64_t shared_blocks(uint64_t rows, uint32_t groups, uint32_t size) {
+    return groups == 1 ? (rows + size - 1) / size : rows / size + groups;
+}
 
 // The checks that the attention's calls have in common.
 int check_attention(const rl_attention *h, const rl_kv_cache *cache, const rl_heads *q, const rl_heads *out, uint32_t rows,
@@ -492,9 +512,9 @@ int rl_attention_create(int device, uint32_t max_rows, uint32_t q_heads, uint32_
     if (!a) return fail(RL_ERR_CAPACITY, "out of host memory");
     a->device = device;
     a->max_rows = max_rows, a->q_heads = q_heads, a->kv_heads = kv_heads, a->dim = dim, a->max_len = max_len;
-    // Room for the least parts of every row within the limit, and for as many workgroups of 32 rows as the device holds.
+    // Room for the least parts of every row within the limit, and for as many workgroups as the device holds.
     const uint64_t heads = (uint64_t)max_rows * q_heads;
-    a->slots = std::max<uint64_t>(std::min(heads * attend_least_parts(attend_tiles(max_len), 2), ATTEND_ROOM), CUS * 3 * 32);
+    a->slots = std::max<uint64_t>(std::min(heads * attend_least_parts(attend_tiles(max_len), 2), ATTEND_ROOM), ATTEND_LEAST);
     hipError_t e = hipMalloc(&a->part_out, a->slots * attend_dim(dim) * sizeof(float));
     if (e == hipSuccess) e = hipMalloc(&a->part_sum, a->slots * sizeof(float2));
     if (e == hipSuccess) e = hipMalloc(&a->part_count, heads * sizeof(uint32_t));
@@ -534,7 +554,7 @@ int rl_attention_rows(rl_attention *h, const rl_kv_cache *cache, const rl_heads 
         return fail(RL_ERR_CAPACITY, "too many sequences times row blocks in a call");
     a.joins = a.parts <= ATTEND_FEW;
     with_type(q->dtype, [&](auto t) {
-        launch_attend<decltype(t)>(a, ATTEND_ALONE, cache->format, two, groups, static_cast<hipStream_t>(stream));
+        launch_attend<decltype(t)>(a, ATTEND_ALONE, cache->format, two ? 2 : 1, groups, static_cast<hipStream_t>(stream));
     });
     return launched("rl_attention_rows launch");
 }
@@ -562,16 +582,41 @@ int rl_attention_shared(rl_attention *h, const rl_kv_cache *cache, const rl_head
                                     rows, max_prefix);
     shared.group_starts = group_starts, shared.group_end = seqs;
     shared.most_rows = rows;
-    const bool shared_two = attend_two(cache->format, h->dim, ((uint64_t)rows * own.group + 15) / 16, (uint64_t)groups * h->kv_heads);
-    uint32_t own_groups, shared_groups;
     // The prefix's parts are joined by each row's own workgroup, so they are few. Room is theirs first: a sequence's own
     // tokens in one part need none.
+    const uint64_t most_parts = std::min<uint64_t>(room, SHARED_PARTS), shared_rows = (uint64_t)rows * own.group;
+    const bool many = shared_rows >= SHARED_MANY * groups;
+    const bool shared_two = attend_two(cache->format, h->dim, (shared_rows + 15) / 16, (uint64_t)groups * h->kv_heads);
     shared.packed = 1;
-    const uint32_t block_rows = shared_two ? 32 : 16;
-    shared.blocks = (uint32_t)((uint64_t)rows * shared.group / block_rows + groups);
-    bool fits = attend_shape(shared, h, (uint64_t)h->kv_heads * shared.blocks, attend_held(q, cache, h, shared_two),
-                             std::min<uint64_t>(room, SHARED_PARTS), &shared_groups);
-    const uint64_t own_room = room - shared.parts > 1 ? std::min<uint64_t>(room - shared.parts, ATTEND_MAX_PARTS - SHARED_PARTS) : 1;
+    uint32_t own_groups, shared_groups;
+    bool fits = true, wider = false;
+    if (many) {
+        const uint32_t tile = shared_tile(attend_dim(h->dim)), tiles = (uint32_t)(((uint64_t)shared.max_len + tile - 1) / tile);
+        // Of one row tile a wave and two, and of the numbers of parts, what takes the least time: rounds of a workgroup a CU,
+        // each a part's tiles, which cost two row tiles 1.7 times as much as one.
+        double least = INFINITY;
+        for (const uint32_t row_tiles : {1u, 2u}) {
+            if (row_tiles > (q->dtype == RL_F32 ? shared_row_tiles<float>(attend_dim(h->dim)) : shared_row_tiles<half_t>(attend_dim(h->dim)))) continue;
+            const uint64_t blocks = shared_blocks(shared_rows, groups, 64 * row_tiles), columns = (uint64_t)h->kv_heads * blocks;
+            for (uint32_t parts = 1; parts <= std::min<uint64_t>(most_parts, tiles); parts++) {
+                const uint64_t part_tiles = (tiles + parts - 1) / parts;
+                const double time = (double)((columns * parts + CUS - 1) / CUS) * (part_tiles + SHARED_START) * (row_tiles == 2 ? 1.7 : 1.0);
+                if (time >= least) continue;
+                least = time, wider = row_tiles == 2;
+                shared.blocks = (uint32_t)blocks, shared.part_tiles = (uint32_t)part_tiles, shared.parts = (uint32_t)((tiles + part_tiles - 1) / part_tiles);
+            }
+        }
+        shared.group_inv = inverse_of(shared.group), shared.blocks_inv = inverse_of(shared.blocks), shared.heads_inv = inverse_of(h->kv_heads);
+        const uint64_t n = ((uint64_t)h->kv_heads * shared.parts + 7) / 8 * 8 * shared.blocks;
+        shared_groups = (uint32_t)n;
+        fits = n <= MAX_ROWS - 1;
+    } else {
+        shared.blocks = (uint32_t)shared_blocks(shared_rows, groups, shared_two ? 32 : 16);
+        fits = attend_shape(shared, h, (uint64_t)h->kv_heads * shared.blocks, attend_held(q, cache, h, shared_two), most_parts, &shared_groups);
+    }
+    // A sequence's own tokens go in one part, which its workgroup joins with the prefix's by itself, up to SHARED_OWN.
+    const uint64_t left = room - shared.parts;
+    const uint64_t own_room = own.max_len <= SHARED_OWN || left <= 1 ? 1 : std::min<uint64_t>(left, ATTEND_MAX_PARTS - SHARED_PARTS);
     fits = fits && attend_shape(own, h, attend_blocks(own, h, two), attend_held(q, cache, h, two), own_room, &own_groups);
     if (!fits) return fail(RL_ERR_CAPACITY, "too many sequences times row blocks in a call");
     own.shared = shared.shared = own.parts > 1 ? own.parts : 0;
@@ -579,8 +624,9 @@ int rl_attention_shared(rl_attention *h, const rl_kv_cache *cache, const rl_head
     own.stride = shared.stride = own.shared + shared.parts;
     with_type(q->dtype, [&](auto t) {
         const hipStream_t s = static_cast<hipStream_t>(stream);
-        launch_attend<decltype(t)>(shared, ATTEND_PREFIX, cache->format, shared_two, shared_groups, s);
-        launch_attend<decltype(t)>(own, ATTEND_JOINED, cache->format, two, own_groups, s);
+        if (many) launch_attend_shared<decltype(t)>(shared, cache->format, wider, shared_groups, s);
+        else launch_attend<decltype(t)>(shared, ATTEND_PREFIX, cache->format, shared_two ? 2 : 1, shared_groups, s);
+        launch_attend<decltype(t)>(own, ATTEND_JOINED, cache->format, two ? 2 : 1, own_groups, s);
     });
     return launched("rl_attention_shared launch");
 }

@@ -81,6 +81,12 @@ SHARED = [
     ([1024, 1024, 1000], [20, 1, 0], [9] * 21, [4] * 21, 16, 2, 128, 16, "bf16", "bf16"),  # a group without sequences
     ([700], [64], [16] * 64, [1] * 64, 64, 1, 64, 48, "f8", "bf16"),
     ([513], [9], [11] * 9, [9] * 9, 5, 5, 112, 16, "bf16", "f32"),
+    ([1300, 40], [30, 3], [7] * 33, [2] * 33, 12, 2, 112, 16, "bf16", "f32"),  # the three parts of f32 queries and weights
+    ([900], [40], [3 + i for i in range(40)], [1] * 40, 8, 2, 256, 32, "f16", "f32"),
+    ([2049], [20], [5] * 20, [3] * 20, 16, 4, 64, 24, "f8", "f32"),
+    ([1025, 3000], [30, 40], [20] * 70, [1] * 70, 16, 2, 48, 48, "i8", "f16"),
+    ([700], [50], [9] * 50, [1] * 50, 16, 4, 256, 7, "bf16", "bf16"),
+    ([65, 64, 63, 1], [40, 40, 40, 40], [1 + i % 5 for i in range(160)], [1] * 160, 8, 2, 80, 16, "f16", "f16"),
 ]
 
 
@@ -123,11 +129,14 @@ def test_shared_as_rows_over_whole_tables(device):
 
 def test_shared_strides_and_large_scores(device):
     g = np.random.default_rng(22)
-    c = Case(g, device, [130, 77], [2, 1], [30, 4, 50], [2, 1, 3], 4, 2, 64, 16, "bf16", "f32", spread=60.0)
-    for pads in ((0, 0), (1, 3), (8, 4)):
-        qs, outs = strided(c.q, *pads, device), strided(c.out, *pads, device)
-        c.call(qs, outs, scale=1.0)
-        c.check(outs, scale=1.0)
+    for more in (1, 40):
+        c = Case(g, device, [130, 77], [2 * more, 1], [30, 4] * more + [50], [2, 1] * more + [3], 4, 2, 64, 16, "bf16", "f32",
+                 spread=60.0)
+        for pads in ((0, 0), (1, 3), (8, 4)):
+            qs, outs = strided(c.q, *pads, device), strided(c.out, *pads, device)
+            for scale in (1.0, -0.5, 0.0):  # of another sign, and all weights alike
+                c.call(qs, outs, scale=scale)
+                c.check(outs, scale=scale)
 
 
 def test_shared_past_its_bounds_gives_nan(device):
@@ -158,9 +167,11 @@ def test_shared_values_out_of_sight(device):
     # Own tokens past a row's, and what stands in the pages' rest, are NaN (fill) or infinite: they reach no row.
     g = np.random.default_rng(24)
     for fmt, dtype in (("bf16", "bf16"), ("f16", "f32"), ("f8", "bf16"), ("i8", "f32")):
-        c = Case(g, device, [50, 21], [2, 2], [3, 30, 17, 1], [2, 3, 1, 1], 4, 2, 64, 16, fmt, dtype, fill=float("inf"))
-        c.call()
-        c.check()
+        for more in (1, 40):  # few rows of a prefix, and many
+            c = Case(g, device, [50, 21], [2 * more, 2], [3, 30] * more + [17, 1], [2, 3] * more + [1, 1], 4, 2, 64, 16, fmt,
+                     dtype, fill=float("inf"))
+            c.call()
+            c.check()
 
 
 def test_shared_scores_of_minus_infinity(device):
