@@ -19,15 +19,18 @@ struct DraftArgs {
     const float *uniforms, *draws;
     int32_t *accepted, *tokens;
     uint32_t vocab, drafts, seqs, chunks;
+    uint32_t per, groups; // chunks of a workgroup, workgroups of a sequence
     double *sums;      // [seq][chunk]
     uint32_t *arrived; // [seq], zero between calls
 };
 
 constexpr uint32_t DRAFT_THREADS = 256, DRAFT_WAVES = 4, DRAFT_CHUNK = 4096, DRAFT_EACH = DRAFT_CHUNK / DRAFT_THREADS;
+constexpr uint32_t DRAFT_PER = 8; // chunks of a workgroup at most
 constexpr uint32_t LIST_EACH = 4, LIST_CHUNK = DRAFT_THREADS * LIST_EACH, LIST_TILE = 1024;
 constexpr int DRAFT_STORED = 0x0F70; // s_waitcnt vmcnt(0)
 
-__device__ inline double probability(float p) { return p > 0.0f && p < INFINITY ? (double)p : 0.0; }
+__device__ inline float positive(float p) { return p > 0.0f && p < INFINITY ? p : 0.0f; }
+__device__ inline double probability(float p) { return (double)positive(p); }
 
 // Inclusive sums over the wave in lane order.
 __device__ inline double wave_scan(double x) {
@@ -111,10 +114,10 @@ __device__ inline void draft_write(const DraftArgs &a, uint32_t s, const DraftSp
 // WIDE: rows are aligned for 16-byte loads.
 template <bool WIDE>
 __global__ void __launch_bounds__(DRAFT_THREADS) k_drafts(DraftArgs a) {
-    __shared__ double waves[DRAFT_WAVES], sums[(1u << 21) / DRAFT_CHUNK];
+    __shared__ double waves[DRAFT_WAVES], sums[(1u << 21) / DRAFT_CHUNK], parts[DRAFT_PER][DRAFT_WAVES];
     __shared__ uint32_t mins[DRAFT_WAVES];
     __shared__ bool last;
-    const uint32_t s = blockIdx.x / a.chunks, chunk = blockIdx.x - s * a.chunks, tid = threadIdx.x, lane = tid % 64;
+    const uint32_t s = blockIdx.x / a.groups, first = (blockIdx.x - s * a.groups) * a.per, tid = threadIdx.x, lane = tid % 64;
     const DraftSpan d = draft_span(a, s);
     const float draw = a.draws[s];
     uint32_t accepted = d.count;
@@ -140,14 +143,12 @@ __global__ void __launch_bounds__(DRAFT_THREADS) k_drafts(DraftArgs a) {
     const float *p = a.target.probs + ((uint64_t)d.begin + s + accepted) * a.target.row_stride;
     const float *q = rejected && a.draft.probs ? a.draft.probs + ((uint64_t)d.begin + accepted) * a.draft.row_stride : nullptr;
     const uint32_t one = rejected && !a.draft.probs ? (uint32_t)a.drafted[d.begin + accepted] : a.vocab; // q is 1 there
-    // What can be drawn of four tokens.
-    const auto left4 = [&](uint32_t v, bool less, double *left) {
-        float x[4] = {}, y[4] = {};
+    // Four tokens' probabilities, zeros past the vocabulary, and what can be drawn of them.
+    const auto load4 = [&](uint32_t v, bool less, f32x4 &x, f32x4 &y) {
+        x = y = f32x4{0, 0, 0, 0};
         if (WIDE && v + 4 <= a.vocab) {
-            const f32x4 pv = *(const f32x4 *)(p + v);
-            const f32x4 qv = less && q ? *(const f32x4 *)(q + v) : f32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = pv[i], y[i] = qv[i];
+            x = *(const f32x4 *)(p + v);
+            if (less && q) y = *(const f32x4 *)(q + v);
         } else
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++)
@@ -155,43 +156,66 @@ __global__ void __launch_bounds__(DRAFT_THREADS) k_drafts(DraftArgs a) {
                     x[i] = p[v + i];
                     if (less && q) y[i] = q[v + i];
                 }
+    };
+    const auto left4 = [&](uint32_t v, bool less, f32x4 x, f32x4 y, double *left) {
 #pragma unroll
         for (uint32_t i = 0; i < 4; i++) {
             const double from = probability(x[i]), take = less && v + i == one ? 1.0 : probability(y[i]);
             left[i] = from > take ? from - take : 0.0;
         }
     };
-    const auto chunk_sum = [&](uint32_t c, bool less) {
-        double left[DRAFT_EACH], sum = 0.0, all;
+    // The wave's part of a chunk's sum. The next chunk is on its way while one is added.
+    constexpr uint32_t QUADS = DRAFT_EACH / 4;
+    f32x4 x[QUADS], y[QUADS];
+    const auto load_chunk = [&](uint32_t c, bool less) {
 #pragma unroll
-        for (uint32_t j = 0; j < DRAFT_EACH / 4; j++) left4(c * DRAFT_CHUNK + (j * DRAFT_THREADS + tid) * 4, less, left + 4 * j);
-#pragma unroll
-        for (uint32_t j = 0; j < DRAFT_EACH; j++) sum += left[j];
-        block_scan(sum, waves, all);
-        return all;
+        for (uint32_t j = 0; j < QUADS; j++) load4(c * DRAFT_CHUNK + (j * DRAFT_THREADS + tid) * 4, less, x[j], y[j]);
     };
-    const double mine = chunk_sum(chunk, true);
-    if (a.chunks > 1) {
-        if (tid == 0) {
-            __hip_atomic_store((uint64_t *)(a.sums + (uint64_t)s * a.chunks + chunk), __builtin_bit_cast(uint64_t, mine),
-                               __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const auto add_chunk = [&](uint32_t c, bool less) { // of what was loaded
+        double sum = 0.0;
+#pragma unroll
+        for (uint32_t j = 0; j < QUADS; j++) {
+            double left[4];
+            left4(c * DRAFT_CHUNK + (j * DRAFT_THREADS + tid) * 4, less, x[j], y[j], left);
+            sum += (left[0] + left[1]) + (left[2] + left[3]);
+        }
+        return sum;
+    };
+    const uint32_t end = min(first + a.per, a.chunks);
+    load_chunk(first, true);
+    for (uint32_t c = first; c < end; c++) {
+        double sum = add_chunk(c, true);
+        if (c + 1 < end) load_chunk(c + 1, true);
+#pragma unroll
+        for (uint32_t d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
+        if (lane == 0) parts[c - first][tid / 64] = sum;
+    }
+    __syncthreads();
+    const auto chunk_total = [&](uint32_t i) { return (parts[i][0] + parts[i][1]) + (parts[i][2] + parts[i][3]); };
+    if (a.groups > 1) {
+        if (tid < end - first)
+            __hip_atomic_store((uint64_t *)(a.sums + (uint64_t)s * a.chunks + first + tid),
+                               __builtin_bit_cast(uint64_t, chunk_total(tid)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (tid == 0) { // of the wave that has stored them all
             __builtin_amdgcn_s_waitcnt(DRAFT_STORED);
-            last = atomicAdd(a.arrived + s, 1u) == a.chunks - 1;
+            last = atomicAdd(a.arrived + s, 1u) == a.groups - 1;
             if (last) __hip_atomic_store(a.arrived + s, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // ready for the next call
         }
         __syncthreads();
         if (!last) return;
     }
     for (uint32_t c = tid; c < a.chunks; c += DRAFT_THREADS)
-        sums[c] = a.chunks > 1 ? __builtin_bit_cast(double, __hip_atomic_load((const uint64_t *)(a.sums + (uint64_t)s * a.chunks + c),
+        sums[c] = a.groups > 1 ? __builtin_bit_cast(double, __hip_atomic_load((const uint64_t *)(a.sums + (uint64_t)s * a.chunks + c),
                                                                              __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
-                               : mine;
+                               : chunk_total(c);
     __syncthreads();
     int32_t token = -1;
     for (uint32_t less = 2; less-- > 0;) { // from max(p - q, 0), and from p where that has nothing
         if (!less) {
             for (uint32_t c = 0; c < a.chunks; c++) {
-                const double all = chunk_sum(c, false);
+                double all;
+                load_chunk(c, false);
+                block_scan(add_chunk(c, false), waves, all);
                 if (tid == 0) sums[c] = all;
             }
             __syncthreads();
@@ -216,7 +240,9 @@ __global__ void __launch_bounds__(DRAFT_THREADS) k_drafts(DraftArgs a) {
         block_scan(before, waves, all);
         double left[DRAFT_EACH];
 #pragma unroll
-        for (uint32_t j = 0; j < DRAFT_EACH / 4; j++) left4(c * DRAFT_CHUNK + tid * DRAFT_EACH + 4 * j, less, left + 4 * j);
+        for (uint32_t j = 0; j < QUADS; j++) load4(c * DRAFT_CHUNK + tid * DRAFT_EACH + 4 * j, less, x[j], y[j]);
+#pragma unroll
+        for (uint32_t j = 0; j < QUADS; j++) left4(c * DRAFT_CHUNK + tid * DRAFT_EACH + 4 * j, less, x[j], y[j], left + 4 * j);
         token = (int32_t)(c * DRAFT_CHUNK + block_pick(left, all, draw == draw ? border : INFINITY, waves, mins));
         break;
     }
@@ -235,26 +261,49 @@ __global__ void __launch_bounds__(DRAFT_THREADS) k_drafts_lists(DraftArgs a) {
     const DraftSpan d = draft_span(a, s);
     const float draw = a.draws[s];
     const auto kept = [](const rl_probs &x, uint64_t row) { return (uint32_t)min((uint64_t)x.kept[row], x.row_stride); };
-    // A token's probability in a list, by a wave.
-    const auto of = [&](const rl_probs &x, uint64_t row, uint32_t token) {
-        const uint32_t n = kept(x, row);
-        for (uint32_t j0 = 0; j0 < n; j0 += 64) {
+    // A token's probability in a list, by a wave. The first 64 entries are loaded before it is known how many there are.
+    struct Head {
+        uint32_t id, n;
+        float p;
+    };
+    const auto head = [&](const rl_probs &x, uint64_t row) {
+        const uint64_t at = row * x.row_stride + min((uint64_t)lane, x.row_stride - 1);
+        return Head{x.ids[at], kept(x, row), x.probs[at]};
+    };
+    const auto of = [&](const rl_probs &x, uint64_t row, const Head &h, uint32_t token) {
+        uint64_t where = __ballot(lane < h.n && h.id == token);
+        if (where) return probability(__shfl(h.p, (int)__ffsll((unsigned long long)where) - 1));
+        for (uint32_t j0 = 64; j0 < h.n; j0 += 64) {
             const uint32_t j = j0 + lane;
-            const bool found = j < n && x.ids[row * x.row_stride + j] == token;
-            const uint64_t where = __ballot(found);
+            where = __ballot(j < h.n && x.ids[row * x.row_stride + j] == token);
             if (where) return probability(x.probs[row * x.row_stride + j0 + (uint32_t)__ffsll((unsigned long long)where) - 1]);
         }
         return 0.0;
     };
     if (tid == 0) refused = d.count;
     __syncthreads();
-    for (uint32_t i = wave; i < d.count; i += DRAFT_WAVES) { // a wave's first refused draft
-        const uint32_t token = (uint32_t)a.drafted[d.begin + i];
-        const double p = of(a.target, (uint64_t)d.begin + s + i, token);
-        const double q = a.draft.probs ? of(a.draft, d.begin + i, token) : 1.0;
-        if ((double)a.uniforms[d.begin + i] * q < p) continue;
-        if (lane == 0) atomicMin(&refused, i);
-        break;
+    for (uint32_t i0 = wave; i0 < d.count; i0 += 2 * DRAFT_WAVES) { // two drafts at a time, up to the wave's first refused one
+        Head target[2], draft[2] = {};
+        uint32_t token[2];
+        float u[2];
+#pragma unroll
+        for (uint32_t k = 0; k < 2; k++) {
+            const uint64_t i = min(i0 + k * DRAFT_WAVES, d.count - 1);
+            target[k] = head(a.target, d.begin + s + i);
+            if (a.draft.probs) draft[k] = head(a.draft, d.begin + i);
+            token[k] = (uint32_t)a.drafted[d.begin + i], u[k] = a.uniforms[d.begin + i];
+        }
+        bool fine = true;
+#pragma unroll
+        for (uint32_t k = 0; k < 2; k++) {
+            const uint32_t i = i0 + k * DRAFT_WAVES;
+            if (!fine || i >= d.count) break;
+            const double p = of(a.target, (uint64_t)d.begin + s + i, target[k], token[k]);
+            const double q = a.draft.probs ? of(a.draft, (uint64_t)d.begin + i, draft[k], token[k]) : 1.0;
+            fine = (double)u[k] * q < p;
+            if (!fine && lane == 0) atomicMin(&refused, i);
+        }
+        if (!fine) break;
     }
     __syncthreads();
     const uint32_t accepted = refused;
@@ -264,35 +313,52 @@ __global__ void __launch_bounds__(DRAFT_THREADS) k_drafts_lists(DraftArgs a) {
     const uint32_t *ids = a.target.ids + row * a.target.row_stride;
     const uint32_t n = kept(a.target, row), others = rejected && a.draft.probs ? kept(a.draft, from) : 0;
     const uint32_t one = rejected && !a.draft.probs ? (uint32_t)a.drafted[d.begin + accepted] : 0;
+    // The first entries are loaded before it is known how many there are.
+    uint32_t id0[LIST_EACH];
+    float p0[LIST_EACH];
+#pragma unroll
+    for (uint32_t i = 0; i < LIST_EACH; i++) {
+        const uint64_t j = min((uint64_t)tid * LIST_EACH + i, a.target.row_stride - 1);
+        id0[i] = ids[j], p0[i] = probs[j];
+    }
+    uint2 entry{};
+    if (rejected && a.draft.probs) {
+        const uint64_t at = from * a.draft.row_stride + min((uint64_t)tid, a.draft.row_stride - 1);
+        entry = make_uint2(a.draft.ids[at], __float_as_uint(a.draft.probs[at]));
+    }
     double left[LIST_EACH];
     // What can be drawn of the entries from `at` on, a run a thread.
     const auto fill = [&](uint32_t at, bool less) {
         uint32_t id[LIST_EACH];
-        double take[LIST_EACH];
+        float take[LIST_EACH];
 #pragma unroll
         for (uint32_t i = 0; i < LIST_EACH; i++) {
             const uint32_t j = at + tid * LIST_EACH + i;
-            left[i] = j < n ? probability(probs[j]) : 0.0;
-            id[i] = j < n ? ids[j] : 0;
-            take[i] = less && rejected && !a.draft.probs && id[i] == one ? 1.0 : 0.0;
+            left[i] = j < n ? probability(at ? probs[j] : p0[i]) : 0.0;
+            id[i] = j >= n ? 0 : at ? ids[j] : id0[i];
+            take[i] = less && rejected && !a.draft.probs && id[i] == one ? 1.0f : 0.0f;
         }
         for (uint32_t j0 = 0; less && j0 < others; j0 += LIST_TILE) {
             const uint32_t m = min(others - j0, LIST_TILE);
             __syncthreads();
             for (uint32_t j = tid; j < m; j += DRAFT_THREADS) {
-                const uint64_t at = from * a.draft.row_stride + j0 + j;
-                tile[j] = make_uint2(a.draft.ids[at], __float_as_uint(a.draft.probs[at]));
+                uint2 x = entry;
+                if (j0 + j != tid) {
+                    const uint64_t at = from * a.draft.row_stride + j0 + j;
+                    x = make_uint2(a.draft.ids[at], __float_as_uint(a.draft.probs[at]));
+                }
+                tile[j] = make_uint2(x.x, __float_as_uint(positive(__uint_as_float(x.y))));
             }
             __syncthreads();
+#pragma unroll 8
             for (uint32_t j = 0; j < m; j++) {
                 const uint2 x = tile[j];
 #pragma unroll
-                for (uint32_t i = 0; i < LIST_EACH; i++)
-                    if (x.x == id[i]) take[i] = probability(__uint_as_float(x.y));
+                for (uint32_t i = 0; i < LIST_EACH; i++) take[i] = x.x == id[i] ? __uint_as_float(x.y) : take[i];
             }
         }
 #pragma unroll
-        for (uint32_t i = 0; i < LIST_EACH; i++) left[i] = left[i] > take[i] ? left[i] - take[i] : 0.0;
+        for (uint32_t i = 0; i < LIST_EACH; i++) left[i] = left[i] > (double)take[i] ? left[i] - (double)take[i] : 0.0;
     };
     int32_t token = -1;
     for (uint32_t less = 2; less-- > 0;) {

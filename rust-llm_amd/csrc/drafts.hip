@@ -2,6 +2,7 @@
 // drafts.h.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <new>
 #include <string>
 
@@ -22,6 +23,9 @@ struct rl_drafts {
 };
 
 namespace {
+
+// Workgroups that the chunks of a call are shared among.
+constexpr uint32_t DRAFT_FILL = 1024;
 
 // What is wrong with a call's probabilities, or null.
 const char *wrong(const rl_probs *p, uint32_t vocab) {
@@ -84,7 +88,10 @@ int rl_drafts_verify(rl_drafts *h, const rl_probs *target, const rl_probs *draft
     if (drafts > 1u << 23) return fail(RL_ERR_CAPACITY, "more than 2^23 drafts in a call");
     if (!starts || !draws || !accepted || !tokens || (drafts && (!drafted || !uniforms)))
         return fail(RL_ERR_ARGUMENT, "drafted, starts, uniforms, draws, accepted and tokens must be device pointers");
-    if ((uint64_t)seqs * h->chunks > 1u << 23) return fail(RL_ERR_CAPACITY, "too many sequences times tokens in a call");
+    // Chunks a workgroup: it has to find the row first, which several share, but few sequences want many workgroups.
+    const uint32_t per = (uint32_t)std::min<uint64_t>(std::max<uint64_t>((uint64_t)seqs * h->chunks / DRAFT_FILL, 1), DRAFT_PER);
+    const uint32_t groups = (h->chunks + per - 1) / per;
+    if ((uint64_t)seqs * groups > 1u << 23) return fail(RL_ERR_CAPACITY, "too many sequences times tokens in a call");
     DeviceGuard guard(h->device);
     if (!guard.ok) return fail(RL_ERR_DEVICE, "cannot select the handle's device");
     DraftArgs a{};
@@ -92,12 +99,12 @@ int rl_drafts_verify(rl_drafts *h, const rl_probs *target, const rl_probs *draft
     if (draft && drafts) a.draft = *draft;
     a.drafted = drafted, a.starts = starts, a.uniforms = uniforms, a.draws = draws;
     a.accepted = accepted, a.tokens = tokens;
-    a.vocab = h->vocab, a.drafts = drafts, a.seqs = seqs, a.chunks = h->chunks;
+    a.vocab = h->vocab, a.drafts = drafts, a.seqs = seqs, a.chunks = h->chunks, a.per = per, a.groups = groups;
     a.sums = h->sums, a.arrived = h->arrived;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (target->ids) hipLaunchKernelGGL(k_drafts_lists, dim3(seqs), dim3(DRAFT_THREADS), 0, s, a);
-    else if (wide(a.target) && wide(a.draft)) hipLaunchKernelGGL(k_drafts<true>, dim3(seqs * a.chunks), dim3(DRAFT_THREADS), 0, s, a);
-    else hipLaunchKernelGGL(k_drafts<false>, dim3(seqs * a.chunks), dim3(DRAFT_THREADS), 0, s, a);
+    else if (wide(a.target) && wide(a.draft)) hipLaunchKernelGGL(k_drafts<true>, dim3(seqs * groups), dim3(DRAFT_THREADS), 0, s, a);
+    else hipLaunchKernelGGL(k_drafts<false>, dim3(seqs * groups), dim3(DRAFT_THREADS), 0, s, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? RL_OK : hip_fail(e, "rl_drafts_verify launch");
 }
