@@ -249,7 +249,8 @@ typedef struct rl_scan rl_scan;
 /* a [channels][state_dim] (negative in use), skip and dt_bias [channels] (or NULL:
  * zeros) f32 on the host, copied. state_dim 4 to 256, a multiple of 4; channels a
  * multiple of groups, at most 2^20. Workspace for calls of up to max_rows tokens in up to
- * max_seqs sequences: at most 34 MB and four states. */
+ * max_seqs sequences: at most 34 MB and four states (rounded up to
+ * whole workgroups). */
 int rl_scan_create(int device, uint32_t max_rows, uint32_t max_seqs, uint32_t channels, uint32_t groups,
                    uint32_t state_dim, const float *a, const float *skip, const float *dt_bias, rl_scan **out);
 void rl_scan_destroy(rl_scan *scan);

@@ -29,15 +29,21 @@ namespace {
 
 // Rows of a sequence up to which one token after the other is the faster form.
 constexpr uint32_t SCAN_SHORT = 16;
-// Workgroups that pieces are made for, and the fewest tokens of one: shorter ones would wait more for their first state than
-// they compute.
-constexpr uint64_t SCAN_FILL = 1024;
-constexpr uint32_t SCAN_LEAST = 64;
+// Workgroups that pieces are made for, the fewest tokens of one, and the most pieces of a sequence: a piece's first state is
+// made of the ends of all before it.
+constexpr uint64_t SCAN_FILL = 1024, SCAN_MOST = 64;
+constexpr uint32_t SCAN_LEAST = 16;
 
-// Tokens of a piece.
-uint32_t piece_size(uint64_t rows, uint32_t columns) {
-    const uint64_t pieces = std::max<uint64_t>(SCAN_FILL / columns, 1);
-    return (uint32_t)std::max<uint64_t>((rows + pieces - 1) / pieces, SCAN_LEAST);
+// Tokens of a piece, 0 for whole sequences. A token takes a wave 0.42 us (its loads, a softplus, 16 exponentials in a row,
+// its output), and the device 0.25 us for each round of a wave a SIMD; pieces take each token twice, 1.8 times the work, and
+// a second launch. us, whole / in pieces, 5120 channels of 16 bf16: one sequence of 33 tokens 19.1 / 18.6, 64 30.7 / 20.2,
+// 128 52.3 / 22.4; 16 of 33 26.6 / 39.0, of 128 88.4 / 97.4 in pieces of 64 and 16.
+uint32_t piece_size(uint64_t rows, uint64_t most, uint64_t seqs, uint32_t columns) {
+    const uint64_t size = std::max({(uint64_t)SCAN_LEAST, (most + SCAN_MOST - 1) / SCAN_MOST, (rows * columns + SCAN_FILL - 1) / SCAN_FILL});
+    const double simds = 1024.0, round = 0.25 * SCAN_WAVES * columns / simds;
+    const double whole = most * std::max(0.42, round * seqs);
+    const double pieces = 8.0 + std::max(1.8 * round * rows, 2 * 0.42 * size + 0.1 * most / size);
+    return pieces < whole ? (uint32_t)size : 0;
 }
 
 }  // namespace
@@ -63,7 +69,8 @@ int rl_scan_create(int device, uint32_t max_rows, uint32_t max_seqs, uint32_t ch
     h->max_rows = max_rows, h->max_seqs = max_seqs, h->channels = channels, h->groups = groups, h->state = state_dim;
     const uint32_t each = scan_each(state_dim), per = SCAN_THREADS / scan_lanes(state_dim, each);
     h->columns = groups * ((channels / groups + per - 1) / per);
-    h->slots = scan_slots(std::min<uint64_t>(max_rows / SCAN_LEAST, std::max<uint64_t>(SCAN_FILL / h->columns, 1)));
+    // Pieces of a call are no more than its rows have, nor than fill the device.
+    h->slots = scan_slots(std::min<uint64_t>(max_rows / SCAN_LEAST, SCAN_FILL / h->columns + 1));
     const size_t size = (size_t)channels * state_dim, all = size + 2 * (size_t)channels;
     float *laid = new (std::nothrow) float[all];
     if (!laid) {
@@ -142,8 +149,8 @@ int rl_scan_rows(rl_scan *h, const rl_heads *x, const rl_heads *dt, const rl_hea
         a.columns = (h->channels + per - 1) / per;
     } else {
         a.columns = h->columns;
-        const uint32_t size = piece_size(rows, h->columns);
-        if (most > size) a.pieces = row_blocks(size);
+        const uint32_t size = piece_size(rows, most, seqs, h->columns);
+        if (size) a.pieces = row_blocks(size);
     }
     const uint64_t blocks = (uint64_t)(steps || !a.pieces.size ? seqs : row_block_count(rows, seqs, a.pieces.size)) * a.columns;
     if (blocks > MAX_ROWS) return fail(RL_ERR_CAPACITY, "too many sequences times channels in a call");

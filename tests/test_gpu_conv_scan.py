@@ -225,6 +225,30 @@ def test_scan_steps_of_any_size(device):
     assert np.all(np.abs(got - want) <= want * 10 * S.E + 2.0 ** -126), (got, want)
 
 
+@pytest.mark.parametrize("rows,channels", [(1100, 4100), (1999, 2000), (640, 300)])
+def test_scan_of_one_long_sequence_and_short_ones(device, rows, channels):
+    # As many pieces as the workspace holds: the handle is made for these rows and no more.
+    g = np.random.default_rng(rows + channels)
+    lens = [rows, 0, 3, 1, 17]
+    t, w = scan_case(g, device, lens, channels, 1, 4, "bf16", False, 0)
+    n = len(lens)
+    states = randn(g, (n, channels, 4), "f32", device)
+    before = states.clone()
+    scan = M.DeviceScan(sum(lens), n, w["a"], 1, w["skip"], w["dt_bias"])
+    out = torch.empty_like(t["x"])
+    slots, starts = i32(range(n), device), i32([0] + list(np.cumsum(lens)), device)
+    scan.rows(t["x"], t["dt"], t["b"], t["c"], out, states, slots, slots, starts)
+    torch.cuda.synchronize()
+    at = 0
+    for i, c in enumerate(lens):
+        part = {k: None if v is None else F.as64(v[at:at + c]) for k, v in t.items()}
+        want, after, off, err = S.scan(**part, a=F.as64(w["a"]), skip=F.as64(w["skip"]), bias=F.as64(w["dt_bias"]),
+                                       state=F.as64(before[i]), pieces=True)
+        assert np.all(np.abs(F.as64(out[at:at + c]) - want) <= off + F.rounding(np.abs(want) + off, "bf16")), i
+        assert np.all(np.abs(F.as64(states[i]) - after) <= err + 2.0 ** -126), i
+        at += c
+
+
 @pytest.mark.parametrize("what", ["conv", "scan", "steps"])
 def test_captured_calls_and_another_stream(device, what):
     g = np.random.default_rng(7)
