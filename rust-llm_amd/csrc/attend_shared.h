@@ -67,9 +67,11 @@ __global__ void __launch_bounds__(SHARED_THREADS, 2) k_attend_shared(AttendArgs 
     const uint2 job = split_by(eight.x * 8 + blockIdx.x % 8, a.cache.heads, a.heads_inv);
     const uint32_t part = job.x, head = job.y;
     if (part >= a.parts) return;
+    typedef const __attribute__((address_space(4))) int32_t constant_i32;
+    const constant_i32 *starts = (constant_i32 *)(uintptr_t)a.starts, *group_starts = (constant_i32 *)(uintptr_t)a.group_starts;
     const auto first_of = [&](uint32_t g) {
-        const int32_t at = min(max(a.group_starts[g], 0), (int32_t)a.group_end);
-        return a.starts ? min(max(a.starts[at], 0), (int32_t)a.rows) : min(at, (int32_t)a.rows);
+        const int32_t at = min(max(group_starts[g], 0), (int32_t)a.group_end);
+        return starts ? min(max(starts[at], 0), (int32_t)a.rows) : min(at, (int32_t)a.rows);
     };
     const auto first_block = [&](uint32_t g) { return (uint32_t)first_of(g) * G / ROWS + g; };
     uint32_t g = 0;
@@ -83,7 +85,7 @@ __global__ void __launch_bounds__(SHARED_THREADS, 2) k_attend_shared(AttendArgs 
     const uint32_t r0 = (eight.y - first_block(g)) * ROWS;
     if (rows <= 0 || r0 >= (uint32_t)rows * G) return;
     const uint32_t count = min((uint32_t)rows * G - r0, (uint32_t)ROWS);
-    const int32_t len = max(a.lens[g], 0);
+    const int32_t len = max(((constant_i32 *)(uintptr_t)a.lens)[g], 0);
     const uint32_t page = a.cache.page, tiles = (len + TILE - 1) / TILE;
     const bool nan = len > (int64_t)a.max_len || (len > 0 && split_by(len - 1, page, a.cache.page_inv).x >= a.table_width);
     const uint32_t begin = part * a.part_tiles, end = min(begin + a.part_tiles, tiles);
@@ -100,7 +102,6 @@ __global__ void __launch_bounds__(SHARED_THREADS, 2) k_attend_shared(AttendArgs 
     // Where tokens lie. P16 (pages of a multiple of 16 tokens): a tile's blocks of 16 each lie in one page, whose numbers are
     // fetched through the scalar cache a tile ahead of the loads. Else a thread looks the page of one token up, two tiles
     // ahead, and leaves its vector in LDS.
-    typedef const __attribute__((address_space(4))) int32_t constant_i32;
     const int32_t *table = a.pages + (uint64_t)g * a.table_width;
     const uint32_t pool = (uint32_t)(a.cache.slots / page), dim_bytes = a.cache.dim * SIZE;
     const auto split_at = [&](uint32_t t) { return split_by(t, page, a.cache.page_inv); };
