@@ -159,8 +159,8 @@ int rl_attention_rows(rl_attention *attention, const rl_kv_cache *cache, const r
 
 /* The same where sequences share long beginnings, whose keys and values are then read
  * once for a group and not once for each sequence. The sequences group_starts[g] ..
- * group_starts[g + 1] (i32 [groups + 1], rising from 0 to seqs) have the same
- * prefix_lens[g] tokens (i32, a negative one as 0) before their own, the t-th of them in
+ * group_starts[g + 1] (i32 [groups + 1], rising; what lies before the first or from the
+ * last on has no prefix) have the same prefix_lens[g] tokens (i32, a negative one as 0) before their own, the t-th of them in
  * slot prefix_pages[g * prefix_width + t / page] * page + t % page. lens and pages are
  * those of their own tokens, which begin a page: every row sees its whole prefix and its
  * own sequence's tokens up to its own, as above without a window. max_prefix bounds the
@@ -257,12 +257,12 @@ void rl_scan_destroy(rl_scan *scan);
 
 /* x, dt, z, out [rows][1][channels] and b, c [rows][groups][state_dim] of one type; z NULL
  * leaves the last factor out, softplus 0 takes s = dt + dt_bias. out may be x, dt or z
- * itself (same data and strides) or must not overlap them. states f32 [state_slots][channels]
+ * itself (same data and strides), or must not overlap an input. states f32 [state_slots][channels]
  * [state_dim], slots_in, slots_out and starts as in rl_delta_rows. most_rows bounds the
  * rows of any one sequence (0: as many as the call has); it may be any number, since it
  * only picks the form that is used for all of them: one token after the other, or long
  * sequences in pieces side by side. Both are as exact as f32 sums, but do not give the
- * same bits. An infinity may read as NaN. */
+ * same bits. An infinity may read as NaN, and so may a dt + dt_bias of 2^127 or more. */
 int rl_scan_rows(rl_scan *scan, const rl_heads *x, const rl_heads *dt, const rl_heads *z, const rl_heads *b,
                  const rl_heads *c, const rl_heads *out, float *states, uint64_t state_slots, const int32_t *slots_in,
                  const int32_t *slots_out, const int32_t *starts, uint32_t rows, uint32_t seqs, int softplus,

@@ -39,7 +39,7 @@ struct AttendArgs {
     uint32_t wide;        // whether q and out are aligned for 16-byte accesses
     float *part_out;      // [row * q_heads + head][part][HD]: sums of the weighted values
     float2 *part_sum;     // [row * q_heads + head][part]: maximum and sum
-    uint32_t *part_count; // [row * q_heads + head]: parts written, ATTEND_NONE if the row sees nothing
+    uint32_t *part_count; // [row * q_heads + head]: parts to join, and ATTEND_NONE if the row sees nothing or has no prefix; zero between calls
     uint32_t parts;       // parts a row has room for
     uint32_t *arrived;    // [row * q_heads + head], of a block's first: its parts that are done; zero between calls
     uint32_t group_inv, blocks_inv, columns_inv, heads_inv, tiles_inv; // inverse_of group, blocks, seqs * kv heads, kv heads, part_tiles
@@ -47,7 +47,7 @@ struct AttendArgs {
     // Shared prefixes. The rows of a group's sequences group_starts[g] .. group_starts[g + 1] see all of its prefix: part p
     // of it is partial result `shared` + p of their `stride`, with a maximum of -inf where it has no tokens.
     const int32_t *group_starts;
-    uint32_t shared, shared_parts, stride, group_end; // group_end: the sequences of the call
+    uint32_t shared, shared_parts, stride, group_end; // group_end: the call's sequences (ATTEND_PREFIX), its groups (ATTEND_JOINED)
 };
 
 // What a launch does: sequences by themselves; the prefixes of groups of sequences, in which `seqs`, `lens`, `pages` and
@@ -82,7 +82,6 @@ inline bool attend_two(uint32_t format, uint32_t dim, uint64_t count, uint64_t c
 // Workgroups of k_attend that share a CU: as many as its registers allow without spills.
 constexpr int attend_resident(uint32_t query_bytes, uint32_t format, uint32_t dim, int row_tiles) {
     const bool eight = format == RL_I8 || format == RL_F8;
-    if (row_tiles == 4 || (row_tiles == 2 && dim > 128)) return 1;
     switch (attend_dim(dim)) {
     case 64: return row_tiles == 1 ? 3 : 2;
     case 128: return row_tiles == 1 ? (eight && query_bytes == 2 ? 3 : 2) : eight ? 2 : 1;
@@ -229,6 +228,11 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
         if (part >= a.parts) return;
     }
     const int32_t first = first_of(s);
+    uint32_t shared_parts = 0; // of the sequence's prefix
+    if constexpr (MODE == ATTEND_JOINED) {
+        const constant_i32 *group_starts = (constant_i32 *)(uintptr_t)a.group_starts;
+        if ((int32_t)s >= group_starts[0] && (int32_t)s < group_starts[a.group_end]) shared_parts = a.shared_parts;
+    }
     const int64_t rows = MODE == ATTEND_PREFIX ? (int64_t)first_of(s + 1) - first : starts ? (int64_t)starts[s + 1] - first : 1;
     if (rows <= 0 || first < 0 || first + rows > a.rows) return; // no rows, or `starts` is not what it should be
     AttendSpan<MODE> span{max(lens[s], 0), (int32_t)rows, (int32_t)a.window}; // a negative length is none
@@ -250,8 +254,6 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
             }
             ((T *)a.out)[row * a.out_row + qh * a.out_head + d] = (T)NAN;
             if (d == 0 && a.lse) a.lse[row * a.q_heads + qh] = NAN;
-            if (d == 0 && MODE == ATTEND_ALONE && !a.joins) a.part_count[row * a.q_heads + qh] = 1; // nothing to join
-            if (d == 0 && MODE == ATTEND_JOINED && a.parts > 1) a.part_count[row * a.q_heads + qh] = 0; // likewise
         }
         return;
     }
@@ -702,23 +704,23 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
                 if (a.parts == 1) {
                     const uint64_t slot = at * a.stride + a.shared;
                     constexpr uint32_t AHEAD = 8; // parts loaded at a time
-                    for (uint32_t p0 = 0; p0 < a.shared_parts; p0 += AHEAD) {
+                    for (uint32_t p0 = 0; p0 < shared_parts; p0 += AHEAD) {
                         float2 more[AHEAD];
                         f32x4 y[AHEAD];
 #pragma unroll
                         for (uint32_t p = 0; p < AHEAD; p++) {
-                            const uint64_t from = slot + min(p0 + p, a.shared_parts - 1);
+                            const uint64_t from = slot + min(p0 + p, shared_parts - 1);
                             more[p] = a.part_sum[from], y[p] = *(const f32x4 *)(a.part_out + from * HD + d);
                         }
 #pragma unroll
                         for (uint32_t p = 0; p < AHEAD; p++)
-                            if (p0 + p < a.shared_parts) attend_add(ms, x, more[p], y[p]);
+                            if (p0 + p < shared_parts) attend_add(ms, x, more[p], y[p]);
                     }
                     attend_write<T>(a, row, qh, d, ms.x == -INFINITY, ms, x, LIFT);
                 } else {
                     *(f32x4 *)(a.part_out + (at * a.stride + part) * HD + d) = x;
                     if (d == 0) a.part_sum[at * a.stride + part] = ms;
-                    if (d == 0 && part == 0) a.part_count[at] = parts;
+                    if (d == 0 && part == 0) a.part_count[at] = parts | (shared_parts ? 0 : ATTEND_NONE);
                 }
                 continue;
             }
@@ -730,8 +732,8 @@ __global__ void __launch_bounds__(ATTEND_THREADS, attend_resident(sizeof(T), FMT
             } else {
                 *(f32x4 *)(a.part_out + (at * a.parts + part) * HD + d) = x;
                 if (d == 0) a.part_sum[at * a.parts + part] = ms;
+                if (d == 0 && part == 0) a.part_count[at] = parts | (none ? ATTEND_NONE : 0);
             }
-            if (d == 0 && part == 0 && !a.joins) a.part_count[at] = parts | (none ? ATTEND_NONE : 0);
         }
     }
     if (MODE != ATTEND_ALONE || parts == 1 || !a.joins) return;
@@ -807,8 +809,8 @@ __global__ void __launch_bounds__(ATTEND_THREADS) k_attend_join(AttendArgs a) {
     const uint64_t at = blockIdx.x;
     constexpr bool JOINED = MODE == ATTEND_JOINED;
     const uint32_t tid = threadIdx.x, count = a.part_count[at], own = min(count & ~ATTEND_NONE, a.parts);
-    if (own <= (JOINED ? 0 : 1)) return; // written already
-    const uint32_t n = own + (JOINED ? a.shared_parts : 0), stride = JOINED ? a.stride : a.parts;
+    if (!own) return; // written already, or no sequence's
+    const uint32_t n = own + (JOINED && !(count & ATTEND_NONE) ? a.shared_parts : 0), stride = JOINED ? a.stride : a.parts;
     const uint32_t c = tid % COLS, p0 = tid / COLS;
     const f32x4 *x = (const f32x4 *)(a.part_out + at * stride * HD) + c;
     const auto slot = [&](uint32_t p) { return JOINED && p >= own ? a.shared + (p - own) : p; };
@@ -822,6 +824,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS) k_attend_join(AttendArgs a) {
     float most = group_max<64>(ms.x);
     if (tid % 64 == 0) reduce[0][tid / 64] = most;
     __syncthreads();
+    if (tid == 0) a.part_count[at] = 0;
     most = fmaxf(fmaxf(reduce[0][0], reduce[0][1]), fmaxf(reduce[0][2], reduce[0][3]));
     const float f = ms.x == -INFINITY ? 0.0f : exp2_fast(ms.x - most);
     factor[tid] = f;

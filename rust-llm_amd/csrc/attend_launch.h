@@ -23,8 +23,6 @@ void launch_attend_rows(const AttendArgs &a, AttendMode mode, uint32_t groups, h
 
 template <typename T, int FMT, int HD>
 void launch_attend_dim(const AttendArgs &a, AttendMode mode, uint32_t row_tiles, uint32_t groups, hipStream_t s) {
-    if constexpr (sizeof(T) == 2)
-        if (row_tiles == 4) return launch_attend_mode<T, FMT, HD, 4, ATTEND_PREFIX>(a, groups, s);
     if (row_tiles == 2) launch_attend_rows<T, FMT, HD, 2>(a, mode, groups, s);
     else launch_attend_rows<T, FMT, HD, 1>(a, mode, groups, s);
 }

@@ -1,14 +1,24 @@
 // Attention over a prefix that many rows share (include/rl_mixers.h).
 //
 // k_attend gives each wave other tokens of the same rows, which suits few rows. Here
-// the four waves of a workgroup have rows of their own, 16 RT each, and the same
-// tokens: a tile of keys and values is loaded once for all, converted to the 16 bits
-// of the products, turned, and laid into LDS as the fragments that the products take,
-// so a wave's own work is its products and its softmax:
-//   S^T = K Q^T, w = 2^(S - m), O^T += V^T w   as in attend.h, per tile of 64 tokens
-// Waves 0 and 1 bring the keys, 2 and 3 the values: in registers while the tile before
-// is computed, into the other of two buffers behind it. Page numbers are looked up two
-// tiles ahead. Every row sees the whole prefix, so only the last tile has a mask.
+// the waves of a workgroup have rows of their own, 16 RT each, and the same tokens: a
+// tile of keys and values is loaded once for all, converted to the 16 bits of the
+// products, turned, and laid into LDS as the fragments that the products take, so a
+// wave's own work is its products and its softmax:
+//   S^T = K Q^T, w = 2^(S - m), O^T += V^T w   as in attend.h, 32 tokens at a time
+// A workgroup has two halves of four waves, with the same rows and every other tile.
+// Waves 0 and 1 of a half bring the keys, 2 and 3 the values: in registers while the
+// tile before is computed, into the other of two buffers behind it. The halves are half
+// a tile apart, so that one's products pass beside the other's softmax (5 % faster than
+// in step). Their sums are added at the end. Every row sees the whole prefix, so only
+// the last tile has a mask.
+//
+// Bound by instructions: on a SIMD matrix and vector instructions of two waves take
+// nearly the sum of their times (8 products and 32 sums 257 cycles, alone 164 and 190),
+// and a tile of 64 tokens and 32 rows of 128 bf16 is 96 products of 16 cycles and about
+// 400 vector instructions of 4 or 5. 256 rows a key-value head, 8 heads of 128, 16384
+// tokens bf16: 46.9 us, 366 TFLOP/s (k_attend 106 us). 640 rows, 8001 tokens int8 in
+// pages of 24, and two prefixes of a half and a third: 129 us, 298 TFLOP/s.
 #pragma once
 #include "attend.h"
 
@@ -86,7 +96,7 @@ __global__ void __launch_bounds__(SHARED_THREADS, 2) k_attend_shared(AttendArgs 
     if (rows <= 0 || r0 >= (uint32_t)rows * G) return;
     const uint32_t count = min((uint32_t)rows * G - r0, (uint32_t)ROWS);
     const int32_t len = max(((constant_i32 *)(uintptr_t)a.lens)[g], 0);
-    const uint32_t page = a.cache.page, tiles = (len + TILE - 1) / TILE;
+    const uint32_t page = a.cache.page, tiles = ((uint32_t)len + TILE - 1) / TILE;
     const bool nan = len > (int64_t)a.max_len || (len > 0 && split_by(len - 1, page, a.cache.page_inv).x >= a.table_width);
     const uint32_t begin = part * a.part_tiles, end = min(begin + a.part_tiles, tiles);
     const auto slot_of = [&](uint32_t r) { // of a row's partial result

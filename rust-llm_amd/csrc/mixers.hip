@@ -580,7 +580,7 @@ int rl_attention_shared(rl_attention *h, const rl_kv_cache *cache, const rl_head
     const bool two = attend_two(cache->format, h->dim, (expanded + 15) / 16, (uint64_t)seqs * h->kv_heads);
     AttendArgs shared = attend_args(h, cache, q, out, lse, rows, starts, prefix_lens, groups, prefix_pages, prefix_width, scale,
                                     rows, max_prefix);
-    shared.group_starts = group_starts, shared.group_end = seqs;
+    shared.group_starts = own.group_starts = group_starts, shared.group_end = seqs, own.group_end = groups;
     shared.most_rows = rows;
     // The prefix's parts are joined by each row's own workgroup, so they are few. Room is theirs first: a sequence's own
     // tokens in one part need none.

@@ -87,6 +87,8 @@ SHARED = [
     ([1025, 3000], [30, 40], [20] * 70, [1] * 70, 16, 2, 48, 48, "i8", "f16"),
     ([700], [50], [9] * 50, [1] * 50, 16, 4, 256, 7, "bf16", "bf16"),
     ([65, 64, 63, 1], [40, 40, 40, 40], [1 + i % 5 for i in range(160)], [1] * 160, 8, 2, 80, 16, "f16", "f16"),
+    ([300], [31], [70] + [3] * 30, [60] + [1] * 30, 8, 2, 128, 16, "bf16", "bf16"),  # one sequence of many rows among single ones
+    ([90, 31], [20, 20], [600] * 40, [1] * 40, 8, 2, 64, 16, "i8", "bf16"),  # more tokens of their own than shared ones
 ]
 
 
@@ -139,9 +141,40 @@ def test_shared_strides_and_large_scores(device):
                 c.check(outs, scale=scale)
 
 
-def test_shared_past_its_bounds_gives_nan(device):
+@pytest.mark.parametrize("heads,own", [(4, 20), (64, 20), (4, 900)])  # few and many rows of a prefix; own tokens in parts
+def test_shared_sequences_of_no_group_and_rows_behind_the_last(device, heads, own):
+    g = np.random.default_rng(27)
+    c = Case(g, device, [0, 300, 0], [2, 3, 2], [own, 5, own, 6, 3, 7, own], [2, 1, 1, 2, 3, 1, 2], heads, 2, 64, 16, "bf16", "bf16")
+    c.call()  # every partial result and count of the handle has been used
+    c.out.fill_(7.0)
+    c.lse.fill_(7.0)
+    c.t.update(groups=i32([2, 5], device), prefix_lens=i32([300], device))
+    c.prefix_table = c.prefix_table[1:2].contiguous()
+    c.call()
+    c.check()
+    # A batch that holds fewer rows than the call has: the others stay as they were.
+    c.out.fill_(7.0)
+    c.lse.fill_(7.0)
+    c.starts[-1] = 10  # the last sequence has none
+    c.call()
+    assert (c.out[10:] == 7.0).all() and (c.lse[10:] == 7.0).all()
+    c.lens, c.counts, c.per = c.lens[:-1], c.counts[:-1], [2, 3, 1]
+    c.check()
+    att = M.DeviceAttention(12, heads, 2, 64, 40000)
+    table = c.table.expand(-1, -1)[:, :1].expand(-1, 2500).contiguous()  # the same page over and over
+    lens = i32([40000] * 7, device)
+    for n in (12, 10):
+        c.out.fill_(7.0)
+        c.starts[-1] = n
+        att.rows(c.cache, c.q, c.out, lens, table, starts=c.starts, lse=c.lse)
+        torch.cuda.synchronize()
+        assert (c.out[n:] == 7.0).all() and (c.out[:n] != 7.0).any((1, 2)).all()
+
+
+@pytest.mark.parametrize("heads", [4, 128])  # few rows and heads of a prefix, and many
+def test_shared_past_its_bounds_gives_nan(device, heads):
     g = np.random.default_rng(23)
-    spec = ([200, 60, 90], [2, 1, 2], [10, 20, 30, 40, 50], [1] * 5, 4, 2, 32, 16, "i8", "bf16")
+    spec = ([200, 60, 90], [2, 1, 2], [10, 20, 30, 40, 50], [1] * 5, heads, 2, 32, 16, "i8", "bf16")
 
     def nan_rows(rows):
         got = np.isnan(F.as64(c.out)).all((1, 2)) & np.isnan(F.as64(c.lse)).all(1)
@@ -153,6 +186,14 @@ def test_shared_past_its_bounds_gives_nan(device):
     nan_rows([0, 1])
     c.call(max_len=45)
     nan_rows([4])
+    c.t["prefix_lens"][0] = 2 ** 31 - 1
+    c.call()
+    nan_rows([0, 1])
+    c = Case(g, device, *spec)
+    c.t["prefix_lens"][0] = -5  # as none: the rows see their own tokens
+    c.call()
+    nan_rows([])
+    attend_check(c.q[:1], c.out[:1], c.lse[:1], [10], [1], [tuple(x[200:] for x in c.stored[0])], "i8", "bf16", 0, 32)
     c.prefix_table[1, 3] = 10 ** 6  # no page of the cache
     c.table[3, 0] = -1
     c.call()
