@@ -32,6 +32,10 @@ constexpr int DRAFT_STORED = 0x0F70; // s_waitcnt vmcnt(0)
 __device__ inline float positive(float p) { return p > 0.0f && p < INFINITY ? p : 0.0f; }
 __device__ inline double probability(float p) { return (double)positive(p); }
 
+// What the running sum has to pass. A draw of 1 or more or NaN passes none, also where rounding brings a running sum above
+// the total.
+__device__ inline double draft_border(float draw, double total) { return draw < 1.0f ? fmax((double)draw * total, 0.0) : INFINITY; }
+
 // Inclusive sums over the wave in lane order.
 __device__ inline double wave_scan(double x) {
     const uint32_t lane = threadIdx.x % 64;
@@ -230,8 +234,8 @@ __global__ void __launch_bounds__(DRAFT_THREADS) k_drafts(DraftArgs a) {
         for (uint32_t i = 0; i < PER; i++) sum += part[i];
         block_scan(sum, waves, total);
         if (!(total > 0.0)) continue;
-        const double border = fmax((double)draw * total, 0.0); // NaN is 0 here, and passes nothing below
-        const uint32_t c = block_pick(part, 0.0, draw == draw ? border : total, waves, mins);
+        const double border = draft_border(draw, total);
+        const uint32_t c = block_pick(part, 0.0, border, waves, mins);
         // The sum of the chunks before it.
         double before = 0.0;
 #pragma unroll
@@ -243,7 +247,7 @@ __global__ void __launch_bounds__(DRAFT_THREADS) k_drafts(DraftArgs a) {
         for (uint32_t j = 0; j < QUADS; j++) load4(c * DRAFT_CHUNK + tid * DRAFT_EACH + 4 * j, less, x[j], y[j]);
 #pragma unroll
         for (uint32_t j = 0; j < QUADS; j++) left4(c * DRAFT_CHUNK + tid * DRAFT_EACH + 4 * j, less, x[j], y[j], left + 4 * j);
-        token = (int32_t)(c * DRAFT_CHUNK + block_pick(left, all, draw == draw ? border : INFINITY, waves, mins));
+        token = (int32_t)(c * DRAFT_CHUNK + block_pick(left, all, border, waves, mins));
         break;
     }
     draft_write(a, s, d, accepted, token);
@@ -260,7 +264,7 @@ __global__ void __launch_bounds__(DRAFT_THREADS) k_drafts_lists(DraftArgs a) {
     const uint32_t s = blockIdx.x, tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
     const DraftSpan d = draft_span(a, s);
     const float draw = a.draws[s];
-    const auto kept = [](const rl_probs &x, uint64_t row) { return (uint32_t)min((uint64_t)x.kept[row], x.row_stride); };
+    const auto kept = [](const rl_probs &x, uint64_t row) { return (uint32_t)min(min((uint64_t)x.kept[row], x.row_stride), (uint64_t)1 << 31); };
     // A token's probability in a list, by a wave. The first 64 entries are loaded before it is known how many there are.
     struct Head {
         uint32_t id, n;
@@ -372,7 +376,7 @@ __global__ void __launch_bounds__(DRAFT_THREADS) k_drafts_lists(DraftArgs a) {
             total += all;
         }
         if (!(total > 0.0)) continue;
-        const double border = draw == draw ? fmax((double)draw * total, 0.0) : INFINITY;
+        const double border = draft_border(draw, total);
         double base = 0.0;
         uint32_t final = DRAFT_NONE; // the last that can be drawn so far
         for (uint32_t at = 0; at < n; at += LIST_CHUNK) {

@@ -167,6 +167,23 @@ def test_rows_and_uniforms_at_their_ends(device):
               None if q is None else other, None if q is None else all_of(n))
 
 
+@pytest.mark.parametrize("vocab", [700, 9000, 400000])
+def test_draws_of_one_or_more_take_the_last(device, vocab):
+    # The last probability is far below the sum's last bit, so running sums in any order may pass the total before it.
+    g = np.random.default_rng(vocab)
+    n = 12
+    target = probs(g, n, vocab, 1.0)
+    target[:, -3] = 1e-30
+    target[:, -2:] = 0.0
+    draws = np.array([1.0, float("nan"), 2.0, float("inf")] * 3, np.float32)
+    none = np.zeros(0)
+    _, tokens = check(device, [0] * n, target, None, none, none, draws, vocab)
+    assert tokens == [vocab - 3] * n
+    ids = np.tile(np.arange(vocab, dtype=np.int32), (n, 1))
+    _, tokens = check(device, [0] * n, target, None, none, none, draws, vocab, ids, np.full(n, vocab, np.int32))
+    assert tokens == [vocab - 3] * n
+
+
 def test_accepted_borders_are_exact(device):
     # u q against p where they are one unit apart or equal: products of f32 values are exact in f64.
     g = np.random.default_rng(9)
