@@ -2,8 +2,9 @@
  * rl_mixers.h — C ABI of the MI355X (gfx950) token mixers: what the layers
  * between the embedding lookup and the output head (rl_head.h) do across the
  * tokens of a sequence. Rotary positions, a paged key-value cache that is
- * quantised as it is written, attention of new tokens over that cache, and the
- * gated delta rule.
+ * quantised as it is written, attention of new tokens over that cache, also behind
+ * prefixes that sequences share, the gated delta rule, the short causal convolution
+ * and the selective state space scan.
  *
  * Conventions as in rl_sampler.h: status codes, rl_sampler_last_error() for the
  * message, stream-ordered calls that return before the kernels finish, one
@@ -165,7 +166,7 @@ int rl_attention_rows(rl_attention *attention, const rl_kv_cache *cache, const r
  * those of their own tokens, which begin a page: every row sees its whole prefix and its
  * own sequence's tokens up to its own, as above without a window. max_prefix bounds the
  * tokens of any one prefix (0: the handle's max_len); past it the rows of the group are
- * NaN. rows * q_heads at most 2^20. */
+ * NaN. Rows from starts[seqs] on are not written. rows * q_heads at most 2^20. */
 int rl_attention_shared(rl_attention *attention, const rl_kv_cache *cache, const rl_heads *q, const rl_heads *out,
                         float *lse, uint32_t rows, const int32_t *starts, const int32_t *lens, uint32_t seqs,
                         const int32_t *pages, uint32_t table_width, const int32_t *group_starts,
@@ -233,7 +234,8 @@ void rl_conv_destroy(rl_conv *conv);
  * among them if it is shorter, in states[slots_out[s]] (nowhere if that is negative),
  * under the rules of rl_delta_rows: the two may be equal; else no slot that a sequence
  * reads is one that another writes, and none is written twice. A slot from state_slots
- * on reads as NaN and is not written. A sequence without rows passes its state on. */
+ * on reads as NaN and is not written. A sequence without rows passes its state on, and
+ * rows from starts[seqs] on are not written. */
 int rl_conv_rows(rl_conv *conv, const rl_heads *x, const rl_heads *out, void *states, uint64_t state_slots,
                  const int32_t *slots_in, const int32_t *slots_out, const int32_t *starts, uint32_t rows, uint32_t seqs,
                  void *stream);
@@ -262,7 +264,8 @@ void rl_scan_destroy(rl_scan *scan);
  * rows of any one sequence (0: as many as the call has); it may be any number, since it
  * only picks the form that is used for all of them: one token after the other, or long
  * sequences in pieces side by side. Both are as exact as f32 sums, but do not give the
- * same bits. An infinity may read as NaN, and so may a dt + dt_bias of 2^127 or more. */
+ * same bits. An infinity may read as NaN, and so may a dt + dt_bias of 2^127 or more.
+ * Rows from starts[seqs] on are not written. */
 int rl_scan_rows(rl_scan *scan, const rl_heads *x, const rl_heads *dt, const rl_heads *z, const rl_heads *b,
                  const rl_heads *c, const rl_heads *out, float *states, uint64_t state_slots, const int32_t *slots_in,
                  const int32_t *slots_out, const int32_t *starts, uint32_t rows, uint32_t seqs, int softplus,

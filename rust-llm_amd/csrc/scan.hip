@@ -119,6 +119,10 @@ int rl_scan_rows(rl_scan *h, const rl_heads *x, const rl_heads *dt, const rl_hea
             return fail(RL_ERR_ARGUMENT, "b and c must have the handle's groups and state_dim");
     for (const rl_heads *t : {dt, z ? z : x, b, c, out})
         if (t->dtype != x->dtype) return fail(RL_ERR_ARGUMENT, "the tensors of a call have one type");
+    for (const rl_heads *t : {x, dt, z ? z : x})
+        if (rows > 1 && t->data == out->data && t->row_stride != out->row_stride)
+            return fail(RL_ERR_ARGUMENT, "in place needs the same strides");
+    if (rows && (out->data == b->data || out->data == c->data)) return fail(RL_ERR_ARGUMENT, "out must not be b or c");
     if (!starts && seqs != rows) return fail(RL_ERR_ARGUMENT, "without starts there is one row a sequence");
     if (rows && !seqs) return fail(RL_ERR_ARGUMENT, "rows without a sequence");
     if (rows > h->max_rows) return fail(RL_ERR_CAPACITY, "rows above the handle's max_rows");

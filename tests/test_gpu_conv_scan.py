@@ -290,6 +290,25 @@ def test_captured_calls_and_another_stream(device, what):
         assert float((out.float() * 0).sum()) == 0.0  # the program's own work between the replays
 
 
+@pytest.mark.parametrize("most", [1, 40, 700])  # token by token, whole sequences, pieces
+def test_rows_behind_the_last_sequence_stay(device, most):
+    g = np.random.default_rng(most)
+    lens, rows, channels = [most, 1, most], 2 * most + 20, 96
+    at = 2 * most + 1
+    starts, slots = i32([0, most, most + 1, at], device), i32([0, 1, 2], device)
+    x, dt = (randn(g, (rows, channels), "f32", device) for _ in range(2))
+    b, c = (randn(g, (rows, 2, 16), "f32", device) for _ in range(2))
+    conv = M.DeviceConv(torch.ones(channels, 4))
+    scan = M.DeviceScan(rows, 3, -torch.ones(channels, 16), groups=2)
+    for call, shape in ((lambda y, p: conv.rows(x, y, p, slots, slots, starts), (4, 3, channels)),
+                        (lambda y, p: scan.rows(x, dt, b, c, y, p, slots, slots, starts, most_rows=most), (4, channels, 16))):
+        y, states = torch.full_like(x, 7.0), torch.full(shape, 2.0, device=device)
+        call(y, states)
+        torch.cuda.synchronize()
+        assert (y[at:] == 7.0).all() and (y[:at] != 7.0).any(1).all()
+        assert (states[3] == 2.0).all() and all((states[i] != 2.0).any() for i in range(3))
+
+
 def test_refusals(device):
     conv = M.DeviceConv(torch.zeros(8, 4))
     scan = M.DeviceScan(4, 2, torch.zeros(8, 16), groups=2)
@@ -313,6 +332,11 @@ def test_refusals(device):
     refused(R.RL_ERR_ARGUMENT, scan.rows, x, x, b[:, :1], b, y, pool, s2, s2, starts)
     refused(R.RL_ERR_ARGUMENT, scan.rows, x, x, b, b[..., :8], y, pool, s2, s2, starts)
     refused(R.RL_ERR_ARGUMENT, scan.rows, x, x, b, b, y, pool, s2, s2)
+    over = torch.zeros(8, 8, device=device)
+    refused(R.RL_ERR_ARGUMENT, scan.rows, over[::2], x, b, b, over[:4], pool, s2, s2, starts)  # in place, but not row by row
+    refused(R.RL_ERR_ARGUMENT, scan.rows, x, over[::2], b, b, over[:4], pool, s2, s2, starts)
+    refused(R.RL_ERR_ARGUMENT, scan.rows, x, x, b, b, over[:4], pool, s2, s2, starts, z=over[::2])
+    refused(R.RL_ERR_ARGUMENT, scan.rows, x, x, b, b, b.view(-1, 8)[:4], pool, s2, s2, starts)
     refused(R.RL_ERR_CAPACITY, scan.rows, *(torch.cat([t, t]) for t in (x, x, b, b, y)), pool, s2, s2, starts)
     refused(R.RL_ERR_CAPACITY, scan.rows, x, x, b, b, y, pool, i32([0, 1, -1], device), i32([0, 1, -1], device), i32([0, 1, 2, 4], device))
     # Nothing to do is no error, and a call without rows passes states on.
