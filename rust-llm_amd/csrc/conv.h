@@ -4,9 +4,16 @@
 //
 // A wave takes 512 channels (16-bit types; 256 of f32) of a run of rows and keeps the
 // W - 1 rows before the current one in registers: a row is read once but for the W - 1
-// that a run reads again of the one before. Bound by HBM. The rows before a sequence's
-// first are its state; the run with the first row reads it and also writes the new one,
-// so a slot may be read and written by one call.
+// that a run reads again of the one before. The rows before a sequence's first are its
+// state; the run with the first row reads it and also writes the new one, so a slot may
+// be read and written by one call.
+//
+// Bound by HBM for long prompts (8192 rows of 8192 bf16 channels, width 4: 44.3 us, 6.1
+// TB/s; rows that are not aligned to 16 bytes 60.2), below that by the instructions of
+// a wave, some 500 cycles a row, of which the exponential and the reciprocal of the
+// activation are a third. Weights are loaded as vectors: one by one, lanes 32 bytes apart,
+// they took twice the time of all the rows (88 us for the same, 16.5 for 1024 rows
+// where it is 9.0 now).
 #pragma once
 #include "row_blocks.h"
 
@@ -89,13 +96,21 @@ __global__ void __launch_bounds__(CONV_LANES) k_conv(ConvArgs a) {
 #pragma unroll
     for (int j = 0; j < W - 1; j++) history[j] = t0 ? load(x + (uint64_t)(t0 - (W - 1) + j) * a.x_row) : before(j);
     float w[W][V], bias[V];
+    const auto weights = [&](const float *from, float *to) {
+        if constexpr (WIDE)
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        const uint32_t c = min(channel(i), a.channels - 1);
-        bias[i] = a.bias[c];
+            for (int i = 0; i < V; i += 4) {
+                const f32x4 v = *(const f32x4 *)(from + channel(i));
 #pragma unroll
-        for (int j = 0; j < W; j++) w[j][i] = a.weight[(uint64_t)j * a.channels + c];
-    }
+                for (int k = 0; k < 4; k++) to[i + k] = v[k];
+            }
+        else
+#pragma unroll
+            for (int i = 0; i < V; i++) to[i] = from[min(channel(i), a.channels - 1)];
+    };
+    weights(a.bias, bias);
+#pragma unroll
+    for (int j = 0; j < W; j++) weights(a.weight + (uint64_t)j * a.channels, w[j]);
     if (!t0) {
         const int32_t to = a.slots_out[r.seq];
         if (to >= 0 && (uint64_t)to < a.state_slots) {

@@ -19,9 +19,10 @@ struct rl_conv {
 
 namespace {
 
-// Rows of a run: 32, which reads W - 1 of 35 twice, where that leaves two waves a SIMD or more; else 8, the least that holds
-// the longest state.
-constexpr uint32_t CONV_LONG = 32, CONV_SHORT = 8, CONV_WAVES = 2048;
+// Rows of a run: the least that holds the longest state. The rows that are read again are still in the L2 and short runs
+// give many waves; us with runs of 8 / 16 / 32, bf16, width 4: 512 x 8192 6.0 / 7.8 / 11.4, 2048 x 8192 14.8 / 14.9 / 17.8,
+// 8192 x 8192 44.3 / 47.7 / 47.2, 8192 x 5120 32.1 / 31.8 / 30.7; width 8 51.1 / 56.6 / 57.1; f32, 1024 x 2027 7.1 / 10.0 / 15.0.
+constexpr uint32_t CONV_RUN = CONV_MAX_WIDTH;
 
 template <typename T, int W, bool WIDE>
 void launch_conv(const ConvArgs &a, uint32_t blocks, bool silu, hipStream_t s) {
@@ -118,7 +119,7 @@ int rl_conv_rows(rl_conv *h, const rl_heads *x, const rl_heads *out, void *state
     const bool vectors = wide(x) && wide(out) && (uintptr_t)states % 16 == 0 && h->channels % vector == 0;
     const uint32_t per = CONV_LANES * (vectors ? vector : 4);
     a.columns = (h->channels + per - 1) / per;
-    a.runs = row_blocks((uint64_t)(rows / CONV_LONG) * a.columns >= CONV_WAVES ? CONV_LONG : CONV_SHORT);
+    a.runs = row_blocks(CONV_RUN);
     const uint64_t blocks = (uint64_t)row_block_count(rows, seqs, a.runs.size) * a.columns;
     if (blocks > 1u << 25) return fail(RL_ERR_CAPACITY, "too many rows times channels in a call");
     with_type(x->dtype, [&](auto t) {
