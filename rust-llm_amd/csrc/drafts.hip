@@ -24,7 +24,8 @@ struct rl_drafts {
 
 namespace {
 
-// Workgroups that the chunks of a call are shared among.
+// Workgroups that the chunks of a call are shared among: each finds the accepted drafts first, so few do that more seldom,
+// but they have to fill the device. 64 sequences of 61 chunks, us: 512 27.7, 1024 28.2, 2048 51.5.
 constexpr uint32_t DRAFT_FILL = 1024;
 
 // What is wrong with a call's probabilities, or null.

@@ -143,7 +143,7 @@ uint32_t attend_tiles(uint64_t tokens) { return (uint32_t)((tokens + ATTEND_TILE
 // this holds parts for have row blocks enough to fill the device. Without a limit 8192 rows of 32 heads and lengths up to
 // 131072 took 11.7 GB, a million tokens 35.
 constexpr uint64_t ATTEND_ROOM = 1u << 20;
-// And at least: a workgroup of 128 rows a CU.
+// And at least, 17 MB for heads of 128: a workgroup of 128 rows a CU.
 constexpr uint64_t ATTEND_LEAST = 1u << 15;
 
 // Parts that lengths up to `tiles` need at the least; one sequence has no others to wait for.
@@ -153,7 +153,7 @@ uint32_t attend_least_parts(uint32_t tiles, uint32_t seqs) {
     return std::min(n, ATTEND_MAX_PARTS);
 }
 
-// Parts of a shared prefix at most: each of a row's columns is joined by one thread, which loads them one after the other.
+// Parts of a shared prefix at most: each of a row's columns is joined by one thread, which loads them eight at a time.
 constexpr uint32_t SHARED_PARTS = 16;
 
 // Rows times heads of a group, on average, from which the kernel whose waves share each tile is taken. Behind 8192 tokens, 8
@@ -166,8 +166,17 @@ constexpr uint64_t SHARED_MANY = 96;
 // sequences of 32 / 8 heads of 128: 16.7 / 18.5, 512 tokens 20.8 / 18.9.
 constexpr uint32_t SHARED_OWN = 128;
 
-// Tiles that a workgroup's start and end cost.
-constexpr uint32_t SHARED_START = 4;
+// What a workgroup's start and end cost, in tiles; with two row tiles a wave a tile costs 1.3 times as much, start and end 2
+// tiles more with heads of 64 and 4 with 128. us, one row tile / two, 32 / 8 heads, 64 rows behind 4096, 8192 and 16384
+// tokens: 128 dims bf16 27.4 / 30.7, 37.8 / 38.8, 57.0 / 51.1, int8 28.7 / 30.9, 40.4 / 38.8, 62.9 / 53.8, 64 dims bf16
+// 20.9 / 21.9, 28.0 / 27.3, 43.2 / 38.3; 160 rows behind 2048 and 4096: 41.9 / 43.9, 55.8 / 52.0; 37.9 / 39.6, 53.6 / 49.1;
+// 27.6 / 26.4, 36.9 / 34.1.
+constexpr double SHARED_START = 4.0, SHARED_TWO = 1.3;
+// Several groups: what the prefixes have on average of the longest one's tokens, and what of a round is lost since workgroups
+// without tokens lie between the others. Three groups, of 8001, 4000 and 2667 tokens, bf16, us: 480 rows in 2 / 6 parts 144.8 /
+// 130.1 (as many rounds as equal lengths would take say 2), 288 rows in 3 / 4 / 5 parts 110.4 / 95.3 / 114.1. Eight alike, of
+// 4096 tokens and 32 rows, 4 / 5 parts 66.5 / 67.2.
+constexpr double SHARED_MEAN = 0.6, SHARED_UNEVEN = 0.2;
 
 // Row blocks of all groups, at most.
 uint64_t shared_blocks(uint64_t rows, uint32_t groups, uint32_t size) {
@@ -593,14 +602,17 @@ int rl_attention_shared(rl_attention *h, const rl_kv_cache *cache, const rl_head
     if (many) {
         const uint32_t tile = shared_tile(attend_dim(h->dim)), tiles = (uint32_t)(((uint64_t)shared.max_len + tile - 1) / tile);
         // Of one row tile a wave and two, and of the numbers of parts, what takes the least time: rounds of a workgroup a CU,
-        // each a part's tiles, which cost two row tiles 1.7 times as much as one.
+        // each a part's tiles. Several groups' blocks are counted as the fewest they may be, and their prefixes as of different
+        // lengths, SHARED_MEAN of the longest together.
         double least = INFINITY;
         for (const uint32_t row_tiles : {1u, 2u}) {
             if (row_tiles > (q->dtype == RL_F32 ? shared_row_tiles<float>(attend_dim(h->dim)) : shared_row_tiles<half_t>(attend_dim(h->dim)))) continue;
-            const uint64_t blocks = shared_blocks(shared_rows, groups, 64 * row_tiles), columns = (uint64_t)h->kv_heads * blocks;
+            const uint64_t blocks = shared_blocks(shared_rows, groups, 64 * row_tiles), columns = h->kv_heads * std::max<uint64_t>((shared_rows + 64 * row_tiles - 1) / (64 * row_tiles), groups);
+            const double each = row_tiles == 2 ? SHARED_TWO : 1.0, ends = SHARED_START + (row_tiles == 2 ? attend_dim(h->dim) / 32 : 0);
             for (uint32_t parts = 1; parts <= std::min<uint64_t>(most_parts, tiles); parts++) {
                 const uint64_t part_tiles = (tiles + parts - 1) / parts;
-                const double time = (double)((columns * parts + CUS - 1) / CUS) * (part_tiles + SHARED_START) * (row_tiles == 2 ? 1.7 : 1.0);
+                const double full = (double)(columns * parts) / CUS, rounds = std::ceil(groups == 1 ? full : full * SHARED_MEAN + SHARED_UNEVEN);
+                const double time = rounds * (part_tiles * each + ends);
                 if (time >= least) continue;
                 least = time, wider = row_tiles == 2;
                 shared.blocks = (uint32_t)blocks, shared.part_tiles = (uint32_t)part_tiles, shared.parts = (uint32_t)((tiles + part_tiles - 1) / part_tiles);

@@ -27,8 +27,12 @@ struct rl_scan {
 
 namespace {
 
-// Rows of a sequence up to which one token after the other is the faster form.
-constexpr uint32_t SCAN_SHORT = 16;
+// k_scan_steps or k_scan: the first has a quarter of the state values a lane, so a shorter way in and out, but forms each
+// softplus and gate four times as often. It is taken for sequences of up to SCAN_FEW tokens, and up to SCAN_SHORT while
+// the call's tokens are no more than SCAN_WORK waves together (each a token of 64 lanes). us, steps / other, 5120 channels
+// of 16 bf16: one sequence of 8 tokens 5.8 / 7.4, of 32 15.8 / 17.1; 8 of 8 7.9 / 8.1; 16 of 4 7.2 / 8.6, of 8 10.6 / 10.0,
+// of 16 18.1 / 14.5; 64 of 2 12.9 / 16.3, of 4 18.5 / 17.9, of 8 30.3 / 21.1; 256 of 2 41.0 / 50.2, of 4 65 / 53.
+constexpr uint32_t SCAN_FEW = 3, SCAN_SHORT = 32, SCAN_WORK = 36864;
 // Workgroups that pieces are made for, the fewest tokens of one, and the most pieces of a sequence: a piece's first state is
 // made of the ends of all before it.
 constexpr uint64_t SCAN_FILL = 1024, SCAN_MOST = 64;
@@ -147,9 +151,10 @@ int rl_scan_rows(rl_scan *h, const rl_heads *x, const rl_heads *dt, const rl_hea
     a.wide = wide(b) && wide(c);
     a.ends = h->ends, a.steps = h->steps;
     const uint32_t most = !starts ? 1 : most_rows ? std::min(most_rows, rows) : rows;
-    const bool steps = most <= SCAN_SHORT;
+    const uint32_t lanes = scan_lanes(h->state, 4);
+    const bool steps = most <= SCAN_FEW || (most <= SCAN_SHORT && (uint64_t)rows * h->channels * lanes / 64 <= SCAN_WORK);
     if (steps) {
-        const uint32_t per = SCAN_THREADS / scan_lanes(h->state, 4);
+        const uint32_t per = SCAN_THREADS / lanes;
         a.columns = (h->channels + per - 1) / per;
     } else {
         a.columns = h->columns;
