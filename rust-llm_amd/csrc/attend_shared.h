@@ -18,7 +18,7 @@
 // and a tile of 64 tokens and 32 rows of 128 bf16 is 96 products of 16 cycles and about
 // 400 vector instructions of 4 or 5. 256 rows a key-value head, 8 heads of 128, 16384
 // tokens bf16: 46.9 us, 366 TFLOP/s (k_attend 106 us). 640 rows, 8001 tokens int8 in
-// pages of 24, and two prefixes of a half and a third: 129 us, 298 TFLOP/s.
+// pages of 24, and two prefixes of a half and a third: 116 us, 332 TFLOP/s.
 #pragma once
 #include "attend.h"
 

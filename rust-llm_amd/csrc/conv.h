@@ -8,8 +8,9 @@
 // state; the run with the first row reads it and also writes the new one, so a slot may
 // be read and written by one call.
 //
-// Bound by HBM for long prompts (8192 rows of 8192 bf16 channels, width 4: 44.3 us, 6.1
-// TB/s; rows that are not aligned to 16 bytes 60.2), below that by the instructions of
+// Bound by HBM for long prompts (8192 rows of 8192 bf16 channels, width 4: 52 us, 5.1
+// TB/s, 44.3 again over the same rows; rows not aligned to 16 bytes 60.2), below that by
+// the instructions of
 // a wave, some 500 cycles a row, of which the exponential and the reciprocal of the
 // activation are a third. Weights are loaded as vectors: one by one, lanes 32 bytes apart,
 // they took twice the time of all the rows (88 us for the same, 16.5 for 1024 rows

@@ -9,7 +9,7 @@
 // row of each side: 64 of 248320 tokens 28.0 us, 4.5 TB/s. For few by the chain of loads
 // (starts, drafted token, two gathers, a chunk, the arrival, the chunk sums, a chunk
 // again): 9.4 us for one of 151936. Lists: a workgroup a sequence, the same chain without
-// the arrival, 8.2 us for 64 of up to 8 drafts and 64 entries.
+// the arrival, 7.8 us for 64 of up to 8 drafts and 64 entries.
 #pragma once
 #include "mix_types.h"
 #include "rl_drafts.h"
