@@ -2,3 +2,4 @@
 #include "attend_launch.h"
 
 template void rl::launch_attend<rl::bhalf_t>(const rl::AttendArgs &, rl::AttendMode, uint32_t, uint32_t, uint32_t, hipStream_t);
+template void rl::launch_attend_both<rl::bhalf_t>(const rl::AttendArgs &, const rl::AttendArgs &, uint32_t, uint32_t, uint32_t, hipStream_t);

@@ -161,10 +161,16 @@ constexpr uint32_t SHARED_PARTS = 16;
 // 31.4 / 29.0, f32 queries 27.1 / 32.9, 35.6 / 34.7; 256 dims 38.5 / 40.4, 54.8 / 42.6; 64 dims 17.1 / 21.2, 21.1 / 21.6.
 constexpr uint64_t SHARED_MANY = 96;
 
-// Own tokens up to which the launch that joins parts costs more than they save: behind a prefix of 1009 tokens, 8 sequences of
+// Own tokens up to which, in a launch of their own, the one that joins parts costs more than they save: behind a prefix of 1009 tokens, 8 sequences of
 // 16 / 4 heads of 256 bf16, us, one part / several: 128 tokens 18.6 / 20.3, 256 21.0 / 20.5, 512 25.8 / 21.0; behind 4096, 4
 // sequences of 32 / 8 heads of 128: 16.7 / 18.5, 512 tokens 20.8 / 18.9.
 constexpr uint32_t SHARED_OWN = 128;
+
+// Workgroups of the sequences' own tokens up to which they go in one launch with the prefix's, and a second one joins both.
+// us, first the prefix and then what joins it / both at once: behind 1000 tokens 8 sequences of up to 64 tokens, 16 / 4 heads
+// of 256 bf16 17.8 / 12.8, of up to 512 20.4 / 13.2; 16 of 32 / 8 heads of 128 13.9 / 11.8, 17.9 / 13.8; 64 of 8 / 8 heads, 512
+// workgroups, 14.6 / 15.0, 26.9 / 24.2, behind 8192 29.0 / 26.0; 90 of them int8, 720 workgroups, 17.1 / 19.0, 28.1 / 27.8.
+constexpr uint64_t SHARED_BOTH = 512;
 
 // What a workgroup's start and end cost, in tiles; with two row tiles a wave a tile costs 1.3 times as much, start and end 2
 // tiles more with heads of 64 and 4 with 128. us, one row tile / two, 32 / 8 heads, 64 rows behind 4096, 8192 and 16384
@@ -585,17 +591,18 @@ int rl_attention_shared(rl_attention *h, const rl_kv_cache *cache, const rl_head
     DeviceGuard guard(h->device);
     if (!guard.ok) return fail(RL_ERR_DEVICE, "cannot select the handle's device");
     AttendArgs own = attend_args(h, cache, q, out, lse, rows, starts, lens, seqs, pages, table_width, scale, most_rows, max_len);
-    const uint64_t expanded = (uint64_t)own.most_rows * own.group;
-    const bool two = attend_two(cache->format, h->dim, (expanded + 15) / 16, (uint64_t)seqs * h->kv_heads);
+    const uint64_t expanded = (uint64_t)own.most_rows * own.group, columns = (uint64_t)seqs * h->kv_heads;
     AttendArgs shared = attend_args(h, cache, q, out, lse, rows, starts, prefix_lens, groups, prefix_pages, prefix_width, scale,
                                     rows, max_prefix);
     shared.group_starts = own.group_starts = group_starts, shared.group_end = seqs, own.group_end = groups;
     shared.most_rows = rows;
     // The prefix's parts are joined by each row's own workgroup, so they are few. Room is theirs first: a sequence's own
     // tokens in one part need none.
-    const uint64_t most_parts = std::min<uint64_t>(room, SHARED_PARTS), shared_rows = (uint64_t)rows * own.group;
-    const bool many = shared_rows >= SHARED_MANY * groups;
-    const bool shared_two = attend_two(cache->format, h->dim, (shared_rows + 15) / 16, (uint64_t)groups * h->kv_heads);
+    const uint64_t shared_rows = (uint64_t)rows * own.group;
+    const bool many = shared_rows >= SHARED_MANY * groups, both = !many && room > 1 && columns * ((expanded + 15) / 16) <= SHARED_BOTH;
+    const uint64_t most_parts = std::min<uint64_t>(room - both, SHARED_PARTS);
+    const bool two = !both && attend_two(cache->format, h->dim, (expanded + 15) / 16, columns);
+    const bool shared_two = !both && attend_two(cache->format, h->dim, (shared_rows + 15) / 16, (uint64_t)groups * h->kv_heads);
     shared.packed = 1;
     uint32_t own_groups, shared_groups;
     bool fits = true, wider = false;
@@ -628,14 +635,16 @@ int rl_attention_shared(rl_attention *h, const rl_kv_cache *cache, const rl_head
     }
     // A sequence's own tokens go in one part, which its workgroup joins with the prefix's by itself, up to SHARED_OWN.
     const uint64_t left = room - shared.parts;
-    const uint64_t own_room = own.max_len <= SHARED_OWN || left <= 1 ? 1 : std::min<uint64_t>(left, ATTEND_MAX_PARTS - SHARED_PARTS);
+    const uint64_t own_room = (own.max_len <= SHARED_OWN && !both) || left <= 1 ? 1 : std::min<uint64_t>(left, ATTEND_MAX_PARTS - SHARED_PARTS);
     fits = fits && attend_shape(own, h, attend_blocks(own, h, two), attend_held(q, cache, h, two), own_room, &own_groups);
     if (!fits) return fail(RL_ERR_CAPACITY, "too many sequences times row blocks in a call");
-    own.shared = shared.shared = own.parts > 1 ? own.parts : 0;
+    own.joins = own.parts == 1 && !both;
+    own.shared = shared.shared = own.joins ? 0 : own.parts;
     own.shared_parts = shared.shared_parts = shared.parts;
     own.stride = shared.stride = own.shared + shared.parts;
     with_type(q->dtype, [&](auto t) {
         const hipStream_t s = static_cast<hipStream_t>(stream);
+        if (both) return launch_attend_both<decltype(t)>(shared, own, cache->format, shared_groups, own_groups, s);
         if (many) launch_attend_shared<decltype(t)>(shared, cache->format, wider, shared_groups, s);
         else launch_attend<decltype(t)>(shared, ATTEND_PREFIX, cache->format, shared_two ? 2 : 1, shared_groups, s);
         launch_attend<decltype(t)>(own, ATTEND_JOINED, cache->format, two ? 2 : 1, own_groups, s);

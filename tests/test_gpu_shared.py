@@ -89,6 +89,11 @@ SHARED = [
     ([65, 64, 63, 1], [40, 40, 40, 40], [1 + i % 5 for i in range(160)], [1] * 160, 8, 2, 80, 16, "f16", "f16"),
     ([300], [31], [70] + [3] * 30, [60] + [1] * 30, 8, 2, 128, 16, "bf16", "bf16"),  # one sequence of many rows among single ones
     ([90, 31], [20, 20], [600] * 40, [1] * 40, 8, 2, 64, 16, "i8", "bf16"),  # more tokens of their own than shared ones
+    # Too many workgroups for one launch, few rows of each group: joined by the sequence's own, in parts, two row tiles.
+    ([100 + 7 * i for i in range(40)], [2] * 40, [1 + i for i in range(80)], [1] * 80, 8, 8, 64, 16, "bf16", "bf16"),
+    ([50 + 3 * i for i in range(40)], [2] * 40, [150 + 3 * i for i in range(80)], [1] * 80, 8, 8, 128, 24, "i8", "f32"),
+    ([500 - 9 * i for i in range(20)], [4] * 20, [2 + i for i in range(80)], [2] * 80, 32, 8, 64, 16, "f8", "f16"),
+    ([200] * 20, [4] * 20, [30] * 80, [5] * 80, 16, 8, 48, 7, "f16", "f16"),
 ]
 
 
