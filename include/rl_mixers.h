@@ -264,8 +264,9 @@ void rl_scan_destroy(rl_scan *scan);
  * rows of any one sequence (0: as many as the call has); it may be any number, since it
  * only picks the form that is used for all of them: one token after the other, or long
  * sequences in pieces side by side. Both are as exact as f32 sums, but do not give the
- * same bits. An infinity may read as NaN, and so may a dt + dt_bias of 2^127 or more.
- * Rows from starts[seqs] on are not written. */
+ * same bits. With softplus the lowest values of dt, and -infinity, are steps of 0, which
+ * leave the state as it is. Another infinity, also one that a product or sum overflows
+ * to, may read as NaN. Rows from starts[seqs] on are not written. */
 int rl_scan_rows(rl_scan *scan, const rl_heads *x, const rl_heads *dt, const rl_heads *z, const rl_heads *b,
                  const rl_heads *c, const rl_heads *out, float *states, uint64_t state_slots, const int32_t *slots_in,
                  const int32_t *slots_out, const int32_t *starts, uint32_t rows, uint32_t seqs, int softplus,

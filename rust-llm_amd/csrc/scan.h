@@ -35,11 +35,12 @@ constexpr uint32_t SCAN_THREADS = 256, SCAN_WAVES = 4;
 __device__ inline uint64_t scan_slot(uint32_t begin, RowBlocks pieces) { return 2 * (uint64_t)split_by(begin, pieces.size, pieces.inv).x; }
 inline uint64_t scan_slots(uint64_t pieces) { return 2 * pieces + 2; } // of a call of that many whole pieces
 
-// ln(1 + e^v), to f32's precision for every v.
+// ln(1 + e^v), to f32's precision for every v: 0 for the lowest ones and -infinity, NaN for NaN.
 __device__ inline float soft_plus(float v) {
     constexpr float L = 1.44269504088896341f, LOW = 1.92596299e-8f, LN2 = 0.693147180559945309f;
     const float m = -fabsf(v), p = m * L;
-    const float e = __builtin_amdgcn_exp2f(p), t = fmaf(e, (fmaf(m, L, -p) + m * LOW) * LN2, e);
+    // The rounding of m L is brought back while e^m is a normal number; below, m L may be infinite and its rounding with it.
+    const float e = __builtin_amdgcn_exp2f(p), t = p > -126.0f ? fmaf(e, (fmaf(m, L, -p) + m * LOW) * LN2, e) : e;
     // ln(1 + t) by the rounded sum u and what the rounding took, at most 2^-24: ln(u) + (1 + t - u) / u. The last division
     // by 1 to 2 is left out, which costs at most a unit in the last place.
     const float u = 1.0f + t;
