@@ -323,8 +323,9 @@ __global__ void __launch_bounds__(SHARED_THREADS, 2) k_attend_shared(AttendArgs 
                     q[rt][p][st][j] = (MK)(x[rt][st][j] * sign);
                     x[rt][st][j] -= (float)q[rt][p][st][j] * sign;
                 }
-        // Not zero, which would make NaN of a masked score: 2^-100 times any other is as good.
-        mult[rt] = fmaxf(fabsf(a.scale) * 1.44269504088896341f * unit_of, 0x1p-100f);
+        // Not zero, which would make NaN of a masked score: times 2^-149 every other is below 2^-21. NaN stays.
+        mult[rt] = fabsf(a.scale) * 1.44269504088896341f * unit_of;
+        if (mult[rt] == 0.0f) mult[rt] = 0x1p-149f;
     }
     f32x4 O[RT][VD];
     float top[RT], total[RT];
