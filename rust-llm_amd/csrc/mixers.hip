@@ -178,11 +178,15 @@ constexpr uint64_t SHARED_BOTH = 512;
 // 20.9 / 21.9, 28.0 / 27.3, 43.2 / 38.3; 160 rows behind 2048 and 4096: 41.9 / 43.9, 55.8 / 52.0; 37.9 / 39.6, 53.6 / 49.1;
 // 27.6 / 26.4, 36.9 / 34.1.
 constexpr double SHARED_START = 4.0, SHARED_TWO = 1.3;
-// Several groups: what the prefixes have on average of the longest one's tokens, and what of a round is lost since workgroups
-// without tokens lie between the others. Three groups, of 8001, 4000 and 2667 tokens, bf16, us: 480 rows in 2 / 6 parts 144.8 /
-// 130.1 (as many rounds as equal lengths would take say 2), 288 rows in 3 / 4 / 5 parts 110.4 / 95.3 / 114.1. Eight alike, of
-// 4096 tokens and 32 rows, 4 / 5 parts 66.5 / 67.2.
-constexpr double SHARED_MEAN = 0.6, SHARED_UNEVEN = 0.2;
+// Several groups, of whose rows and prefixes the host knows no more than the sum and the longest: they are counted as alike, their
+// workgroups by what they have to do in all, and at the end half a workgroup's time, when some CUs have nothing left. 27 shapes
+// of 2 to 20 groups, 32 to 640 rows of each and 1200 to 25000 tokens, heads of 64, 128 and 256 dims: a call takes longer than
+// with the best number of parts and row tiles by, on average / at most, in whole rounds on the right:
+//   prefixes alike                              16 % / 43 %    18 % / 64 %
+//   a half, a third and so on of the first one  12 % / 49 %    19 % / 109 %
+//   one ten times as long as the others          7 % / 44 %    26 % / 141 %
+//   one, or half of them, a tenth of the others  8 % / 44 %    14 % / 89 %
+constexpr double SHARED_END = 0.5;
 
 // Row blocks of all groups, at most.
 uint64_t shared_blocks(uint64_t rows, uint32_t groups, uint32_t size) {
@@ -609,20 +613,21 @@ int rl_attention_shared(rl_attention *h, const rl_kv_cache *cache, const rl_head
     if (many) {
         const uint32_t tile = shared_tile(attend_dim(h->dim)), tiles = (uint32_t)(((uint64_t)shared.max_len + tile - 1) / tile);
         // Of one row tile a wave and two, and of the numbers of parts, what takes the least time: rounds of a workgroup a CU,
-        // each a part's tiles. Several groups' blocks are counted as the fewest they may be, and their prefixes as of different
-        // lengths, SHARED_MEAN of the longest together.
+        // each a part's tiles.
         double least = INFINITY;
         for (const uint32_t row_tiles : {1u, 2u}) {
             if (row_tiles > (q->dtype == RL_F32 ? shared_row_tiles<float>(attend_dim(h->dim)) : shared_row_tiles<half_t>(attend_dim(h->dim)))) continue;
-            const uint64_t blocks = shared_blocks(shared_rows, groups, 64 * row_tiles), columns = h->kv_heads * std::max<uint64_t>((shared_rows + 64 * row_tiles - 1) / (64 * row_tiles), groups);
+            const uint64_t size = 64 * row_tiles, columns = h->kv_heads * groups * ((shared_rows + groups * size - 1) / (groups * size));
             const double each = row_tiles == 2 ? SHARED_TWO : 1.0, ends = SHARED_START + (row_tiles == 2 ? attend_dim(h->dim) / 32 : 0);
             for (uint32_t parts = 1; parts <= std::min<uint64_t>(most_parts, tiles); parts++) {
                 const uint64_t part_tiles = (tiles + parts - 1) / parts;
-                const double full = (double)(columns * parts) / CUS, rounds = std::ceil(groups == 1 ? full : full * SHARED_MEAN + SHARED_UNEVEN);
+                const double full = (double)(columns * parts) / CUS;
+                const double rounds = groups == 1 ? std::ceil(full) : std::max(full, 1.0) + SHARED_END;
                 const double time = rounds * (part_tiles * each + ends);
                 if (time >= least) continue;
                 least = time, wider = row_tiles == 2;
-                shared.blocks = (uint32_t)blocks, shared.part_tiles = (uint32_t)part_tiles, shared.parts = (uint32_t)((tiles + part_tiles - 1) / part_tiles);
+                shared.blocks = (uint32_t)shared_blocks(shared_rows, groups, size);
+                shared.part_tiles = (uint32_t)part_tiles, shared.parts = (uint32_t)((tiles + part_tiles - 1) / part_tiles);
             }
         }
         shared.group_inv = inverse_of(shared.group), shared.blocks_inv = inverse_of(shared.blocks), shared.heads_inv = inverse_of(h->kv_heads);
