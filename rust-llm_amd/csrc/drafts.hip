@@ -91,8 +91,7 @@ int rl_drafts_verify(rl_drafts *h, const rl_probs *target, const rl_probs *draft
         return fail(RL_ERR_ARGUMENT, "drafted, starts, uniforms, draws, accepted and tokens must be device pointers");
     // Chunks a workgroup: it has to find the row first, which several share, but few sequences want many workgroups.
     const uint32_t per = (uint32_t)std::min<uint64_t>(std::max<uint64_t>((uint64_t)seqs * h->chunks / DRAFT_FILL, 1), DRAFT_PER);
-    const uint32_t groups = (h->chunks + per - 1) / per;
-    if ((uint64_t)seqs * groups > 1u << 23) return fail(RL_ERR_CAPACITY, "too many sequences times tokens in a call");
+    const uint32_t groups = (h->chunks + per - 1) / per; // times 2^16 sequences: 2^22 workgroups at most
     DeviceGuard guard(h->device);
     if (!guard.ok) return fail(RL_ERR_DEVICE, "cannot select the handle's device");
     DraftArgs a{};
