@@ -312,8 +312,8 @@ __global__ void __launch_bounds__(SHARED_THREADS, 2) k_attend_shared(AttendArgs 
 #pragma unroll
                 for (int j = 0; j < 8; j++) x[rt][st][j] *= down;
         }
-        // The scale's sign goes to the queries: scores are then compared before they are scaled.
-        const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+        // The scale's sign goes to the queries: scores are then compared before they are scaled. So does NaN.
+        const float sign = a.scale < 0.0f ? -1.0f : a.scale >= 0.0f ? 1.0f : a.scale;
 #pragma unroll
         for (int p = 0; p < QP; p++)
 #pragma unroll
@@ -323,9 +323,8 @@ __global__ void __launch_bounds__(SHARED_THREADS, 2) k_attend_shared(AttendArgs 
                     q[rt][p][st][j] = (MK)(x[rt][st][j] * sign);
                     x[rt][st][j] -= (float)q[rt][p][st][j] * sign;
                 }
-        // Not zero, which would make NaN of a masked score: times 2^-149 every other is below 2^-21. NaN stays.
-        mult[rt] = fabsf(a.scale) * 1.44269504088896341f * unit_of;
-        if (mult[rt] == 0.0f) mult[rt] = 0x1p-149f;
+        // Not zero, which would make NaN of a masked score: times 2^-149 every other is below 2^-21.
+        mult[rt] = fmaxf(fabsf(a.scale) * 1.44269504088896341f * unit_of, 0x1p-149f);
     }
     f32x4 O[RT][VD];
     float top[RT], total[RT];
