@@ -57,8 +57,9 @@ void rl_drafts_destroy(rl_drafts *drafts);
  * uniforms f32 [drafts] and draws f32 [seqs] in [0, 1); a draw of 1 or more or NaN
  * takes the last token that can be drawn, one below 0 the first.
  *
- * accepted i32 [seqs], which like tokens must not overlap an input: drafts accepted. tokens i32 [drafts + seqs]: from starts[s] + s
- * on the accepted ones, the drawn one and -1 up to the next sequence's. */
+ * accepted i32 [seqs], which like tokens must not overlap an input: drafts accepted.
+ * tokens i32 [drafts + seqs]: from starts[s] + s on the accepted ones, the drawn one and
+ * -1 up to the next sequence's. */
 int rl_drafts_verify(rl_drafts *drafts_handle, const rl_probs *target, const rl_probs *draft, const int32_t *drafted,
                      const int32_t *starts, const float *uniforms, const float *draws, uint32_t drafts, uint32_t seqs,
                      int32_t *accepted, int32_t *tokens, void *stream);

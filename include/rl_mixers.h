@@ -161,8 +161,9 @@ int rl_attention_rows(rl_attention *attention, const rl_kv_cache *cache, const r
 /* The same where sequences share long beginnings, whose keys and values are then read
  * once for a group and not once for each sequence. The sequences group_starts[g] ..
  * group_starts[g + 1] (i32 [groups + 1], rising; what lies before the first or from the
- * last on has no prefix) have the same prefix_lens[g] tokens (i32, a negative one as 0) before their own, the t-th of them in
- * slot prefix_pages[g * prefix_width + t / page] * page + t % page. lens and pages are
+ * last on has no prefix) have the same prefix_lens[g] tokens (i32, a negative one as 0)
+ * before their own, the t-th of them in slot
+ * prefix_pages[g * prefix_width + t / page] * page + t % page. lens and pages are
  * those of their own tokens, which begin a page: every row sees its whole prefix and its
  * own sequence's tokens up to its own, as above without a window. max_prefix bounds the
  * tokens of any one prefix (0: the handle's max_len); past it the rows of the group are
@@ -216,7 +217,8 @@ int rl_delta_rows(rl_delta *delta, const rl_heads *q, const rl_heads *k, const r
  * Every channel's row is the sum of its last `width` rows:
  *   y[t][c] = act(bias[c] + sum_j weight[c][j] x[t - width + 1 + j][c])
  * with act(y) = y or y / (1 + e^-y). The width - 1 rows before a sequence's first are
- * its state, as they came in. Sums are f32, rounded once to the output's type. */
+ * its state, as they came in. Sums are f32, rounded once to the output's type; below
+ * 2^-119 an activated one may be 0. */
 enum { RL_CONV_PLAIN = 0, RL_CONV_SILU = 1 };
 
 typedef struct rl_conv rl_conv;
@@ -251,8 +253,8 @@ typedef struct rl_scan rl_scan;
 /* a [channels][state_dim] (negative in use), skip and dt_bias [channels] (or NULL:
  * zeros) f32 on the host, copied. state_dim 4 to 256, a multiple of 4; channels a
  * multiple of groups, at most 2^20. Workspace for calls of up to max_rows tokens in up to
- * max_seqs sequences: at most 34 MB and four states (rounded up to
- * whole workgroups). */
+ * max_seqs sequences, beside the copies of a, skip and dt_bias: at most 37 MB and four
+ * states, each group's channels rounded up to whole workgroups (16 to 256 of them). */
 int rl_scan_create(int device, uint32_t max_rows, uint32_t max_seqs, uint32_t channels, uint32_t groups,
                    uint32_t state_dim, const float *a, const float *skip, const float *dt_bias, rl_scan **out);
 void rl_scan_destroy(rl_scan *scan);

@@ -13,12 +13,19 @@
 // in step). Their sums are added at the end. Every row sees the whole prefix, so only
 // the last tile has a mask.
 //
-// Bound by instructions: on a SIMD matrix and vector instructions of two waves take
-// nearly the sum of their times (8 products and 32 sums 257 cycles, alone 164 and 190),
-// and a tile of 64 tokens and 32 rows of 128 bf16 is 96 products of 16 cycles and about
-// 400 vector instructions of 4 or 5. 256 rows a key-value head, 8 heads of 128, 16384
-// tokens bf16: 46.9 us, 366 TFLOP/s (k_attend 106 us). 640 rows, 8001 tokens int8 in
-// pages of 24, and two prefixes of a half and a third: 116 us, 332 TFLOP/s.
+// Bound in the tiles by instructions, which two waves on a SIMD pass with some overlap
+// only (8 products and 32 sums take 257 cycles, alone 164 and 190): a tile of 64 tokens
+// and 32 rows of 128 bf16 is 96 products of 16 cycles and 480 vector instructions a
+// wave. Beside the tiles by the start and the end of a workgroup, the one a CU holds:
+// the chain of pages, queries and the first tile, and the sums by way of LDS.
+// 256 rows a key-value head, 8 heads of 128, 16384 tokens bf16: 48 us, 358 TFLOP/s
+// (k_attend 106 us). Its 256 workgroups have 16 tiles of 1.41 us each (in 8, 4, 2 and 1
+// parts 69, 114, 204 and 385 us), which leaves 25 for start and end. Over the whole, waves
+// issue 35 % of their time, 20 % they wait for a unit and 46 % for loads, LDS and each
+// other; matrix units are busy 28 %, vector units 42 %. 640 rows, 8001 tokens int8 in
+// pages of 24, and two prefixes of a half and a third: 115 us, 335 TFLOP/s, two rounds of
+// workgroups of 21 tiles, 1.6 us each, and 25 for start and end. f32 queries, in two or
+// three parts: the first call 78 us, over f16 62, the second 203.
 #pragma once
 #include "attend.h"
 

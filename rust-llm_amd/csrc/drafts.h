@@ -6,7 +6,7 @@
 // arrive finds the chunk that the draw falls into and goes through it once more. Sums
 // are f64 (products and differences of f32 values are exact there, or nearly), and their
 // order does not depend on how workgroups arrive. Bound by HBM for many sequences, one
-// row of each side: 64 of 248320 tokens 28.0 us, 4.5 TB/s. For few by the chain of loads
+// row of each side: 64 of 248320 tokens 29 us, 4.4 TB/s. For few by the chain of loads
 // (starts, drafted token, two gathers, a chunk, the arrival, the chunk sums, a chunk
 // again): 9.4 us for one of 151936. Lists: a workgroup a sequence, the same chain without
 // the arrival, 7.8 us for 64 of up to 8 drafts and 64 entries.

@@ -55,7 +55,7 @@ __device__ inline float scan_step(const ScanArgs &a, T dt, float bias) {
 
 // Single tokens and short runs. L lanes hold a channel, four state values each, so
 // states move as whole vectors. Bound by HBM, the state in and out: 64 sequences of
-// 5120 channels of 16 take 10.8 us, 3.9 TB/s.
+// 5120 channels of 16 take 13.0 us over inputs that change, 3.4 TB/s.
 template <typename T, int L>
 __global__ void __launch_bounds__(SCAN_THREADS) k_scan_steps(ScanArgs a) {
     const uint32_t s = blockIdx.x / a.columns, column = blockIdx.x - s * a.columns, lane = threadIdx.x % 64;
@@ -108,12 +108,15 @@ __global__ void __launch_bounds__(SCAN_THREADS) k_scan_steps(ScanArgs a) {
 // sums are formed once for S of them. A workgroup takes 256 / L channels of a group
 // through a piece of one sequence; b and c of the next tokens are staged in LDS in f32
 // and read by all. Where a call has too few channels to fill the device its sequences
-// go in pieces: PIECE_ENDS leaves what each but the last does to a state of zeros,
+// go in pieces: SCAN_ENDS leaves what each but the last does to a state of zeros,
 // and the pass with the outputs makes each piece's first state of those before it.
-// Bound by instructions: an exponential (8.7 cycles a wave) and three or four products
-// (4.7) a token, channel, state value and pass, of which 8192 tokens of 5120 channels of
-// 16 have 97 and 116 us in the two passes; the whole call takes 306, that of 24
-// prompts of up to 701 tokens, 1536 channels of 32 in f32, 131.
+// Bound by instructions: while a CU has waves its vector units issue without a pause.
+// A wave's instruction takes them 4 cycles, an exponential 8. 8192 tokens of 5120
+// channels of 16: 64 and 90 million instructions in the two passes and 12 and 15 million
+// exponentials and logarithms among them, 140 and 201 us at 2.1 GHz. A token, channel
+// and state value has 5 or 6 of these slots, two thirds of all; the others are softplus,
+// gates, sums and loads. 24 prompts of up to 701 tokens, 1536 channels of 32 in f32:
+// 59 and 88 us, of which instructions 46 and 68; CUs that are done wait for the last.
 enum ScanPass { SCAN_ENDS, SCAN_OUTPUTS };
 
 template <typename T, int S, int L, ScanPass PASS>
